@@ -518,6 +518,68 @@ int lutb_peer_barrier(int32_t n_ranks, int32_t rank, void *const *flags, uint64_
 int lutb_peer_sgd_update(int32_t n_ranks, int32_t rank, const float *const *grads, float *const *weights,
                          int64_t begin, int64_t end, float scale, void *stream);
 
+/*
+ * ---------------------------------------------------------------- what joins blocks in the residual stream
+ * No counterpart in the reference, which composes torch modules here (dropout, BatchNorm1d, the sum; LUTTransformer.forward,
+ * src/spiky/lut/LUTTransformer.py).  Arrays are contiguous, rows of `width` elements, and aligned to their elements (rows of a
+ * multiple of eight elements in 16-byte aligned arrays take wide accesses).  Outputs overlap no input.
+ */
+#define LUTB_F32 0 /* element types */
+#define LUTB_BF16 1
+#define LUTB_F16 2
+#define LUTB_NORM_NONE 0
+#define LUTB_NORM_RMS 1   /* x / sqrt(mean(x^2) + eps) */
+#define LUTB_NORM_LAYER 2 /* (x - mean) / sqrt(mean((x - mean)^2) + eps) */
+
+/*
+ * Dropout without a stored mask: y[i] = x[i] * 2^32 / (2^32 - T) or 0 where element i is dropped, T = round(p * 2^32); a dropped
+ * element is 0 whatever it was.  The backward pass is the same call on the output's gradient.
+ *   random  int64 [2] on the device: seed and offset, read when the kernel runs; site is added to the offset
+ * Element i takes the 16-bit digit i % 8 (low halves first) of the Philox4x32-10 block with the key `seed` and the counter
+ * (i / 8, offset + site), 64 bits each, and a second digit from the same counter with bit 63 of its first half set; it is dropped
+ * when first * 2^16 + second < T.  y may be x.
+ */
+int lutb_dropout(int type, int64_t n, double p, const int64_t *random, int64_t site, const void *x, void *y, void *stream);
+
+/* used = state, then the state's offset grows by count; one launch, so that replayed graphs move on. */
+int lutb_dropout_advance(int64_t *state, int64_t count, int64_t *used, void *stream);
+
+typedef struct lutb_join_cfg {
+    int64_t rows, width;
+    int64_t gate_rows;   /* rows that share a gate row: 0 no gate, 1 a gate for each element, rows one gate row for all */
+    int64_t site;        /* of the dropout */
+    double dropout;      /* probability */
+    int32_t stream_type; /* x, h, dh, dx */
+    int32_t branch_type; /* f, y, dy, df: the stream's type, or any with a float32 stream */
+    int32_t param_type;  /* norm weights and biases and their gradients: float32 or the branch's type */
+    int32_t gate_type;   /* gate and dgate: float32 or the branch's type */
+    int32_t after;       /* norm of the branch, LUTB_NORM_* */
+    int32_t before;      /* norm of the new stream, for the next block */
+    float eps;           /* of both norms, positive */
+    float skip_scale, branch_scale;
+    int32_t reserved0;
+} lutb_join_cfg;
+
+/*
+ * h = skip_scale x + branch_scale gate * N_after(drop(f)), y = N_before(h); N is the norm times a weight plus a bias (NULL: 1, 0).
+ * y is formed from h before its rounding.  With f == NULL (then h, gate and the parameters of N_after are NULL and dropout is 0)
+ * y = N_before(x): the norm before a block alone.  stats: float [rows][4], what the backward pass needs; NULL to leave it out.
+ */
+int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const void *f, const void *gate, const void *after_weight,
+                      const void *after_bias, const void *before_weight, const void *before_bias, const int64_t *random,
+                      void *h, void *y, float *stats, void *stream);
+
+/*
+ * Gradients of the above from dh and dy (one of them may be NULL: zeros); each output may be NULL.  random, site and dropout are
+ * the forward call's, and so are stats.  Sums over rows (of the parameters, and of a gate row that several rows share) are taken
+ * in float32 in an order that does not change from call to call.  The workspace is 16-byte aligned, not kept between calls.
+ */
+size_t lutb_join_backward_workspace(const lutb_join_cfg *cfg);
+int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const void *f, const void *gate, const void *after_weight,
+                       const void *after_bias, const void *before_weight, const int64_t *random, const float *stats,
+                       const void *dh, const void *dy, void *dx, void *df, void *dgate, void *d_after_weight, void *d_after_bias,
+                       void *d_before_weight, void *d_before_bias, void *workspace, size_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -20,6 +20,9 @@ PRODUCT_KEEP_HIST, PRODUCT_REUSE_HIST = 0x100, 0x200   # flags or'ed into the va
 INT8_DEQUANT_F32, INT8_DEQUANT_EXACT = 0, 1
 # kernel family of the sparse forward / input-gradient passes (include/spiky_b200.h)
 SPARSE_AUTO, SPARSE_GATHER, SPARSE_STAGED = 0, 1, 2
+# element types and norms of the residual-stream operators (include/spiky_b200.h)
+F32, BF16, F16 = 0, 1, 2
+NORM_NONE, NORM_RMS, NORM_LAYER = 0, 1, 2
 
 
 class LayerCfg(ctypes.Structure):
@@ -64,6 +67,28 @@ class SparseIndexC(ctypes.Structure):
     ]
 
 
+class JoinCfg(ctypes.Structure):
+    """Mirror of ``lutb_join_cfg``."""
+
+    _fields_ = [
+        ("rows", ctypes.c_int64),
+        ("width", ctypes.c_int64),
+        ("gate_rows", ctypes.c_int64),
+        ("site", ctypes.c_int64),
+        ("dropout", ctypes.c_double),
+        ("stream_type", ctypes.c_int32),
+        ("branch_type", ctypes.c_int32),
+        ("param_type", ctypes.c_int32),
+        ("gate_type", ctypes.c_int32),
+        ("after", ctypes.c_int32),
+        ("before", ctypes.c_int32),
+        ("eps", ctypes.c_float),
+        ("skip_scale", ctypes.c_float),
+        ("branch_scale", ctypes.c_float),
+        ("reserved0", ctypes.c_int32),
+    ]
+
+
 _vp = ctypes.c_void_p
 _i64 = ctypes.c_int64
 _int = ctypes.c_int
@@ -71,6 +96,7 @@ _dbl = ctypes.c_double
 _size = ctypes.c_size_t
 _cfgp = ctypes.POINTER(LayerCfg)
 _spp = ctypes.POINTER(SparseIndexC)
+_joinp = ctypes.POINTER(JoinCfg)
 
 # name -> (restype, argtypes); every symbol include/spiky_b200.h declares is listed here
 SIGNATURES = {
@@ -130,6 +156,11 @@ SIGNATURES = {
                                     ctypes.c_float, _vp]),
     "lutb_nonseq_sparse_forward": (_int, [_cfgp, _spp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "lutb_nonseq_sparse_backward": (_int, [_cfgp, _spp, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _dbl, _vp]),
+    "lutb_dropout": (_int, [_int, _i64, _dbl, _vp, _i64, _vp, _vp, _vp]),
+    "lutb_dropout_advance": (_int, [_vp, _i64, _vp, _vp]),
+    "lutb_join_forward": (_int, [_joinp] + [_vp] * 12),
+    "lutb_join_backward_workspace": (_size, [_joinp]),
+    "lutb_join_backward": (_int, [_joinp] + [_vp] * 18 + [_size, _vp]),
     "lutb_nonseq_sparse_table_grad": (_int, [_cfgp, _spp, _i64, _vp, _vp, _int, _vp, _dbl, _i64, _i64, _vp]),
 }
 

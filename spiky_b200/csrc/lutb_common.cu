@@ -135,7 +135,7 @@ static const char *const kKernelNames[K_COUNT] = {
     "check_positional", "concat_forward", "concat_backward", "concat_weight_update",
     "int8_gather",
     "product_hist", "product_hist_forward", "product_row_dots", "product_route", "product_hist_weight_grad",
-    "dense_to_sparse", "fp32_gemm", "peer_sgd_update", "peer_barrier", "peer_broadcast", "zero_buffers",
+    "dense_to_sparse", "fp32_gemm", "peer_sgd_update", "peer_barrier", "peer_broadcast", "zero_buffers", "dropout", "join_forward", "join_backward", "join_sums",
 };
 
 struct EventPair {

@@ -97,6 +97,10 @@ enum KernelId {
     K_PEER_BARRIER,
     K_PEER_BROADCAST,
     K_ZERO_BUFFERS,
+    K_DROPOUT,
+    K_JOIN_FORWARD,
+    K_JOIN_BACKWARD,
+    K_JOIN_SUMS,
     K_COUNT
 };
 
