@@ -5,12 +5,19 @@ Same constructor arguments, attribute names and forward contract as the referenc
 ``num_layers`` blocks of [LUT attention over the whole context -> dropout -> (BatchNorm1d) -> residual,
 LUT feed-forward on every token -> dropout -> (BatchNorm1d) -> residual], then a LUT unembedder to the
 vocabulary.  ``forward(tokens[B, S]) -> logits[B, S, V]``.
+
+Beyond the reference: ``norm`` ('rms' or 'layer') puts a norm of each token before every block and before the unembedder,
+``norm_after`` one after every block, ``gated`` a learned gate row on every block's output, ``skip_scale`` and ``branch_scale`` scale the two
+parts of every residual sum, and ``counter_dropout`` draws the dropout masks from (``dropout_seed``, a buffer that counts training
+passes) instead of storing them.  Each block is then joined to the stream, with the next block's norm, in one kernel
+(:mod:`spiky_b200.residual`).
 """
 import torch
 import torch.nn as nn
 
 from .lut_layer import (Conv2DLUTLayer, GradientPolicy, GradientType, LUTLayer, LUTSharedContext,  # noqa: F401
                         SynapseMeta, _normalise_device)
+from .residual import ResidualJoin, RowNorm, counter_dropout as _counter_dropout, dropout_state, take_dropout_state
 
 
 class LUTTransformer(nn.Module):
@@ -19,8 +26,18 @@ class LUTTransformer(nn.Module):
                  concatenation_product=True, sliced_product_mode=False, unified_pe=False, do_normalise_weights=False,
                  weights_gradient_policy=None, device=None, synapse_meta=SynapseMeta(), lut_shared_context=None,
                  seed=None, summation_dtype=torch.float32, _int_rescaler=0.001, _forward_group_size=32,
-                 _backward_group_size=32, dropout=0.0, use_batch_norm=False):
+                 _backward_group_size=32, dropout=0.0, use_batch_norm=False, norm=None, norm_after=False, gated=False, skip_scale=1.0,
+                 branch_scale=1.0, counter_dropout=False, dropout_seed=None):
         super().__init__()
+        if norm not in (None, "rms", "layer"):
+            raise ValueError("norm is None, 'rms' or 'layer'")
+        if norm_after and norm is None:
+            raise ValueError("norm_after needs norm")
+        shaped = norm is not None or gated or skip_scale != 1.0 or branch_scale != 1.0
+        if use_batch_norm and shaped:
+            raise ValueError("use_batch_norm goes without norm, gated, skip_scale and branch_scale")
+        if dropout_seed is not None and not counter_dropout:
+            raise ValueError("dropout_seed is the seed of counter_dropout")
         self.vocab_size = vocab_size
         self.embedding_dim = embedding_dim
         self.context_size = context_size
@@ -37,6 +54,8 @@ class LUTTransformer(nn.Module):
         self.weights_gradient_policy = weights_gradient_policy
         self.dropout = dropout
         self.use_batch_norm = use_batch_norm
+        self.norm, self.norm_after, self.gated, self.counter_dropout = norm, norm_after, gated, counter_dropout
+        self._joined = shaped or (counter_dropout and not use_batch_norm)
         self.unified_pe = unified_pe
         self.no_ffn = no_ffn
         self.device = torch.device("cpu") if device is None else _normalise_device(device)
@@ -82,6 +101,18 @@ class LUTTransformer(nn.Module):
                                   output_kernel_shape=embedding_dim, receptive_field_shape=embedding_dim,
                                   receptive_field_stride_shape=embedding_dim, **seq)
 
+        def join():
+            return ResidualJoin(n_emb, branch_norm=norm if norm_after else None, next_norm=norm, gated=gated, skip_scale=skip_scale,
+                                branch_scale=branch_scale, dropout=dropout if counter_dropout else 0.0, device=self.device)
+
+        self._n_dropouts = num_layers * (1 if no_ffn else 2)
+        if counter_dropout:
+            if dropout_seed is None:
+                dropout_seed = int(torch.randint(2 ** 62, (1,))) if seed is None else seed
+            self.register_buffer("dropout_state", dropout_state(dropout_seed, self.device))
+        if norm is not None:
+            self.first_norm = RowNorm(n_emb, norm, device=self.device)
+
         self.layers = nn.ModuleList()
         for li in range(num_layers):
             block = nn.ModuleDict()
@@ -93,6 +124,10 @@ class LUTTransformer(nn.Module):
                 block["ffn"] = per_token_lut(n_emb, None if seed is None else base + num_heads)
                 block["ffn_dropout"] = nn.Dropout(dropout)
                 block["ffn_bn"] = nn.BatchNorm1d(n_emb, device=self.device) if use_batch_norm else None
+            if self._joined:
+                block["attention_join"] = join()
+                if not no_ffn:
+                    block["ffn_join"] = join()
             self.layers.append(block)
         self.unembedder = per_token_lut(vocab_size, seed)
 
@@ -131,12 +166,23 @@ class LUTTransformer(nn.Module):
                 layer.to(device=dev)
         return self
 
-    @staticmethod
-    def _residual_branch(z, out, dropout, bn):
-        out = dropout(out)
+    def _residual_branch(self, z, out, dropout, bn, state, site):
+        if not self.counter_dropout:
+            out = dropout(out)
+        elif state is not None:
+            out = _counter_dropout(out, self.dropout, state, site)
         if bn is not None:
             out = bn(out.reshape(-1, out.shape[-1])).reshape(out.shape)
         return z + out
+
+    def _add(self, z, out, block, part, state, site):
+        """The stream with a block's output, and what the next block reads of it."""
+        if not self._joined:
+            z = self._residual_branch(z, out, block[part + "_dropout"], block[part + "_bn"], state, site)
+            return z, z
+        if not self.counter_dropout:
+            out = block[part + "_dropout"](out)
+        return block[part + "_join"](z, out, state, site)
 
     # ------------------------------------------------------------------ forward
     def forward(self, tokens):
@@ -149,18 +195,25 @@ class LUTTransformer(nn.Module):
         if record:
             self._debug_last_forward.append(z.detach().clone())
         flat = isinstance(self.embedding_dim, int)
+        state = None   # of this pass's dropouts, each with a site of its own
+        if self.counter_dropout and self.training and self.dropout > 0.0:
+            state = take_dropout_state(self.dropout_state, self._n_dropouts)
+        site = 0
+        y = z if self.norm is None else self.first_norm(z)
         for block in self.layers:
-            att_in = z if flat else z.reshape((B, S) + tuple(self.embedding_dim))
+            att_in = y if flat else y.reshape((B, S) + tuple(self.embedding_dim))
             att = block["attention_lut"](att_in.contiguous()).reshape(B, S, E)
             if record:
                 self._debug_last_forward.append(att.detach().clone())
-            z = self._residual_branch(z, att, block["attention_dropout"], block["attention_bn"])
+            z, y = self._add(z, att, block, "attention", state, site)
+            site += 1
             if not self.no_ffn:
-                ffn = block["ffn"](z.reshape(B * S, 1, E)).reshape(B, S, E)
+                ffn = block["ffn"](y.reshape(B * S, 1, E)).reshape(B, S, E)
                 if record:
                     self._debug_last_forward.append(ffn.detach().clone())
-                z = self._residual_branch(z, ffn, block["ffn_dropout"], block["ffn_bn"])
-        return self.unembedder(z.reshape(B * S, 1, E)).reshape(B, S, self.vocab_size)
+                z, y = self._add(z, ffn, block, "ffn", state, site)
+                site += 1
+        return self.unembedder(y.reshape(B * S, 1, E)).reshape(B, S, self.vocab_size)
 
     def get_profile_statistics(self) -> str:
         """Kernel timings collected by the opt-in profiler of the CUDA library, one line per kernel family."""
