@@ -1,7 +1,7 @@
 // Dropout whose mask is a function of (seed, offset, element) and is never stored: the backward pass forms it again.
 #include <math.h>
 
-#include "residual.cuh"
+#include "residual_rows.cuh"
 
 namespace lutb {
 
@@ -18,17 +18,40 @@ DropRule drop_rule(double p) {
     return r;
 }
 
-// A thread takes the eight elements of a generator block.
-template <class T>
-__global__ void __launch_bounds__(256) dropout_kernel(int64_t n, const T *x, T *y, const int64_t *random, uint64_t site, const DropRule rule) {
+// A thread takes the eight elements of a generator block, two such blocks (VEC) side by side: their rounds are independent and share the
+// keys.  VEC: whole blocks in 16-byte aligned arrays; the others element by element.
+template <class T, bool VEC>
+__global__ void __launch_bounds__(256) dropout_kernel(int64_t first, int64_t n, const T *x, T *y, const int64_t *random, uint64_t site, const DropRule rule) {
     const DropKey key = drop_key(random, site);
-    const int64_t blocks = (n + 7) / 8;
-    for (int64_t b = blockIdx.x * 256ll + threadIdx.x; b < blocks; b += gridDim.x * 256ll) {
-        const uint32_t kept = keep_bits((uint64_t)b, key, rule);
+    if constexpr (VEC) {
+        constexpr int kSide = 2;
+        for (int64_t b = blockIdx.x * (256ll * kSide) + threadIdx.x; 8 * b < n; b += gridDim.x * (256ll * kSide)) {
+            uint4 in[kSide][kParts<T>];
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int64_t i = 8 * b + j;
-            if (i < n) y[i] = from_f32<T>((kept >> j & 1) ? to_f32(x[i]) * rule.scale : 0.0f);
+            for (int k = 0; k < kSide; k++)
+#pragma unroll
+                for (int q = 0; q < kParts<T>; q++)
+                    if (8 * (b + 256 * k) < n) in[k][q] = reinterpret_cast<const uint4 *>(x + 8 * (b + 256 * k))[q];
+            uint32_t kept[kSide];
+#pragma unroll
+            for (int k = 0; k < kSide; k++) kept[k] = keep_bits((uint64_t)(b + 256 * k), key, rule);
+#pragma unroll
+            for (int k = 0; k < kSide; k++) {
+                if (8 * (b + 256 * k) >= n) break;
+                float2 v[4];
+                unpack8<T>(in[k], v);
+                drop8(v, kept[k], rule.scale);
+                store8(y + 8 * (b + 256 * k), v);
+            }
+        }
+    } else {
+        for (int64_t b = first / 8 + blockIdx.x * 256ll + threadIdx.x; 8 * b < n; b += gridDim.x * 256ll) {
+            const uint32_t kept = keep_bits((uint64_t)b, key, rule);
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int64_t i = 8 * b + j;
+                if (i < n) y[i] = from_f32<T>((kept >> j & 1) ? to_f32(x[i]) * rule.scale : 0.0f);
+            }
         }
     }
 }
@@ -42,10 +65,22 @@ __global__ void dropout_advance_kernel(int64_t *state, int64_t count, int64_t *u
 
 template <class T>
 static int launch_dropout(int64_t n, const void *x, void *y, const int64_t *random, uint64_t site, const DropRule &rule, cudaStream_t stream) {
-    const int64_t blocks = ((n + 7) / 8 + 255) / 256, cap = (int64_t)device_info().sm_count * 8;
-    KernelScope scope(K_DROPOUT, stream);
-    dropout_kernel<T><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, stream>>>(n, static_cast<const T *>(x), static_cast<T *>(y), random, site, rule);
-    LUTB_LAUNCH_CHECK();
+    const T *from = static_cast<const T *>(x);
+    T *to = static_cast<T *>(y);
+    const bool vec = (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % 16 == 0;
+    const int64_t whole = vec ? n / 8 * 8 : 0, cap = (int64_t)device_info().sm_count * 8;
+    if (whole) {
+        const int64_t blocks = (whole / 8 + 511) / 512;
+        KernelScope scope(K_DROPOUT, stream);
+        dropout_kernel<T, true><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, stream>>>(0, whole, from, to, random, site, rule);
+        LUTB_LAUNCH_CHECK();
+    }
+    if (whole < n) {
+        const int64_t blocks = ((n - whole + 7) / 8 + 255) / 256;
+        KernelScope scope(K_DROPOUT, stream);
+        dropout_kernel<T, false><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, stream>>>(whole, n, from, to, random, site, rule);
+        LUTB_LAUNCH_CHECK();
+    }
     return LUTB_OK;
 }
 

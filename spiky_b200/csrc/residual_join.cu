@@ -2,7 +2,7 @@
 // block, forward and backward; without a block the norm alone.
 #include <math.h>
 
-#include "residual_join.cuh"
+#include "residual_rows.cuh"
 
 namespace lutb {
 
@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(kRowThreads) join_forward_kernel(const JoinArg
     __shared__ float scratch[kRowThreads / 32];
     const DropKey key = a.drop.on ? drop_key(a.random, a.site) : DropKey{};
     const float width = (float)a.width;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+    for (int64_t row = blockIdx.x * a.chunk_rows, end = min(row + a.chunk_rows, a.rows); row < end; row++) {
         JoinRow<X, F> j(a, row);
         float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
         if (a.after != LUTB_NORM_NONE) {
@@ -188,7 +188,15 @@ __global__ void __launch_bounds__(kRowThreads) join_backward_kernel(const JoinAr
                     static_cast<F *>(a.df)[j.at + c] = from_f32<F>(k ? dt * (a.drop.on ? a.drop.scale : 1.0f) : 0.0f);
                 }
             });
-            __syncthreads();   // (another thread may have these columns in the next row)
+        }
+        if (gate_summed && a.gate_direct) {
+            for (int64_t c0 = threadIdx.x * 8ll; c0 < a.width; c0 += kRowThreads * 8ll)   // (this thread's columns)
+                for (int64_t c = c0; c < min(c0 + 8, a.width); c++) {
+                    if (a.gate_f32)
+                        static_cast<float *>(a.dgate)[group * a.width + c] = gate_sums[c];
+                    else
+                        static_cast<F *>(a.dgate)[group * a.width + c] = from_f32<F>(gate_sums[c]);
+                }
         }
     }
 }
@@ -224,16 +232,17 @@ __global__ void __launch_bounds__(1024) join_sums_kernel(const SumList l, int64_
     }
 }
 
-JoinSplit join_split(int64_t rows, int64_t group_rows, int64_t blocks_wanted) {
-    const int64_t groups = (rows + group_rows - 1) / group_rows;
+// `at_once`: rows that a block takes together.
+static JoinSplit join_split(int64_t rows, int64_t group_rows, int64_t blocks_wanted, int at_once) {
+    const int64_t groups = rows / group_rows;
     JoinSplit best{};
     int64_t best_rounds = INT64_MAX;
     for (int64_t turns = 1; turns <= 4; turns++) {   // chunks a block takes one after another
         int64_t k = turns * blocks_wanted / groups;
         k = k < 1 ? 1 : k > group_rows ? group_rows : k;
-        const int64_t chunk_rows = (group_rows + k - 1) / k;
+        const int64_t steps = ((group_rows + k - 1) / k + at_once - 1) / at_once, chunk_rows = steps * at_once;
         k = (group_rows + chunk_rows - 1) / chunk_rows;
-        const int64_t chunks = groups * k, rounds = (chunks + blocks_wanted - 1) / blocks_wanted * chunk_rows;
+        const int64_t chunks = groups * k, rounds = (chunks + blocks_wanted - 1) / blocks_wanted * steps;
         if (rounds < best_rounds) {
             best_rounds = rounds;
             best = {group_rows, k, chunk_rows, chunks, (int)(chunks < blocks_wanted ? chunks : blocks_wanted)};
@@ -242,10 +251,55 @@ JoinSplit join_split(int64_t rows, int64_t group_rows, int64_t blocks_wanted) {
     return best;
 }
 
+// Rows up to kRowMaxWidth have the row kernels, two blocks of 256 threads an SM (128 registers a thread, half of shared memory each).
 static JoinSplit split_of(const lutb_join_cfg *cfg, bool gate_gradient) {
     const bool summed = gate_gradient && cfg->gate_rows > 1;
-    const int sm = device_info().sm_count;   // (0 where there is no device: a size can be asked for all the same)
-    return join_split(cfg->rows, summed ? cfg->gate_rows : cfg->rows, (sm > 0 ? sm : 148) * 4ll);
+    const int have = device_info().sm_count, sm = have > 0 ? have : 148;   // (no device: a size can be asked for all the same)
+    const int64_t group_rows = summed ? cfg->gate_rows : cfg->rows;
+    if (cfg->width > kRowMaxWidth) return join_split(cfg->rows, group_rows, sm * 4ll, 1);
+    const RowShape s = row_shape(cfg->width);
+    return join_split(cfg->rows, group_rows, (int64_t)sm * (2 * kRowMaxThreads / s.threads) / s.cluster, s.teams);
+}
+static void take_split(JoinArgs &a, const JoinSplit &s) {
+    a.group_rows = s.group_rows;
+    a.per_group = s.per_group;
+    a.chunk_rows = s.chunk_rows;
+    a.chunks = s.chunks;
+}
+
+int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs &a, const RowShape &s, int clusters, size_t smem, cudaStream_t stream) {
+    if (smem > kPlainSmem - 12 * 1024) {   // (the kernels' own arrays take up to 11 KB)
+        const int device = device_info().device;
+        const uint32_t bit = device < 32 ? 1u << device : 0;
+        if (!(opted.load(std::memory_order_relaxed) & bit)) {
+            LUTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemPerBlock - 12 * 1024));
+            opted.fetch_or(bit, std::memory_order_relaxed);
+        }
+    }
+    JoinArgs args = a;
+    RowShape shape = s;
+    void *params[2] = {&args, &shape};
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)(clusters * s.cluster));
+    config.blockDim = dim3((unsigned)s.threads);
+    config.dynamicSmemBytes = smem;
+    config.stream = stream;
+    cudaLaunchAttribute attribute[1];
+    if (s.cluster > 1) {
+        attribute[0].id = cudaLaunchAttributeClusterDimension;
+        attribute[0].val.clusterDim.x = (unsigned)s.cluster;
+        attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+        config.attrs = attribute;
+        config.numAttrs = 1;
+    }
+    LUTB_CUDA(cudaLaunchKernelExC(&config, kernel, params));
+    return LUTB_OK;
+}
+
+static bool all_aligned16(std::initializer_list<const void *> list) {
+    uintptr_t all = 0;
+    for (const void *p : list) all |= reinterpret_cast<uintptr_t>(p);
+    return all % 16 == 0;
 }
 
 static int check_join(const lutb_join_cfg *c) {
@@ -319,12 +373,14 @@ extern "C" int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const 
     JoinArgs a = join_args(cfg);
     a.x = x; a.f = f; a.gate = gate; a.aw = after_weight; a.ab = after_bias; a.bw = before_weight; a.bb = before_bias;
     a.h = h; a.y = y; a.stats = reinterpret_cast<float4 *>(stats); a.random = random; a.gate_rows = cfg->gate_rows;
-    const int64_t cap = (int64_t)device_info().sm_count * 8;
-    const unsigned blocks = (unsigned)(a.rows < cap ? a.rows : cap);
+    const JoinSplit split = split_of(cfg, false);
+    take_split(a, split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    return by_types(cfg, [&](auto xt, auto ft) {
+    const bool vec = cfg->width % kRowElems == 0 && all_aligned16({x, f, gate, after_weight, after_bias, before_weight, before_bias, h, y});
+    return by_types(cfg, [&](auto xt, auto ft) -> int {
         KernelScope scope(K_JOIN_FORWARD, s);
-        join_forward_kernel<decltype(xt), decltype(ft)><<<blocks, kRowThreads, 0, s>>>(a);
+        if (cfg->width <= kRowMaxWidth) return join_rows<decltype(xt), decltype(ft)>(false, vec, a, row_shape(cfg->width), split.blocks, s);
+        join_forward_kernel<decltype(xt), decltype(ft)><<<split.blocks, kRowThreads, 0, s>>>(a);
         LUTB_LAUNCH_CHECK();
         return (int)LUTB_OK;
     });
@@ -374,7 +430,9 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     a.dh = dh; a.dy = dy; a.dx = dx; a.df = df; a.dgate = dgate;
     const bool gate_summed = dgate != nullptr && cfg->gate_rows > 1;
     const JoinSplit split = split_of(cfg, dgate != nullptr);
-    a.group_rows = split.group_rows; a.per_group = split.per_group; a.chunk_rows = split.chunk_rows; a.chunks = split.chunks;
+    take_split(a, split);
+    a.gate_direct = gate_summed && split.per_group == 1;
+    const bool gate_parts = gate_summed && !(a.gate_direct && cfg->width <= kRowMaxWidth);   // (the kernel for wide rows sums there in any case)
     SumList l{};
     float *at = static_cast<float *>(workspace);
     size_t need = 0;
@@ -385,7 +443,7 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
         l.count++;
         need += (size_t)split.blocks * cfg->width;
     }
-    if (gate_summed) {
+    if (gate_parts) {
         a.gate_sums = at + need;
         l.from[l.count] = a.gate_sums; l.to[l.count] = dgate; l.parts[l.count] = split.per_group; l.f32[l.count] = a.gate_f32;
         need += (size_t)split.chunks * cfg->width;
@@ -393,13 +451,19 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     LUTB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need * sizeof(float)), LUTB_ERR_WORKSPACE,
                  "workspace of %zu bytes needed", need * sizeof(float));
     LUTB_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, LUTB_ERR_ALIGN, "workspace must be 16-byte aligned");
-    return by_types(cfg, [&](auto xt, auto ft) {
+    const bool vec = cfg->width % kRowElems == 0 &&
+                     all_aligned16({x, f, gate, after_weight, after_bias, before_weight, dh, dy, dx, df, dgate});
+    return by_types(cfg, [&](auto xt, auto ft) -> int {
         {
             KernelScope scope(K_JOIN_BACKWARD, s);
-            join_backward_kernel<decltype(xt), decltype(ft)><<<split.blocks, kRowThreads, 0, s>>>(a);
-            LUTB_LAUNCH_CHECK();
+            if (cfg->width <= kRowMaxWidth) {
+                if (int rc = join_rows<decltype(xt), decltype(ft)>(true, vec, a, row_shape(cfg->width), split.blocks, s)) return rc;
+            } else {
+                join_backward_kernel<decltype(xt), decltype(ft)><<<split.blocks, kRowThreads, 0, s>>>(a);
+                LUTB_LAUNCH_CHECK();
+            }
         }
-        const int64_t out_rows = l.count + (gate_summed ? split.chunks / split.per_group : 0);
+        const int64_t out_rows = l.count + (gate_summed && !a.gate_direct ? split.chunks / split.per_group : 0);
         if (out_rows) {
             KernelScope scope(K_JOIN_SUMS, s);
             const dim3 grid((unsigned)((cfg->width + 31) / 32), (unsigned)out_rows);

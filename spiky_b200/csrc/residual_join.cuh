@@ -34,7 +34,6 @@ struct JoinSplit {
     int64_t group_rows, per_group, chunk_rows, chunks;
     int blocks;
 };
-JoinSplit join_split(int64_t rows, int64_t group_rows, int64_t blocks_wanted);
 
 template <class F>
 __device__ __forceinline__ float join_param(const void *p, bool f32, int64_t at, float none) {
