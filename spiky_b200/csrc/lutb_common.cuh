@@ -144,6 +144,8 @@ int peer_wait_errors(int *count_out);
 int contract_wait_errors(int *count_out);
 // The same of the staged inference kernel (infer_staged.cu).
 int staged_wait_errors(int *count_out);
+// The same of the residual joins' clusters (residual_rows.cuh).
+int join_wait_errors(int *count_out);
 
 // In-place conversion of int32 fixed-point accumulators to fp32
 // (reference: convert_integers_to_floats_logic, proto:200-213).

@@ -251,14 +251,46 @@ static JoinSplit join_split(int64_t rows, int64_t group_rows, int64_t blocks_wan
     return best;
 }
 
-// Rows up to kRowMaxWidth have the row kernels, two blocks of 256 threads an SM (128 registers a thread, half of shared memory each).
-static JoinSplit split_of(const lutb_join_cfg *cfg, bool gate_gradient) {
-    const bool summed = gate_gradient && cfg->gate_rows > 1;
+// fn(X{}, F{}) for the element types of the stream and the branch
+template <class Fn>
+static auto by_types(const lutb_join_cfg *c, Fn fn) {
+    if (c->branch_type == LUTB_BF16) return c->stream_type == LUTB_F32 ? fn(float(), __nv_bfloat16()) : fn(__nv_bfloat16(), __nv_bfloat16());
+    if (c->branch_type == LUTB_F16) return c->stream_type == LUTB_F32 ? fn(float(), __half()) : fn(__half(), __half());
+    return fn(float(), float());
+}
+
+constexpr size_t kForwardStatic = 10 * 1024, kBackwardStatic = 12 * 1024;   // the kernels' own arrays at most, and what a block takes beside them
+constexpr size_t kForwardVecStatic = 2 * 1024, kBackwardTeamStatic = 3 * 1024;
+
+// Gives the shape its stages (the most of three with which as many threads as registers allow are resident, 512 an SM or, forward, 384; the most that fit
+// otherwise) and returns how many blocks the device holds.
+static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, RowShape &s) {
     const int have = device_info().sm_count, sm = have > 0 ? have : 148;   // (no device: a size can be asked for all the same)
-    const int64_t group_rows = summed ? cfg->gate_rows : cfg->rows;
-    if (cfg->width > kRowMaxWidth) return join_split(cfg->rows, group_rows, sm * 4ll, 1);
-    const RowShape s = row_shape(cfg->width);
-    return join_split(cfg->rows, group_rows, (int64_t)sm * (2 * kRowMaxThreads / s.threads) / s.cluster, s.teams);
+    const size_t own = backward ? (s.kind == TEAM_WARP ? kBackwardStatic : kBackwardTeamStatic) : vec ? kForwardVecStatic : kForwardStatic;
+    const int most = 512 / s.threads, wanted = backward ? most : 384 / s.threads > 1 ? 384 / s.threads : 1;
+    int blocks = 1;
+    for (s.stages = 3; s.stages >= 1; s.stages--) {
+        const size_t dynamic = by_types(cfg, [&](auto xt, auto ft) { return join_rows_smem<decltype(xt), decltype(ft)>(backward, vec, s, cfg->gate_rows == 1); });
+        blocks = dynamic > kMaxSmemPerBlock - kBackwardStatic ? 0 : (int)(kMaxSmemPerBlock / (dynamic + own));
+        if (blocks >= wanted || (s.stages == 2 && blocks >= 1) || s.stages == 1) break;
+    }
+    return (int64_t)sm * (blocks < 1 ? 1 : blocks < most ? blocks : most);
+}
+// How the rows are dealt, and to what shape of block (rows up to kRowMaxWidth have the row kernels).
+static JoinSplit split_forward(const lutb_join_cfg *cfg, bool vec, RowShape &s) {
+    const int have = device_info().sm_count;
+    if (cfg->width > kRowMaxWidth) return join_split(cfg->rows, cfg->rows, (have > 0 ? have : 148) * 8ll, 1);
+    s = forward_shape(cfg->width, vec);
+    const int64_t blocks = resident(cfg, false, vec, s);
+    return join_split(cfg->rows, cfg->rows, blocks, s.teams);
+}
+static JoinSplit split_backward(const lutb_join_cfg *cfg, bool gate_gradient, RowShape &s) {
+    const int64_t group_rows = gate_gradient && cfg->gate_rows > 1 ? cfg->gate_rows : cfg->rows;
+    const int have = device_info().sm_count;
+    if (cfg->width > kRowMaxWidth) return join_split(cfg->rows, group_rows, (have > 0 ? have : 148) * 4ll, 1);
+    s = backward_shape(cfg->width);
+    const int64_t blocks = resident(cfg, true, true, s);
+    return join_split(cfg->rows, group_rows, blocks / s.cluster, s.teams);
 }
 static void take_split(JoinArgs &a, const JoinSplit &s) {
     a.group_rows = s.group_rows;
@@ -268,11 +300,11 @@ static void take_split(JoinArgs &a, const JoinSplit &s) {
 }
 
 int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs &a, const RowShape &s, int clusters, size_t smem, cudaStream_t stream) {
-    if (smem > kPlainSmem - 12 * 1024) {   // (the kernels' own arrays take up to 11 KB)
+    if (smem > kPlainSmem - kBackwardStatic) {
         const int device = device_info().device;
         const uint32_t bit = device < 32 ? 1u << device : 0;
         if (!(opted.load(std::memory_order_relaxed) & bit)) {
-            LUTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemPerBlock - 12 * 1024));
+            LUTB_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemPerBlock - kBackwardStatic));
             opted.fetch_or(bit, std::memory_order_relaxed);
         }
     }
@@ -341,12 +373,16 @@ static JoinArgs join_args(const lutb_join_cfg *c) {
     return a;
 }
 
-// fn(X{}, F{}) for the element types of the stream and the branch
-template <class Fn>
-static int by_types(const lutb_join_cfg *c, Fn fn) {
-    if (c->branch_type == LUTB_BF16) return c->stream_type == LUTB_F32 ? fn(float(), __nv_bfloat16()) : fn(__nv_bfloat16(), __nv_bfloat16());
-    if (c->branch_type == LUTB_F16) return c->stream_type == LUTB_F32 ? fn(float(), __half()) : fn(__half(), __half());
-    return fn(float(), float());
+int join_wait_errors(int *count_out) {
+    int all = 0, one = 0;
+    int (*const each[5])(int *) = {join_rows_wait_errors<float, float>, join_rows_wait_errors<__nv_bfloat16, __nv_bfloat16>,
+                                   join_rows_wait_errors<__half, __half>, join_rows_wait_errors<float, __nv_bfloat16>, join_rows_wait_errors<float, __half>};
+    for (auto read : each) {
+        if (int rc = read(&one)) return rc;
+        all += one;
+    }
+    *count_out = all;
+    return LUTB_OK;
 }
 
 }  // namespace lutb
@@ -373,13 +409,14 @@ extern "C" int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const 
     JoinArgs a = join_args(cfg);
     a.x = x; a.f = f; a.gate = gate; a.aw = after_weight; a.ab = after_bias; a.bw = before_weight; a.bb = before_bias;
     a.h = h; a.y = y; a.stats = reinterpret_cast<float4 *>(stats); a.random = random; a.gate_rows = cfg->gate_rows;
-    const JoinSplit split = split_of(cfg, false);
+    const bool vec = cfg->width % kRowElems == 0 && all_aligned16({x, f, gate, after_weight, after_bias, before_weight, before_bias, h, y});
+    RowShape shape{};
+    const JoinSplit split = split_forward(cfg, vec, shape);
     take_split(a, split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
-    const bool vec = cfg->width % kRowElems == 0 && all_aligned16({x, f, gate, after_weight, after_bias, before_weight, before_bias, h, y});
     return by_types(cfg, [&](auto xt, auto ft) -> int {
         KernelScope scope(K_JOIN_FORWARD, s);
-        if (cfg->width <= kRowMaxWidth) return join_rows<decltype(xt), decltype(ft)>(false, vec, a, row_shape(cfg->width), split.blocks, s);
+        if (cfg->width <= kRowMaxWidth) return join_rows<decltype(xt), decltype(ft)>(false, vec, a, shape, split.blocks, s);
         join_forward_kernel<decltype(xt), decltype(ft)><<<split.blocks, kRowThreads, 0, s>>>(a);
         LUTB_LAUNCH_CHECK();
         return (int)LUTB_OK;
@@ -389,7 +426,8 @@ extern "C" int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const 
 extern "C" size_t lutb_join_backward_workspace(const lutb_join_cfg *cfg) {
     using namespace lutb;
     if (check_join(cfg) || cfg->rows == 0) return 0;
-    const JoinSplit plain = split_of(cfg, false), gated = split_of(cfg, true);
+    RowShape shape{};
+    const JoinSplit plain = split_backward(cfg, false, shape), gated = split_backward(cfg, true, shape);
     const int64_t blocks = plain.blocks > gated.blocks ? plain.blocks : gated.blocks;
     return (size_t)((4 * blocks + (cfg->gate_rows > 1 ? gated.chunks : 0)) * cfg->width) * sizeof(float);
 }
@@ -429,7 +467,8 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     a.stats = reinterpret_cast<float4 *>(const_cast<float *>(stats)); a.random = random;
     a.dh = dh; a.dy = dy; a.dx = dx; a.df = df; a.dgate = dgate;
     const bool gate_summed = dgate != nullptr && cfg->gate_rows > 1;
-    const JoinSplit split = split_of(cfg, dgate != nullptr);
+    RowShape shape{};
+    const JoinSplit split = split_backward(cfg, dgate != nullptr, shape);
     take_split(a, split);
     a.gate_direct = gate_summed && split.per_group == 1;
     const bool gate_parts = gate_summed && !(a.gate_direct && cfg->width <= kRowMaxWidth);   // (the kernel for wide rows sums there in any case)
@@ -457,7 +496,7 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
         {
             KernelScope scope(K_JOIN_BACKWARD, s);
             if (cfg->width <= kRowMaxWidth) {
-                if (int rc = join_rows<decltype(xt), decltype(ft)>(true, vec, a, row_shape(cfg->width), split.blocks, s)) return rc;
+                if (int rc = join_rows<decltype(xt), decltype(ft)>(true, vec, a, shape, split.blocks, s)) return rc;
             } else {
                 join_backward_kernel<decltype(xt), decltype(ft)><<<split.blocks, kRowThreads, 0, s>>>(a);
                 LUTB_LAUNCH_CHECK();

@@ -1,44 +1,68 @@
 // Row kernels of the residual joins: a row's elements stay in registers from the first sum to the last store.
 //
-// A thread has eight elements of a row.  A team of threads has a row: a part of a warp up to 256 elements, a block up to 2048, a cluster of up
-// to eight blocks up to 16384; sums over a row go through shuffles, shared memory and the cluster's shared memory accordingly, one
-// exchange for each norm and direction (a norm's mean and squares are combined from the warps' own by the pairwise formula of Chan, Golub
-// and LeVeque, 1979, so that no square is taken about a mean that is far off).  What a team does depends on the width alone, so that a row's
-// result does not depend on the rows beside it.
+// A thread has groups of eight elements of a row.  A team of threads has a row: a warp or a part of one, or a block, in the backward pass beyond
+// 2048 elements a cluster of up to eight blocks; sums over a row go through shuffles, shared memory and the cluster's shared memory
+// accordingly, one exchange for each norm and direction (a norm's mean and squares are combined from the warps' own by the pairwise
+// formula of Chan, Golub and LeVeque, 1979, so that no square is taken about a mean that is far off).  What a team does depends on the width
+// alone, so that a row's result does not depend on the rows beside it.
 //
-// Rows in 16-byte aligned arrays of a multiple of eight elements (VEC): a thread's elements are neighbours, it fetches those of the next
-// rows with 16-byte asynchronous copies into slots of shared memory of its own (no barrier), and one generator block decides its mask.
+// Rows in 16-byte aligned arrays of a multiple of eight elements (VEC): a group is eight neighbours, a thread fetches the groups of the next
+// rows with 16-byte asynchronous copies into slots of shared memory of its own (no barrier), and one generator block decides a group's mask.
 // Other rows: a thread's elements are a team apart, so that a warp's loads are neighbours, and the mask's bytes go through shared memory.
 #pragma once
 
 #include <atomic>
 
+#include "mbarrier.cuh"
 #include "residual_join.cuh"
 
 namespace lutb {
 
-constexpr int kRowElems = 8, kRowMaxThreads = 256, kRowMaxCluster = 8;
-constexpr int64_t kRowMaxWidth = (int64_t)kRowElems * kRowMaxThreads * kRowMaxCluster;
+constexpr int kRowElems = 8;
+constexpr int kBackwardThreads = 256, kForwardThreads = 512, kRowMaxCluster = 8;
+constexpr int64_t kRowMaxWidth = 16384;   // 512 threads of four groups forward, eight blocks of 256 threads of one group backward
+
+
+enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_CLUSTER = 2, TEAM_ANY = 3 };   // ANY: told at run time (rows that are not VEC)
 
 struct RowShape {
+    int groups;                 // of a thread
     int team, teams, threads;   // threads of a row in a block, rows a block has at a time, threads of a block
     int cluster, slice;         // blocks of a row, columns of a block
+    int kind;                   // RowTeam
+    int stages;                 // rows whose elements a thread has room for in shared memory: this one and those that are fetched
 };
-inline RowShape row_shape(int64_t width) {
-    RowShape s{};
-    s.cluster = 1;
-    while (width > (int64_t)s.cluster * kRowElems * kRowMaxThreads) s.cluster *= 2;
-    const int t = (int)(((width + kRowElems - 1) / kRowElems + s.cluster - 1) / s.cluster);
-    s.slice = t * kRowElems;
+inline void shape_team(RowShape &s, int64_t width, int block) {
+    const int64_t each = (int64_t)s.groups * kRowElems;
+    const int t = (int)(((width + each - 1) / each + s.cluster - 1) / s.cluster);
+    s.slice = (int)(t * each);
     if (t <= 32) {
         s.team = 1;
         while (s.team < t) s.team *= 2;
-        s.threads = kRowMaxThreads;
+        s.threads = block;
         s.teams = s.threads / s.team;
+        s.kind = TEAM_WARP;
     } else {
         s.team = s.threads = (t + 31) / 32 * 32;
         s.teams = 1;
+        s.kind = s.cluster > 1 ? TEAM_CLUSTER : TEAM_BLOCK;
     }
+}
+// Forward: up to 256 elements one group a thread, up to 1024 four, always within a warp; then blocks.  Rows that are not VEC have one group up to
+// 2048, where a warp's loads cover more neighbours.
+inline RowShape forward_shape(int64_t width, bool vec) {
+    RowShape s{};
+    s.cluster = 1;
+    s.groups = width <= (vec ? 256 : 2048) ? 1 : 4;
+    shape_team(s, width, 128);
+    return s;
+}
+// Backward: one group, whose five sums over the rows take forty registers.
+inline RowShape backward_shape(int64_t width) {
+    RowShape s{};
+    s.cluster = s.groups = 1;
+    while (width > (int64_t)s.cluster * kRowElems * kBackwardThreads) s.cluster *= 2;
+    shape_team(s, width, kBackwardThreads);
     return s;
 }
 
@@ -68,6 +92,17 @@ __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 __device__ __forceinline__ float total(const float2 *v) {
     const float2 s = add2(add2(v[0], v[1]), add2(v[2], v[3]));
     return s.x + s.y;
+}
+__device__ __forceinline__ void zero8(float2 *v) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) v[k] = make_float2(0.0f, 0.0f);
+}
+__device__ __forceinline__ void drop8(float2 *v, uint32_t kept, float scale) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        v[k].x = (kept >> (2 * k) & 1) ? v[k].x * scale : 0.0f;
+        v[k].y = (kept >> (2 * k) & 2) ? v[k].y * scale : 0.0f;
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ eight elements
@@ -112,74 +147,184 @@ __device__ __forceinline__ void store8(T *p, const float2 *v) {
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
 
 // ------------------------------------------------------------------------------------------------ a thread's place
-struct RowPlace {
-    int tid, t, team, teams, which;   // thread in the block, in its team; threads of a team, teams, this one
-    int cluster, rank;
-    int64_t width, first, limit;      // columns of the block: first .. limit - 1
-    float warp_count;                 // elements of the warp
-    uint32_t valid;                   // which of the eight elements exist
-    uint32_t parity;
-    float4 (*slots)[kRowMaxCluster * kRowMaxThreads / 32];
-
-    template <bool VEC>
-    __device__ __forceinline__ int64_t column(int k) const { return VEC ? first + t * 8 + k : first + t + (int64_t)k * team; }
+// Values that warps exchange: of two numbers each, two sets in turn (a set is written again only after the barrier of the next one, which a
+// thread reaches when it has read this one).
+template <int WARPS, int CLUSTER>
+struct RowSlots {
+    float a[2][WARPS * CLUSTER], b[2][WARPS * CLUSTER];
+    float count[WARPS];    // elements of the warps
+    uint64_t arrived[2];   // clusters: all blocks' values of a set have come
 };
 
+struct RowPlace {
+    int t, team, teams, which;   // thread in its team; threads of a team, teams, this one
+    int cluster, rank;
+    int64_t first;               // the block's first column
+    uint32_t valid;              // which elements exist: a bit a group (VEC) or an element
+    uint32_t turn;               // exchanges so far
+    float width, inverse;        // of a row, in elements
+    bool waits;                  // false after a wait that ran out
+};
+
+// Column k of group g.
 template <bool VEC>
-__device__ __forceinline__ RowPlace row_place(const JoinArgs &a, const RowShape &s, float4 (*slots)[kRowMaxCluster * kRowMaxThreads / 32]) {
+__device__ __forceinline__ int64_t row_column(const RowPlace &p, int g, int k) {
+    return VEC ? p.first + (int64_t)(g * p.team + p.t) * 8 + k : p.first + p.t + (int64_t)(g * 8 + k) * p.team;
+}
+template <bool VEC>
+__device__ __forceinline__ bool row_valid(const RowPlace &p, int g, int k) { return p.valid >> (VEC ? g : g * 8 + k) & 1; }
+
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// (no memory is handed over: nothing is waited for but the blocks themselves)
+__device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory"); }
+
+template <bool VEC, int G, class Slots>
+__device__ __forceinline__ RowPlace row_place(const JoinArgs &a, const RowShape &s, Slots &slots) {
     RowPlace p;
-    p.tid = threadIdx.x;
+    const int tid = threadIdx.x;
     p.team = s.team;
     p.teams = s.teams;
-    p.which = p.tid / s.team;
-    p.t = p.tid - p.which * s.team;
+    p.which = tid / s.team;
+    p.t = tid - p.which * s.team;
     p.cluster = s.cluster;
     p.rank = s.cluster > 1 ? (int)(blockIdx.x % s.cluster) : 0;
-    p.width = a.width;
     p.first = (int64_t)p.rank * s.slice;
-    p.limit = min(p.first + s.slice, a.width);
+    p.width = (float)a.width;
+    p.inverse = 1.0f / p.width;
+    p.turn = 0;
+    p.waits = true;
     p.valid = 0;
+    const int64_t limit = min(p.first + s.slice, a.width);
+    int count = 0;
 #pragma unroll
-    for (int k = 0; k < 8; k++) p.valid |= (p.column<VEC>(k) < p.limit ? 1u : 0u) << k;
-    p.warp_count = (float)__reduce_add_sync(0xffffffffu, __popc(p.valid));
-    p.parity = 0;
-    p.slots = slots;
+    for (int g = 0; g < G; g++) {
+        if (VEC) {
+            if (row_column<VEC>(p, g, 0) < limit) p.valid |= 1u << g, count += 8;
+        } else {
+#pragma unroll
+            for (int k = 0; k < 8; k++)
+                if (row_column<VEC>(p, g, k) < limit) p.valid |= 1u << (g * 8 + k), count++;
+        }
+    }
+    if (s.team > 32) {
+        constexpr int kAll = sizeof(slots.a[0]) / sizeof(float), kWarps = sizeof(slots.count) / sizeof(float);
+        for (int k = tid; k < kAll; k += blockDim.x) slots.a[0][k] = slots.a[1][k] = slots.b[0][k] = slots.b[1][k] = 0.0f;
+        if (tid < kWarps) slots.count[tid] = 0.0f;
+        count = __reduce_add_sync(0xffffffffu, count);
+        __syncthreads();
+        if ((tid & 31) == 0) slots.count[tid >> 5] = (float)count;
+        if (s.cluster > 1) {
+            if (tid == 0) {
+                mbar_init(smem_u32(&slots.arrived[0]), 1);
+                mbar_init(smem_u32(&slots.arrived[1]), 1);
+                fence_barrier_init();
+            }
+            cluster_sync();   // the row's blocks are there and ready
+        } else {
+            __syncthreads();
+        }
+    }
     return p;
 }
 
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 __device__ __forceinline__ float team_sum(float v, int team) {   // teams of a warp or a part of one
-    for (int o = team >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        const float other = __shfl_xor_sync(0xffffffffu, v, o);
+        v += o < team ? other : 0.0f;
+    }
     return v;
 }
-// A warp's values to every block of the row; they can be read after the sync, until the next but one.
-__device__ __forceinline__ void publish(const RowPlace &p, float4 v) {
-    const int lane = p.tid & 31, warps = p.team >> 5;
-    if (p.cluster == 1) {
-        if (lane == 0) p.slots[p.parity][p.tid >> 5] = v;
-    } else if (lane < p.cluster) {
-        uint32_t at = (uint32_t)__cvta_generic_to_shared(&p.slots[p.parity][p.rank * warps + (p.tid >> 5)]);
-        asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(at) : "r"(lane));
-        asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w) : "memory");
+template <int TEAM>
+__device__ __forceinline__ bool within_warp(const RowPlace &p) { return TEAM == TEAM_WARP || (TEAM == TEAM_ANY && p.team <= 32); }
+template <int TEAM>
+__device__ __forceinline__ bool over_cluster(const RowPlace &p) { return TEAM == TEAM_CLUSTER || (TEAM == TEAM_ANY && p.cluster > 1); }
+
+static __device__ int g_join_wait_errors;   // bounded waits that ran out (lutb_device_wait_errors)
+
+// Every warp's two values to every warp of the row.  A cluster's blocks store them into each other's slots asynchronously, with the arrival
+// counted on the receiver's barrier: a cluster-wide barrier would also wait for this block's stores of results to global memory
+// (measured: 5 us a row).  A wait that runs out is counted, and later ones are not begun.
+template <int TEAM, class Slots>
+__device__ __forceinline__ void publish(const RowPlace &p, Slots &slots, float a, float b) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, set = p.turn & 1;
+    if (!over_cluster<TEAM>(p)) {
+        if (lane == 0) {
+            slots.a[set][warp] = a;
+            slots.b[set][warp] = b;
+        }
+        return;
+    }
+    const int warps = p.team >> 5;
+    if (threadIdx.x == 0) mbar_arrive_expect_tx(smem_u32(&slots.arrived[set]), (uint32_t)(8 * warps * p.cluster));
+    if (lane < p.cluster) {
+        const int at = p.rank * (kBackwardThreads / 32) + warp;
+        uint32_t to_a = smem_u32(&slots.a[set][at]), to_b = smem_u32(&slots.b[set][at]), bar = smem_u32(&slots.arrived[set]);
+        asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(to_a) : "r"(lane));
+        asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(to_b) : "r"(lane));
+        asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(bar) : "r"(lane));
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to_a), "r"(__float_as_uint(a)), "r"(bar) : "memory");
+        asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(to_b), "r"(__float_as_uint(b)), "r"(bar) : "memory");
     }
 }
-__device__ __forceinline__ void meet(const RowPlace &p) {
-    if (p.cluster == 1)
+__device__ __forceinline__ bool arrived(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+template <int TEAM, class Slots>
+__device__ __forceinline__ void collect(RowPlace &p, Slots &slots) {
+    if (!over_cluster<TEAM>(p)) {
         __syncthreads();
-    else
-        cluster_sync();
+        return;
+    }
+    const uint32_t bar = smem_u32(&slots.arrived[p.turn & 1]), parity = p.turn >> 1 & 1;
+    if (!p.waits || arrived(bar, parity)) return;
+    const long long t0 = clock64();
+    while (!arrived(bar, parity)) {
+        if (clock64() - t0 > kWaitLimitCycles) {
+            if (threadIdx.x == 0) atomicAdd(&g_join_wait_errors, 1);
+            p.waits = false;
+            return;
+        }
+    }
+}
+// The sum of a set of slots, always in the same order.
+template <int N>
+__device__ __forceinline__ float slot_sum(const float *from) {
+    float2 s = make_float2(0.0f, 0.0f);
+#pragma unroll
+    for (int k = 0; k < N; k += 4) {
+        const float4 v = *reinterpret_cast<const float4 *>(from + k);
+        s = add2(s, add2(make_float2(v.x, v.y), make_float2(v.z, v.w)));
+    }
+    return s.x + s.y;
+}
+template <int TEAM, class Slots>
+__device__ __forceinline__ float all_slots(const RowPlace &p, const float *from) {
+    constexpr int kWarps = sizeof(Slots::count) / sizeof(float);
+    float s = slot_sum<kWarps>(from);
+    if (over_cluster<TEAM>(p))
+        for (int r = 1; r < p.cluster; r++) s += slot_sum<kWarps>(from + r * kWarps);
+    return s;
 }
 // Sums of two values over the row; `between` runs while the others arrive.
-template <class Fn>
-__device__ __forceinline__ float2 row_sums(RowPlace &p, float a, float b, bool second, Fn between) {
-    if (p.team <= 32) {
+template <int TEAM, class Slots, class Fn>
+__device__ __forceinline__ float2 row_sums(RowPlace &p, Slots &slots, float a, float b, bool second, Fn between) {
+    if (within_warp<TEAM>(p)) {
         a = team_sum(a, p.team);
         if (second) b = team_sum(b, p.team);
         between();
@@ -187,83 +332,100 @@ __device__ __forceinline__ float2 row_sums(RowPlace &p, float a, float b, bool s
     }
     a = warp_sum(a);
     if (second) b = warp_sum(b);
-    publish(p, make_float4(a, b, 0.0f, 0.0f));
+    publish<TEAM>(p, slots, a, b);
     between();
-    meet(p);
-    float2 s = make_float2(0.0f, 0.0f);
-    const int n = p.cluster * (p.team >> 5);
-    for (int k = 0; k < n; k++) s = add2(s, *reinterpret_cast<const float2 *>(&p.slots[p.parity][k]));
-    p.parity ^= 1;
+    collect<TEAM>(p, slots);
+    const float2 s = make_float2(all_slots<TEAM, Slots>(p, slots.a[p.turn & 1]), second ? all_slots<TEAM, Slots>(p, slots.b[p.turn & 1]) : 0.0f);
+    p.turn++;
     return s;
 }
 // Mean (0 for an RMS norm) and reciprocal deviation of the row's values; values of no element are 0.
-template <bool VEC>
-__device__ __forceinline__ float2 row_stats(RowPlace &p, const float2 *v, bool layer, float eps) {
-    const float width = (float)p.width;
+template <bool VEC, int G, int TEAM, class Slots>
+__device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const float2 (*v)[4], bool layer, float eps) {
+    auto sum = [&]() {
+        float s = 0.0f;
+#pragma unroll
+        for (int g = 0; g < G; g++) s += total(v[g]);
+        return s;
+    };
     auto squares = [&](float mean) {
         float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
-        for (int k = 0; k < 4; k++) {
-            float2 d = add2(v[k], both(-mean));
-            if (!VEC) {
-                d.x = (p.valid >> (2 * k) & 1) ? d.x : 0.0f;
-                d.y = (p.valid >> (2 * k) & 2) ? d.y : 0.0f;
+        for (int g = 0; g < G; g++) {
+            float2 q = make_float2(0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                float2 d = add2(v[g][k], both(-mean));
+                if (!VEC) {
+                    d.x = row_valid<VEC>(p, g, 2 * k) ? d.x : 0.0f;
+                    d.y = row_valid<VEC>(p, g, 2 * k + 1) ? d.y : 0.0f;
+                }
+                q = fma2(d, d, q);
             }
-            s = fma2(d, d, s);
+            if (VEC && !row_valid<VEC>(p, g, 0)) q = make_float2(0.0f, 0.0f);
+            s = add2(s, q);
         }
-        return p.valid ? s.x + s.y : 0.0f;
+        return s.x + s.y;
     };
-    if (p.team <= 32) {
-        const float mean = layer ? team_sum(total(v), p.team) / width : 0.0f;
-        return make_float2(mean, rsqrtf(team_sum(squares(mean), p.team) / width + eps));
+    if (within_warp<TEAM>(p)) {
+        const float mean = layer ? team_sum(sum(), p.team) / p.width : 0.0f;
+        return make_float2(mean, rsqrtf(team_sum(squares(mean), p.team) * p.inverse + eps));
     }
-    float mean = 0.0f;
+    const int set = p.turn & 1;
+    float mean = 0.0f, s;
     if (layer) {
-        const float s = warp_sum(p.valid ? total(v) : 0.0f);
-        mean = p.warp_count > 0.0f ? s / p.warp_count : 0.0f;
+        const float count = slots.count[threadIdx.x >> 5];
+        mean = count > 0.0f ? warp_sum(sum()) / count : 0.0f;
     }
-    publish(p, make_float4(mean, warp_sum(squares(mean)), p.warp_count, 0.0f));
-    meet(p);
-    const int n = p.cluster * (p.team >> 5);
-    float s = 0.0f;
+    publish<TEAM>(p, slots, warp_sum(squares(mean)), mean);
+    collect<TEAM>(p, slots);
+    s = all_slots<TEAM, Slots>(p, slots.a[set]);
     mean = 0.0f;
     if (layer) {
-        for (int k = 0; k < n; k++) mean += p.slots[p.parity][k].x * p.slots[p.parity][k].z;
-        mean /= width;
+        constexpr int kWarps = sizeof(Slots::count) / sizeof(float);
+        float m[kWarps], n[kWarps];
+#pragma unroll
+        for (int k = 0; k < kWarps; k++) {
+            m[k] = slots.b[set][k];
+            n[k] = slots.count[k];
+            mean = fmaf(m[k], n[k], mean);
+        }
+        mean /= p.width;
+        float between = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWarps; k++) between = fmaf(n[k] * (m[k] - mean), m[k] - mean, between);
+        s += between;
     }
-    for (int k = 0; k < n; k++) {
-        const float4 w = p.slots[p.parity][k];
-        const float d = w.x - mean;
-        s += layer ? w.y + w.z * d * d : w.y;
-    }
-    p.parity ^= 1;
-    return make_float2(mean, rsqrtf(s / width + eps));
+    p.turn++;
+    return make_float2(mean, rsqrtf(s * p.inverse + eps));
 }
 
-// Eight of a parameter's values; `none` where there is no such parameter, 0 for columns beyond the row.
+// Eight of a parameter's values: `none` where there is no such parameter, 0 for columns beyond the row.
 template <class F, bool VEC>
-__device__ __forceinline__ void param8(const RowPlace &p, const void *from, bool f32, int64_t at, float none, float scale, float2 *v) {
-    float e[8];
-    if (VEC && from != nullptr && p.valid) {
-        const int64_t c = at + p.column<VEC>(0);
-        if (f32) {
-            const uint4 part[2] = {reinterpret_cast<const uint4 *>(static_cast<const float *>(from) + c)[0],
-                                   reinterpret_cast<const uint4 *>(static_cast<const float *>(from) + c)[1]};
+__device__ __forceinline__ void param8(const RowPlace &p, int g, const void *from, bool f32, int64_t at, float none, float2 *v) {
+    if constexpr (VEC) {
+        if (from == nullptr || !row_valid<VEC>(p, g, 0)) {
+            const float e = row_valid<VEC>(p, g, 0) ? none : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = both(e);
+            return;
+        }
+        const int64_t c = at + row_column<VEC>(p, g, 0);
+        if (sizeof(F) == 4 || f32) {
+            const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const float *>(from) + c);
+            const uint4 part[2] = {__ldg(q), __ldg(q + 1)};
             unpack8<float>(part, v);
         } else {
-            uint4 part[kParts<F>];
-#pragma unroll
-            for (int q = 0; q < kParts<F>; q++) part[q] = reinterpret_cast<const uint4 *>(static_cast<const F *>(from) + c)[q];
+            const uint4 part[1] = {__ldg(reinterpret_cast<const uint4 *>(static_cast<const F *>(from) + c))};
             unpack8<F>(part, v);
         }
     } else {
+        float e[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) e[k] = (p.valid >> k & 1) ? join_param<F>(from, f32, at + p.column<VEC>(k), none) : 0.0f;
+        for (int k = 0; k < 8; k++) e[k] = row_valid<VEC>(p, g, k) ? join_param<F>(from, f32, at + row_column<VEC>(p, g, k), none) : 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
     }
-#pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = mul2(v[k], both(scale));
 }
 
 // The rows of a block in turn: chunk by chunk, `teams` rows at a time.
@@ -285,128 +447,128 @@ struct RowCursor {
     }
 };
 
-// The next rows' elements, in this thread's slots of shared memory (VEC), or nothing.
-template <int STAGES>
+// The next rows' elements, in this thread's slots of shared memory.  With one stage a row is fetched when its turn comes.
 struct RowRing {
-    uint4 *at;         // [stage][part][thread]
-    int parts, threads, tid;
-    uint32_t fill = 0, take = 0;
-    __device__ __forceinline__ void fetch(int part, const void *from, int n) const {
-        for (int q = 0; q < n; q++)
-            copy16((uint32_t)__cvta_generic_to_shared(at + ((int)fill * parts + part + q) * threads + tid), static_cast<const uint4 *>(from) + q);
+    uint4 *at;          // [stage][part][thread], from this thread's first
+    int parts, threads, stages;
+    int fill, take;
+    template <int N>
+    __device__ __forceinline__ void fetch(int part, const void *from) const {
+        const uint32_t to = smem_u32(at + (fill * parts + part) * threads);
+#pragma unroll
+        for (int q = 0; q < N; q++) copy16(to + q * threads * 16, static_cast<const uint4 *>(from) + q);
     }
     __device__ __forceinline__ void filled() {
         asm volatile("cp.async.commit_group;" ::: "memory");
-        fill = fill + 1 == STAGES ? 0 : fill + 1;
+        fill = fill + 1 == stages ? 0 : fill + 1;
     }
-    __device__ __forceinline__ void ready() const { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 2) : "memory"); }
-    __device__ __forceinline__ void taken() { take = take + 1 == STAGES ? 0 : take + 1; }
+    __device__ __forceinline__ void ready() const {
+        if (stages == 3)
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+        else
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+    }
+    __device__ __forceinline__ void taken() { take = take + 1 == stages ? 0 : take + 1; }
     template <class T>
     __device__ __forceinline__ void get(int part, float2 *v) const {
         uint4 w[kParts<T>];
 #pragma unroll
-        for (int q = 0; q < kParts<T>; q++) w[q] = at[((int)take * parts + part + q) * threads + tid];
+        for (int q = 0; q < kParts<T>; q++) w[q] = at[(take * parts + part + q) * threads];
         unpack8<T>(w, v);
     }
 };
 
 template <class T, bool VEC>
-__device__ __forceinline__ void load_apart(const RowPlace &p, const T *row, bool on, float2 *v) {
+__device__ __forceinline__ void load_apart(const RowPlace &p, int g, const T *row, bool on, float2 *v) {
     float e[8];
 #pragma unroll
-    for (int k = 0; k < 8; k++) e[k] = on && (p.valid >> k & 1) ? to_f32(row[p.column<VEC>(k)]) : 0.0f;
+    for (int k = 0; k < 8; k++) e[k] = on && row_valid<VEC>(p, g, k) ? to_f32(row[row_column<VEC>(p, g, k)]) : 0.0f;
 #pragma unroll
     for (int k = 0; k < 4; k++) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
 }
 template <class T, bool VEC>
-__device__ __forceinline__ void store_row(const RowPlace &p, T *row, const float2 *v) {
+__device__ __forceinline__ void store_row(const RowPlace &p, int g, T *row, const float2 *v) {
     if constexpr (VEC) {
-        if (p.valid) store8(row + p.column<VEC>(0), v);
+        if (row_valid<VEC>(p, g, 0)) store8(row + row_column<VEC>(p, g, 0), v);
     } else {
 #pragma unroll
         for (int k = 0; k < 8; k++)
-            if (p.valid >> k & 1) row[p.column<VEC>(k)] = from_f32<T>(k & 1 ? v[k >> 1].y : v[k >> 1].x);
+            if (row_valid<VEC>(p, g, k)) row[row_column<VEC>(p, g, k)] = from_f32<T>(k & 1 ? v[k >> 1].y : v[k >> 1].x);
     }
 }
-__device__ __forceinline__ void zero8(float2 *v) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = make_float2(0.0f, 0.0f);
-}
 
-// The mask of a thread's eight elements, as bits.  Rows that are not VEC: the team's generator blocks as bytes in shared memory, two sets
+// The masks of a thread's groups, eight bits each.  Rows that are not VEC: the team's generator blocks as bytes in shared memory, two sets
 // in turn, so that one barrier a row is enough.
-template <bool VEC>
-__device__ __forceinline__ uint32_t row_mask(const RowPlace &p, const JoinArgs &a, const DropKey &key, int64_t row, uint8_t *bytes, uint32_t turn) {
+template <bool VEC, int G>
+__device__ __forceinline__ uint32_t row_mask(const RowPlace &p, const JoinArgs &a, const DropKey &key, int64_t row, uint8_t *bytes, uint32_t set) {
     const int64_t at = row * a.width + p.first;
-    if (VEC) return keep_bits((uint64_t)(at + p.t * 8) >> 3, key, a.drop);
-    uint8_t *own = bytes + ((int)turn * p.teams + p.which) * (p.team + 1);
+    uint32_t kept = 0;
+    if (VEC) {
+#pragma unroll
+        for (int g = 0; g < G; g++) kept |= keep_bits((uint64_t)(at >> 3) + g * p.team + p.t, key, a.drop) << (8 * g);
+        return kept;
+    }
+    uint8_t *own = bytes + ((int)set * p.teams + p.which) * (G * p.team + 1);
     const int off = (int)(at & 7);
-    own[p.t] = (uint8_t)keep_bits(((uint64_t)at >> 3) + p.t, key, a.drop);
-    if (p.t == 0) own[p.team] = (uint8_t)keep_bits(((uint64_t)at >> 3) + p.team, key, a.drop);
+#pragma unroll
+    for (int g = 0; g < G; g++) own[g * p.team + p.t] = (uint8_t)keep_bits((uint64_t)(at >> 3) + g * p.team + p.t, key, a.drop);
+    if (p.t == 0) own[G * p.team] = (uint8_t)keep_bits((uint64_t)(at >> 3) + G * p.team, key, a.drop);
     if (p.team <= 32)
         __syncwarp();
     else
         __syncthreads();
-    uint32_t kept = 0;
 #pragma unroll
-    for (int k = 0; k < 8; k++) {
+    for (int k = 0; k < 8 * G; k++) {
         const int e = off + p.t + k * p.team;
         kept |= (uint32_t)(own[e >> 3] >> (e & 7) & 1) << k;
     }
     return kept;
 }
-__device__ __forceinline__ void drop8(float2 *v, uint32_t kept, float scale) {
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        v[k].x = (kept >> (2 * k) & 1) ? v[k].x * scale : 0.0f;
-        v[k].y = (kept >> (2 * k) & 2) ? v[k].y * scale : 0.0f;
-    }
-}
-constexpr size_t kMaskBytes = 2 * 2 * kRowMaxThreads;   // two sets, a byte a thread and one a team
+template <int G, int THREADS>
+constexpr size_t kMaskBytes = 2 * (G * THREADS + THREADS);   // two sets, a byte a group and one a team
 
 // ------------------------------------------------------------------------------------------------ forward
 // BRANCH: 0 no branch (the norm alone), 1 a branch, 2 a branch with a norm of its own.  NEXT: the norm before the next block.
 template <class X, class F>
-constexpr int kForwardParts = kParts<X> + kParts<F>;   // x, f; two more for a gate of each element
-constexpr int kForwardStages = 3;
+constexpr int kForwardParts = kParts<X> + kParts<F>;   // of a group: x, f; two more for a gate of each element
+template <int G, int TEAM>
+constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : G == 1 ? 256 : kForwardThreads;
 
-template <class X, class F, int BRANCH, bool NEXT, bool VEC>
-__global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
+template <class X, class F, int BRANCH, bool NEXT, bool VEC, int G, int TEAM>
+__global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
+    constexpr int kThreads = kThreadsOf<G, TEAM>;
     extern __shared__ uint4 dynamic[];
-    __shared__ float4 slots[2][kRowMaxCluster * kRowMaxThreads / 32];
-    __shared__ uint8_t masks[VEC ? 1 : kMaskBytes];
-    RowPlace p = row_place<VEC>(a, shape, slots);
+    __shared__ __align__(16) RowSlots<TEAM == TEAM_WARP ? 4 : kThreads / 32, 1> slots;
+    __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<G, kThreads>];
+    RowPlace p = row_place<VEC, G>(a, shape, slots);
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
-    float2 aw[4], ab[4], gate[4], bw[4], bb[4];
-    if (BRANCH == 2) {
-        param8<F, VEC>(p, a.aw, a.params_f32, 0, 1.0f, 1.0f, aw);
-        param8<F, VEC>(p, a.ab, a.params_f32, 0, 0.0f, 1.0f, ab);
-    }
-    if (NEXT) {
-        param8<F, VEC>(p, a.bw, a.params_f32, 0, 1.0f, 1.0f, bw);
-        param8<F, VEC>(p, a.bb, a.params_f32, 0, 0.0f, 1.0f, bb);
-    }
     const bool gate_each = BRANCH && a.gate_rows == 1;
-    int64_t gate_end = 0;   // first row of another gate row
-    if (BRANCH && a.gate_rows == 0) param8<F, VEC>(p, nullptr, true, 0, 1.0f, a.branch, gate);
-
-    RowRing<kForwardStages> ring{dynamic, kForwardParts<X, F> + (gate_each ? 2 : 0), (int)blockDim.x, p.tid};
-    const int64_t stride = gridDim.x / shape.cluster;
-    RowCursor load{(int64_t)(blockIdx.x / shape.cluster), 0, 0}, here = load;
+    constexpr int kX = 0, kF = kParts<X>, kGate = kForwardParts<X, F>;
+    const int parts = kForwardParts<X, F> + (gate_each ? 2 : 0);
+    RowRing ring{dynamic + threadIdx.x, G * parts, (int)blockDim.x, shape.stages, 0, 0};
+    const int64_t stride = gridDim.x;
+    RowCursor load{(int64_t)blockIdx.x, 0, 0}, here = load;
     load.enter(a);
-    here.enter(a);
+    here = load;
+    const X *const x_in = static_cast<const X *>(a.x);
+    const F *const f_in = static_cast<const F *>(a.f);
     auto fetch = [&]() {
         if (VEC) {
             if (load.more(a)) {
-                const int64_t row = load.base + p.which, at = row * a.width + p.column<VEC>(0);
-                if (row < load.end && p.valid) {
-                    ring.fetch(0, static_cast<const X *>(a.x) + at, kParts<X>);
-                    if (BRANCH) ring.fetch(kParts<X>, static_cast<const F *>(a.f) + at, kParts<F>);
-                    if (gate_each) {
-                        if (a.gate_f32)
-                            ring.fetch(kParts<X> + kParts<F>, static_cast<const float *>(a.gate) + at, 2);
-                        else
-                            ring.fetch(kParts<X> + kParts<F>, static_cast<const F *>(a.gate) + at, kParts<F>);
+                const int64_t row = load.base + p.which, at = row * a.width;
+                if (row < load.end) {
+#pragma unroll
+                    for (int g = 0; g < G; g++) {
+                        if (!row_valid<VEC>(p, g, 0)) break;
+                        const int64_t c = at + row_column<VEC>(p, g, 0);
+                        ring.fetch<kParts<X>>(g * parts + kX, x_in + c);
+                        if (BRANCH) ring.fetch<kParts<F>>(g * parts + kF, f_in + c);
+                        if (gate_each) {
+                            if (sizeof(F) == 4 || a.gate_f32)
+                                ring.fetch<2>(g * parts + kGate, static_cast<const float *>(a.gate) + c);
+                            else
+                                ring.fetch<kParts<F>>(g * parts + kGate, static_cast<const F *>(a.gate) + c);
+                        }
                     }
                 }
                 load.next(a, p.teams, stride);
@@ -414,100 +576,131 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_forward_kernel(co
             ring.filled();
         }
     };
-#pragma unroll
-    for (int s = 0; s < kForwardStages - 1; s++) fetch();
-    if (p.cluster > 1) cluster_sync();   // the row's blocks are there
-    uint32_t turn = 0;
+    for (int s = 1; s < shape.stages; s++) fetch();
+    uint32_t set = 0;
+    int64_t gate_at = 0, gate_end = 0;   // the gate row in use, the first row of another one
     for (; here.more(a); here.next(a, p.teams, stride)) {
         const int64_t row = here.base + p.which, at = row * a.width;
         const bool on = row < here.end;
         if (BRANCH && a.gate_rows > 1 && on && row >= gate_end) {
             const int64_t gate_row = row / a.gate_rows;
             gate_end = (gate_row + 1) * a.gate_rows;
-            param8<F, VEC>(p, a.gate, a.gate_f32, gate_row * a.width, 1.0f, a.branch, gate);
+            gate_at = gate_row * a.width;
         }
-        uint32_t kept = 0xffu;
-        if (BRANCH && a.drop.on) kept = row_mask<VEC>(p, a, key, row, masks, turn);
-        turn ^= 1;
-        float2 h[4], v[4];
-        if (VEC) {
-            ring.ready();
-            ring.template get<X>(0, h);
-            if (BRANCH) ring.template get<F>(kParts<X>, v);
-            if (gate_each) {
-                if (a.gate_f32)
-                    ring.template get<float>(kParts<X> + kParts<F>, gate);
-                else
-                    ring.template get<F>(kParts<X> + kParts<F>, gate);
-            }
-            ring.taken();
-            if (!on || !p.valid) {
-                zero8(h);
-                if (BRANCH) zero8(v);
-                if (gate_each) zero8(gate);
-            }
-        } else {
-            load_apart<X, VEC>(p, static_cast<const X *>(a.x) + at, on, h);
-            if (BRANCH) load_apart<F, VEC>(p, static_cast<const F *>(a.f) + at, on, v);
-            if (gate_each) {
-                if (a.gate_f32)
-                    load_apart<float, VEC>(p, static_cast<const float *>(a.gate) + at, on, gate);
-                else
-                    load_apart<F, VEC>(p, static_cast<const F *>(a.gate) + at, on, gate);
-            }
-        }
+        uint32_t kept = 0xffffffffu;
+        if (BRANCH && a.drop.on) kept = row_mask<VEC, G>(p, a, key, row, masks, set);
+        set ^= 1;
+        float2 v[G][4];
         float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
-        if (BRANCH) {
-            if (gate_each)
-#pragma unroll
-                for (int k = 0; k < 4; k++) gate[k] = mul2(gate[k], both(a.branch));
-            if (a.drop.on) drop8(v, kept, a.drop.scale);
-            if (BRANCH == 2) {
-                const float2 s = row_stats<VEC>(p, v, a.after == LUTB_NORM_LAYER, a.eps);
-                st.x = s.x;
-                st.y = s.y;
-#pragma unroll
-                for (int k = 0; k < 4; k++) v[k] = fma2(mul2(add2(v[k], both(-s.x)), both(s.y)), aw[k], ab[k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) h[k] = fma2(gate[k], v[k], mul2(h[k], both(a.skip)));
+        if (VEC) {
+            if (shape.stages == 1) fetch();
+            ring.ready();
         }
-        fetch();
-        if (BRANCH && on) store_row<X, VEC>(p, static_cast<X *>(a.h) + at, h);
+        if (BRANCH) {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                if (VEC) {
+                    ring.get<F>(g * parts + kF, v[g]);
+                    if (!on || !row_valid<VEC>(p, g, 0)) zero8(v[g]);
+                } else {
+                    load_apart<F, VEC>(p, g, f_in + at, on, v[g]);
+                }
+                if (a.drop.on) drop8(v[g], kept >> (8 * g), a.drop.scale);
+            }
+        }
+        if (BRANCH == 2) {
+            const float2 s = row_stats<VEC, G, TEAM>(p, slots, v, a.after == LUTB_NORM_LAYER, a.eps);
+            st.x = s.x;
+            st.y = s.y;
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                float2 w[4], b[4];
+                param8<F, VEC>(p, g, a.aw, a.params_f32, 0, 1.0f, w);
+                param8<F, VEC>(p, g, a.ab, a.params_f32, 0, 0.0f, b);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = fma2(mul2(add2(v[g][k], both(-s.x)), both(s.y)), w[k], b[k]);
+            }
+        }
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            float2 x[4];
+            if (VEC) {
+                ring.get<X>(g * parts + kX, x);
+                if (!on || !row_valid<VEC>(p, g, 0)) zero8(x);
+            } else {
+                load_apart<X, VEC>(p, g, x_in + at, on, x);
+            }
+            if (BRANCH) {
+                float2 gate[4];
+                if (!gate_each) {
+                    param8<F, VEC>(p, g, a.gate, a.gate_f32, gate_at, 1.0f, gate);
+                } else if (VEC) {
+                    if (sizeof(F) == 4 || a.gate_f32)
+                        ring.get<float>(g * parts + kGate, gate);
+                    else
+                        ring.get<F>(g * parts + kGate, gate);
+                    if (!on || !row_valid<VEC>(p, g, 0)) zero8(gate);
+                } else if (a.gate_f32) {
+                    load_apart<float, VEC>(p, g, static_cast<const float *>(a.gate) + at, on, gate);
+                } else {
+                    load_apart<F, VEC>(p, g, static_cast<const F *>(a.gate) + at, on, gate);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = fma2(mul2(gate[k], both(a.branch)), v[g][k], mul2(x[k], both(a.skip)));
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = x[k];
+            }
+        }
+        if (VEC) {
+            ring.taken();
+            if (shape.stages > 1) fetch();
+        }
+        if (BRANCH && on)
+#pragma unroll
+            for (int g = 0; g < G; g++) store_row<X, VEC>(p, g, static_cast<X *>(a.h) + at, v[g]);
         if (NEXT) {
-            const float2 s = row_stats<VEC>(p, h, a.before == LUTB_NORM_LAYER, a.eps);
+            const float2 s = row_stats<VEC, G, TEAM>(p, slots, v, a.before == LUTB_NORM_LAYER, a.eps);
             st.z = s.x;
             st.w = s.y;
+            if (on)
 #pragma unroll
-            for (int k = 0; k < 4; k++) h[k] = fma2(mul2(add2(h[k], both(-s.x)), both(s.y)), bw[k], bb[k]);
-            if (on) store_row<F, VEC>(p, static_cast<F *>(a.y) + at, h);
+                for (int g = 0; g < G; g++) {
+                    float2 w[4], b[4];
+                    param8<F, VEC>(p, g, a.bw, a.params_f32, 0, 1.0f, w);
+                    param8<F, VEC>(p, g, a.bb, a.params_f32, 0, 0.0f, b);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) w[k] = fma2(mul2(add2(v[g][k], both(-s.x)), both(s.y)), w[k], b[k]);
+                    store_row<F, VEC>(p, g, static_cast<F *>(a.y) + at, w);
+                }
         }
-        if (a.stats && on && p.t == 0 && p.rank == 0) a.stats[row] = st;
+        if (a.stats && on && p.t == 0) a.stats[row] = st;
     }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
 template <class X, class F>
 constexpr int kBackwardParts = 2 * kParts<X> + 2 * kParts<F>;   // x, dh, f, dy; two more for a gate of each element
-template <class X, class F>
-constexpr int kBackwardStages = sizeof(X) + sizeof(F) == 8 ? 2 : 3;
 constexpr int kBackwardParams = 4;   // aw, ab, bw, gate
 
 // See join_backward_kernel for the formulas.  A thread's sums over its rows stay in registers to the end (of the chunk, for a gate row).
-template <class X, class F, int BRANCH, bool NEXT, bool VEC>
-__global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(const JoinArgs a, const RowShape shape) {
+template <class X, class F, int BRANCH, bool NEXT, bool VEC, int TEAM>
+__global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel(const JoinArgs a, const RowShape shape) {
+    constexpr bool kTeams = TEAM == TEAM_WARP || TEAM == TEAM_ANY, kClusters = TEAM == TEAM_CLUSTER || TEAM == TEAM_ANY;
     extern __shared__ uint4 dynamic[];
-    __shared__ float4 slots[2][kRowMaxCluster * kRowMaxThreads / 32];
-    __shared__ uint8_t masks[VEC ? 1 : kMaskBytes];
-    __shared__ float2 joined[4 * kRowMaxThreads];   // the teams' sums of a block
-    RowPlace p = row_place<VEC>(a, shape, slots);
-    const int threads = blockDim.x;
+    __shared__ __align__(16) RowSlots<kBackwardThreads / 32, kClusters ? kRowMaxCluster : 1> slots;
+    __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<1, kBackwardThreads>];
+    __shared__ float2 joined[kTeams ? 4 * kBackwardThreads : 1];   // the teams' sums of a block
+    RowPlace p = row_place<VEC, 1>(a, shape, slots);
+    const int threads = blockDim.x, tid = threadIdx.x;
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
     // parameters in slots of this thread's own: [parameter][half][thread]
-    float4 *const params = reinterpret_cast<float4 *>(dynamic) + p.tid;
+    float4 *const params = reinterpret_cast<float4 *>(dynamic) + tid;
     auto keep_param = [&](int which, const void *from, bool f32, int64_t at, float none, float scale) {
         float2 v[4];
-        param8<F, VEC>(p, from, f32, at, none, scale, v);
+        param8<F, VEC>(p, 0, from, f32, at, none, v);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = mul2(v[k], both(scale));
         params[(2 * which) * threads] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
         params[(2 * which + 1) * threads] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
     };
@@ -527,28 +720,28 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
     int64_t gate_end = 0;   // first row of another gate row
     if (BRANCH && a.gate_rows == 0) keep_param(3, nullptr, true, 0, 1.0f, a.branch);
 
-    RowRing<kBackwardStages<X, F>> ring{dynamic + 2 * kBackwardParams * threads, kBackwardParts<X, F> + (gate_each ? 2 : 0), threads, p.tid};
+    RowRing ring{dynamic + 2 * kBackwardParams * threads + tid, kBackwardParts<X, F> + (gate_each ? 2 : 0), threads, shape.stages, 0, 0};
     constexpr int kDh = kParts<X>, kF = 2 * kParts<X>, kDy = kF + kParts<F>, kGate = kDy + kParts<F>;
     const int64_t stride = gridDim.x / shape.cluster, own = blockIdx.x / shape.cluster;
     RowCursor load{own, 0, 0}, here = load;
     load.enter(a);
-    here.enter(a);
+    here = load;
     const X *const x_in = static_cast<const X *>(a.x), *const dh_in = static_cast<const X *>(a.dh);
     const F *const f_in = static_cast<const F *>(a.f), *const dy_in = static_cast<const F *>(a.dy);
     auto fetch = [&]() {
         if (VEC) {
             if (load.more(a)) {
-                const int64_t row = load.base + p.which, at = row * a.width + p.column<VEC>(0);
+                const int64_t row = load.base + p.which, at = row * a.width + row_column<VEC>(p, 0, 0);
                 if (row < load.end && p.valid) {
-                    if (NEXT) ring.fetch(0, x_in + at, kParts<X>);
-                    if (dh_in) ring.fetch(kDh, dh_in + at, kParts<X>);
-                    if (BRANCH) ring.fetch(kF, f_in + at, kParts<F>);
-                    if (NEXT) ring.fetch(kDy, dy_in + at, kParts<F>);
+                    if (NEXT) ring.fetch<kParts<X>>(0, x_in + at);
+                    if (dh_in) ring.fetch<kParts<X>>(kDh, dh_in + at);
+                    if (BRANCH) ring.fetch<kParts<F>>(kF, f_in + at);
+                    if (NEXT) ring.fetch<kParts<F>>(kDy, dy_in + at);
                     if (gate_each) {
-                        if (a.gate_f32)
-                            ring.fetch(kGate, static_cast<const float *>(a.gate) + at, 2);
+                        if (sizeof(F) == 4 || a.gate_f32)
+                            ring.fetch<2>(kGate, static_cast<const float *>(a.gate) + at);
                         else
-                            ring.fetch(kGate, static_cast<const F *>(a.gate) + at, kParts<F>);
+                            ring.fetch<kParts<F>>(kGate, static_cast<const F *>(a.gate) + at);
                     }
                 }
                 load.next(a, p.teams, stride);
@@ -562,10 +755,10 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
     for (int s = 0; s < kSums; s++) zero8(sums[s]);
     // this thread's sum of eight columns, joined over the block's teams, handed on column by column
     auto hand_out = [&](const float2 *v, auto put) {
-        if (p.teams == 1) {
+        if (!kTeams || p.teams == 1) {
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                if (p.valid >> k & 1) put(p.column<VEC>(k), k & 1 ? v[k >> 1].y : v[k >> 1].x);
+                if (row_valid<VEC>(p, 0, k)) put(row_column<VEC>(p, 0, k), k & 1 ? v[k >> 1].y : v[k >> 1].x);
             return;
         }
         float *all = reinterpret_cast<float *>(joined);
@@ -573,17 +766,14 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
 #pragma unroll
         for (int k = 0; k < 8; k++) all[(VEC ? p.t * 8 + k : p.t + k * p.team) + p.which * p.team * 8] = k & 1 ? v[k >> 1].y : v[k >> 1].x;
         __syncthreads();
-        for (int c = p.tid; c < (int)a.width; c += threads) {
+        for (int c = tid; c < (int)a.width; c += threads) {
             float s = 0.0f;
             for (int w = 0; w < p.teams; w++) s += all[w * p.team * 8 + c];
             put((int64_t)c, s);
         }
     };
-#pragma unroll
-    for (int s = 0; s < kBackwardStages<X, F> - 1; s++) fetch();
-    if (p.cluster > 1) cluster_sync();
-    uint32_t turn = 0;
-    const float width = (float)a.width;
+    for (int s = 1; s < shape.stages; s++) fetch();
+    uint32_t set = 0;
     while (here.more(a)) {
         const int64_t row = here.base + p.which, at = row * a.width, chunk = here.chunk;
         const bool on = row < here.end;
@@ -594,20 +784,21 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
             keep_param(3, a.gate, a.gate_f32, gate_row * a.width, 1.0f, a.branch);
         }
         uint32_t kept = 0xffu;
-        if (BRANCH && a.drop.on) kept = row_mask<VEC>(p, a, key, row, masks, turn);
-        turn ^= 1;
+        if (BRANCH && a.drop.on) kept = row_mask<VEC, 1>(p, a, key, row, masks, set);
+        set ^= 1;
         float2 d[4], t[4], z[4], g[4];   // dh, the branch, the stream, dy
         if (VEC) {
+            if (shape.stages == 1) fetch();
             ring.ready();
-            if (NEXT) ring.template get<X>(0, z);
-            if (dh_in) ring.template get<X>(kDh, d);
-            if (BRANCH) ring.template get<F>(kF, t);
-            if (NEXT) ring.template get<F>(kDy, g);
+            if (NEXT) ring.get<X>(0, z);
+            if (dh_in) ring.get<X>(kDh, d);
+            if (BRANCH) ring.get<F>(kF, t);
+            if (NEXT) ring.get<F>(kDy, g);
         } else {
-            if (NEXT) load_apart<X, VEC>(p, x_in + at, on, z);
-            if (dh_in) load_apart<X, VEC>(p, dh_in + at, on, d);
-            if (BRANCH) load_apart<F, VEC>(p, f_in + at, on, t);
-            if (NEXT) load_apart<F, VEC>(p, dy_in + at, on, g);
+            if (NEXT) load_apart<X, VEC>(p, 0, x_in + at, on, z);
+            if (dh_in) load_apart<X, VEC>(p, 0, dh_in + at, on, d);
+            if (BRANCH) load_apart<F, VEC>(p, 0, f_in + at, on, t);
+            if (NEXT) load_apart<F, VEC>(p, 0, dy_in + at, on, g);
         }
         if (dh_in == nullptr || (VEC && (!on || !p.valid))) zero8(d);
         if (VEC && (!on || !p.valid)) {
@@ -621,15 +812,15 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
                 param(3, gate);
             else {
                 if (VEC) {
-                    if (a.gate_f32)
-                        ring.template get<float>(kGate, gate);
+                    if (sizeof(F) == 4 || a.gate_f32)
+                        ring.get<float>(kGate, gate);
                     else
-                        ring.template get<F>(kGate, gate);
+                        ring.get<F>(kGate, gate);
                     if (!on || !p.valid) zero8(gate);
                 } else if (a.gate_f32) {
-                    load_apart<float, VEC>(p, static_cast<const float *>(a.gate) + at, on, gate);
+                    load_apart<float, VEC>(p, 0, static_cast<const float *>(a.gate) + at, on, gate);
                 } else {
-                    load_apart<F, VEC>(p, static_cast<const F *>(a.gate) + at, on, gate);
+                    load_apart<F, VEC>(p, 0, static_cast<const F *>(a.gate) + at, on, gate);
                 }
 #pragma unroll
                 for (int k = 0; k < 4; k++) gate[k] = mul2(gate[k], both(a.branch));
@@ -637,7 +828,7 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
         }
         if (VEC) {
             ring.taken();
-            fetch();
+            if (shape.stages > 1) fetch();
         }
         float2 n[4];   // the branch after its norm; t becomes its normalised values
         if (BRANCH) {
@@ -667,7 +858,7 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
                 s1 = fma2(u[k], z[k], s1);
             }
             const bool layer = a.before == LUTB_NORM_LAYER;
-            const float2 c = row_sums(p, s1.x + s1.y, layer ? total(u) : 0.0f, layer, [&]() {
+            const float2 c = row_sums<TEAM>(p, slots, s1.x + s1.y, layer ? total(u) : 0.0f, layer, [&]() {
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     if (on) {
@@ -676,7 +867,7 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
                     }
                 }
             });
-            const float c1 = -c.x / width, c2 = layer ? -c.y / width : 0.0f;
+            const float c1 = -c.x * p.inverse, c2 = layer ? -c.y * p.inverse : 0.0f;
 #pragma unroll
             for (int k = 0; k < 4; k++) d[k] = fma2(both(st.w), fma2(z[k], both(c1), add2(u[k], both(c2))), d[k]);
         }
@@ -684,17 +875,17 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
             float2 o[4];
 #pragma unroll
             for (int k = 0; k < 4; k++) o[k] = BRANCH ? mul2(d[k], both(a.skip)) : d[k];
-            store_row<X, VEC>(p, static_cast<X *>(a.dx) + at, o);
+            store_row<X, VEC>(p, 0, static_cast<X *>(a.dx) + at, o);
         }
         if (BRANCH) {
             if (gate_each && a.dgate && on) {
                 float2 o[4];
 #pragma unroll
                 for (int k = 0; k < 4; k++) o[k] = mul2(mul2(d[k], both(a.branch)), n[k]);
-                if (a.gate_f32)
-                    store_row<float, VEC>(p, static_cast<float *>(a.dgate) + at, o);
+                if (sizeof(F) == 4 || a.gate_f32)
+                    store_row<float, VEC>(p, 0, static_cast<float *>(a.dgate) + at, o);
                 else
-                    store_row<F, VEC>(p, static_cast<F *>(a.dgate) + at, o);
+                    store_row<F, VEC>(p, 0, static_cast<F *>(a.dgate) + at, o);
             }
             if (gate_summed && on) {
 #pragma unroll
@@ -708,13 +899,13 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
                 for (int k = 0; k < 4; k++) {
                     v[k] = mul2(d[k], w[k]);
                     if (!VEC) {
-                        v[k].x = (p.valid >> (2 * k) & 1) ? v[k].x : 0.0f;
-                        v[k].y = (p.valid >> (2 * k) & 2) ? v[k].y : 0.0f;
+                        v[k].x = row_valid<VEC>(p, 0, 2 * k) ? v[k].x : 0.0f;
+                        v[k].y = row_valid<VEC>(p, 0, 2 * k + 1) ? v[k].y : 0.0f;
                     }
                     s1 = fma2(v[k], t[k], s1);
                 }
                 const bool layer = a.after == LUTB_NORM_LAYER, here_too = VEC ? p.valid != 0 : true;
-                const float2 c = row_sums(p, here_too ? s1.x + s1.y : 0.0f, layer && here_too ? total(v) : 0.0f, layer, [&]() {
+                const float2 c = row_sums<TEAM>(p, slots, here_too ? s1.x + s1.y : 0.0f, layer && here_too ? total(v) : 0.0f, layer, [&]() {
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
                         if (on) {
@@ -723,13 +914,13 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
                         }
                     }
                 });
-                const float c1 = -c.x / width, c2 = layer ? -c.y / width : 0.0f;
+                const float c1 = -c.x * p.inverse, c2 = layer ? -c.y * p.inverse : 0.0f;
 #pragma unroll
                 for (int k = 0; k < 4; k++) d[k] = mul2(both(st.y), fma2(t[k], both(c1), add2(v[k], both(c2))));
             }
             if (a.df && on) {
                 if (a.drop.on) drop8(d, kept, a.drop.scale);
-                store_row<F, VEC>(p, static_cast<F *>(a.df) + at, d);
+                store_row<F, VEC>(p, 0, static_cast<F *>(a.df) + at, d);
             }
         }
         here.next(a, p.teams, stride);
@@ -739,7 +930,7 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
                 v *= a.branch;
                 if (!a.gate_direct)
                     a.gate_sums[out + c] = v;
-                else if (a.gate_f32)
+                else if (sizeof(F) == 4 || a.gate_f32)
                     static_cast<float *>(a.dgate)[out + c] = v;
                 else
                     static_cast<F *>(a.dgate)[out + c] = from_f32<F>(v);
@@ -754,43 +945,63 @@ __global__ void __launch_bounds__(kRowMaxThreads, 2) join_rows_backward_kernel(c
             hand_out(sums[s], [&](int64_t c, float v) { to[c] = v; });
         }
     }
+    if (over_cluster<TEAM>(p)) cluster_meet();   // (no block is gone while another may store into it)
 }
 
 // ------------------------------------------------------------------------------------------------ launches
 int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs &a, const RowShape &s, int clusters, size_t smem, cudaStream_t stream);
 
-template <class X, class F, bool VEC>
-int launch_join_rows(bool backward, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream) {
-    static std::atomic<uint32_t> opted[2][6];
-    const int kind = (a.f == nullptr ? 0 : a.after == LUTB_NORM_NONE ? 1 : 2) * 2 + (backward ? a.dy != nullptr : a.y != nullptr);
-    const void *kernel = nullptr;
-#define LUTB_KIND(B, N)                                                                                      \
-    case 2 * B + N:                                                                                          \
-        kernel = backward ? reinterpret_cast<const void *>(&join_rows_backward_kernel<X, F, B, N != 0, VEC>) \
-                          : reinterpret_cast<const void *>(&join_rows_forward_kernel<X, F, B, N != 0, VEC>); \
-        break;
-    switch (kind) {
-        LUTB_KIND(0, 1)
-        LUTB_KIND(1, 0)
-        LUTB_KIND(1, 1)
-        LUTB_KIND(2, 0)
-        LUTB_KIND(2, 1)
-    }
-#undef LUTB_KIND
-    LUTB_REQUIRE(kernel != nullptr, LUTB_ERR_MODE, "nothing to compute");
-    const int gate = a.f != nullptr && a.gate_rows == 1 ? 2 : 0;
+// Shared memory of a block besides the kernel's own arrays.
+template <class X, class F>
+size_t join_rows_smem(bool backward, bool vec, const RowShape &s, bool gate_each) {
+    const int gate = gate_each ? 2 : 0;
     size_t parts = backward ? 2 * kBackwardParams : 0;
-    if (VEC) parts += backward ? (kBackwardParts<X, F> + gate) * kBackwardStages<X, F> : (kForwardParts<X, F> + gate) * kForwardStages;
-    return launch_rows(kernel, opted[backward][kind], a, s, clusters, parts * 16 * s.threads, stream);
+    if (vec) parts += (size_t)s.stages * (backward ? kBackwardParts<X, F> + gate : s.groups * (kForwardParts<X, F> + gate));
+    return parts * 16 * s.threads;
+}
+template <class X, class F, int BRANCH, bool NEXT>
+const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
+#define LUTB_FORWARD(VEC, G, TEAM) reinterpret_cast<const void *>(&join_rows_forward_kernel<X, F, BRANCH, NEXT, VEC, G, TEAM>)
+#define LUTB_BACKWARD(VEC, TEAM) reinterpret_cast<const void *>(&join_rows_backward_kernel<X, F, BRANCH, NEXT, VEC, TEAM>)
+    if (backward) {
+        if (!vec) return LUTB_BACKWARD(false, TEAM_ANY);
+        return s.kind == TEAM_WARP ? LUTB_BACKWARD(true, TEAM_WARP) : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(true, TEAM_BLOCK) : LUTB_BACKWARD(true, TEAM_CLUSTER);
+    }
+    if (!vec) return s.groups == 1 ? LUTB_FORWARD(false, 1, TEAM_ANY) : LUTB_FORWARD(false, 4, TEAM_ANY);
+    if (s.kind == TEAM_WARP) return s.groups == 1 ? LUTB_FORWARD(true, 1, TEAM_WARP) : LUTB_FORWARD(true, 4, TEAM_WARP);
+    return LUTB_FORWARD(true, 4, TEAM_BLOCK);
+#undef LUTB_FORWARD
+#undef LUTB_BACKWARD
+}
+template <class X, class F>
+int launch_join_rows(bool backward, bool vec, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream) {
+    static std::atomic<uint32_t> opted[2][2][6][6];
+    const int kind = (a.f == nullptr ? 0 : a.after == LUTB_NORM_NONE ? 1 : 2) * 2 + (backward ? a.dy != nullptr : a.y != nullptr);
+    const void *kernel = kind == 1   ? join_rows_kernel<X, F, 0, true>(backward, vec, s)
+                         : kind == 2 ? join_rows_kernel<X, F, 1, false>(backward, vec, s)
+                         : kind == 3 ? join_rows_kernel<X, F, 1, true>(backward, vec, s)
+                         : kind == 4 ? join_rows_kernel<X, F, 2, false>(backward, vec, s)
+                         : kind == 5 ? join_rows_kernel<X, F, 2, true>(backward, vec, s)
+                                     : nullptr;
+    LUTB_REQUIRE(kernel != nullptr, LUTB_ERR_MODE, "nothing to compute");
+    const size_t smem = join_rows_smem<X, F>(backward, vec, s, a.f != nullptr && a.gate_rows == 1);
+    return launch_rows(kernel, opted[backward][vec][kind][backward ? s.kind : 2 * s.kind + (s.groups > 1)], a, s, clusters, smem, stream);
 }
 
-// defined for each pair of types in a file of its own
-#define LUTB_JOIN_ROWS(X, F)                                                                                                              \
-    template <>                                                                                                                           \
-    int join_rows<X, F>(bool backward, bool vec, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream) {                \
-        return vec ? launch_join_rows<X, F, true>(backward, a, s, clusters, stream) : launch_join_rows<X, F, false>(backward, a, s, clusters, stream); \
-    }
+// for each pair of types in a file of its own
 template <class X, class F>
 int join_rows(bool backward, bool vec, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream);
+template <class X, class F>
+int join_rows_wait_errors(int *count);
+#define LUTB_JOIN_ROWS(X, F)                                                                                                        \
+    template <>                                                                                                                     \
+    int join_rows<X, F>(bool backward, bool vec, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream) {        \
+        return launch_join_rows<X, F>(backward, vec, a, s, clusters, stream);                                                      \
+    }                                                                                                                               \
+    template <>                                                                                                                     \
+    int join_rows_wait_errors<X, F>(int *count) {                                                                                   \
+        LUTB_CUDA(cudaMemcpyFromSymbol(count, g_join_wait_errors, sizeof(int)));                                                    \
+        return LUTB_OK;                                                                                                             \
+    }
 
 }  // namespace lutb
