@@ -522,7 +522,7 @@ int lutb_peer_sgd_update(int32_t n_ranks, int32_t rank, const float *const *grad
  * ---------------------------------------------------------------- what joins blocks in the residual stream
  * No counterpart in the reference, which composes torch modules here (dropout, BatchNorm1d, the sum; LUTTransformer.forward,
  * src/spiky/lut/LUTTransformer.py).  Arrays are contiguous, rows of `width` elements, and aligned to their elements (rows of a
- * multiple of eight elements in 16-byte aligned arrays take wide accesses).  Outputs overlap no input.
+ * multiple of eight elements, with inputs aligned to 16 bytes and outputs to 32, take wide accesses).  Outputs overlap no input.
  */
 #define LUTB_F32 0 /* element types */
 #define LUTB_BF16 1

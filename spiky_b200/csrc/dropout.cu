@@ -67,7 +67,7 @@ template <class T>
 static int launch_dropout(int64_t n, const void *x, void *y, const int64_t *random, uint64_t site, const DropRule &rule, cudaStream_t stream) {
     const T *from = static_cast<const T *>(x);
     T *to = static_cast<T *>(y);
-    const bool vec = (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(y)) % 16 == 0;
+    const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 32 == 0;
     const int64_t whole = vec ? n / 8 * 8 : 0, cap = (int64_t)device_info().sm_count * 8;
     if (whole) {
         const int64_t blocks = (whole / 8 + 511) / 512;

@@ -259,38 +259,77 @@ static auto by_types(const lutb_join_cfg *c, Fn fn) {
     return fn(float(), float());
 }
 
-constexpr size_t kForwardStatic = 10 * 1024, kBackwardStatic = 12 * 1024;   // the kernels' own arrays at most, and what a block takes beside them
-constexpr size_t kForwardVecStatic = 2 * 1024, kBackwardTeamStatic = 3 * 1024;
+// The kernels' own arrays at most, and what a block takes beside them.
+constexpr size_t kForwardStatic = 10 * 1024, kForwardVecStatic = 2 * 1024, kBackwardStatic = 12 * 1024, kBackwardTeamStatic = 4 * 1024;
 
-// Gives the shape its stages (the most of three with which as many threads as registers allow are resident, 512 an SM or, forward, 384; the most that fit
-// otherwise) and returns how many blocks the device holds.
+int resident_clusters(const void *kernel, const RowShape &s, size_t smem) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemPerBlock - kBackwardStatic) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3((unsigned)(s.cluster * 64));
+    config.blockDim = dim3((unsigned)s.threads);
+    config.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attribute[1];
+    attribute[0].id = cudaLaunchAttributeClusterDimension;
+    attribute[0].val.clusterDim.x = (unsigned)s.cluster;
+    attribute[0].val.clusterDim.y = attribute[0].val.clusterDim.z = 1;
+    config.attrs = attribute;
+    config.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kernel, &config) != cudaSuccess) {
+        cudaGetLastError();
+        return 0;
+    }
+    return n;
+}
+
+// Gives the shape its stages (the most of three with which as many threads as registers allow are resident, 512 an SM or, forward, 384; two or one
+// otherwise) and returns how many teams of blocks the device holds: a cluster beyond those would run in a second round.
 static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, RowShape &s) {
-    const int have = device_info().sm_count, sm = have > 0 ? have : 148;   // (no device: a size can be asked for all the same)
+    const DeviceInfo info = device_info();
+    const int sm = info.sm_count > 0 ? info.sm_count : 148;   // (no device: a size can be asked for all the same)
     const size_t own = backward ? (s.kind == TEAM_WARP ? kBackwardStatic : kBackwardTeamStatic) : vec ? kForwardVecStatic : kForwardStatic;
     const int most = 512 / s.threads, wanted = backward ? most : 384 / s.threads > 1 ? 384 / s.threads : 1;
     int blocks = 1;
+    size_t dynamic = 0;
     for (s.stages = 3; s.stages >= 1; s.stages--) {
-        const size_t dynamic = by_types(cfg, [&](auto xt, auto ft) { return join_rows_smem<decltype(xt), decltype(ft)>(backward, vec, s, cfg->gate_rows == 1); });
+        dynamic = by_types(cfg, [&](auto xt, auto ft) { return join_rows_smem<decltype(xt), decltype(ft)>(backward, vec, s, cfg->gate_rows == 1); });
         blocks = dynamic > kMaxSmemPerBlock - kBackwardStatic ? 0 : (int)(kMaxSmemPerBlock / (dynamic + own));
         if (blocks >= wanted || (s.stages == 2 && blocks >= 1) || s.stages == 1) break;
     }
-    return (int64_t)sm * (blocks < 1 ? 1 : blocks < most ? blocks : most);
+    blocks = blocks < 1 ? 1 : blocks < most ? blocks : most;
+    if (s.cluster == 1) return (int64_t)sm * blocks;
+    // (asking takes some twenty microseconds: the last answer for each pair of types is kept)
+    struct Asked {
+        int device, threads, cluster, clusters;
+        size_t smem;
+    };
+    static thread_local Asked kept[9] = {};
+    Asked &k = kept[cfg->stream_type * 3 + cfg->branch_type];
+    if (info.sm_count > 0 && (k.clusters == 0 || k.device != info.device || k.threads != s.threads || k.cluster != s.cluster || k.smem != dynamic))
+        k = {info.device, s.threads, s.cluster,
+             by_types(cfg, [&](auto xt, auto ft) { return join_rows_clusters<decltype(xt), decltype(ft)>(s, dynamic); }), dynamic};
+    return info.sm_count > 0 && k.clusters > 0 ? k.clusters : sm * blocks / s.cluster;
 }
-// How the rows are dealt, and to what shape of block (rows up to kRowMaxWidth have the row kernels).
+static bool row_kernels(const lutb_join_cfg *cfg) { return cfg->width <= kRowMaxWidth && cfg->rows <= kRowMaxRows; }
+
+// How the rows are dealt, and to what shape of block (unless rows are too wide or too many for the row kernels).
 static JoinSplit split_forward(const lutb_join_cfg *cfg, bool vec, RowShape &s) {
     const int have = device_info().sm_count;
-    if (cfg->width > kRowMaxWidth) return join_split(cfg->rows, cfg->rows, (have > 0 ? have : 148) * 8ll, 1);
+    if (!row_kernels(cfg)) return join_split(cfg->rows, cfg->rows, (have > 0 ? have : 148) * 8ll, 1);
     s = forward_shape(cfg->width, vec);
     const int64_t blocks = resident(cfg, false, vec, s);
     return join_split(cfg->rows, cfg->rows, blocks, s.teams);
 }
-static JoinSplit split_backward(const lutb_join_cfg *cfg, bool gate_gradient, RowShape &s) {
+static JoinSplit split_backward(const lutb_join_cfg *cfg, bool gate_gradient, bool vec, RowShape &s) {
     const int64_t group_rows = gate_gradient && cfg->gate_rows > 1 ? cfg->gate_rows : cfg->rows;
     const int have = device_info().sm_count;
-    if (cfg->width > kRowMaxWidth) return join_split(cfg->rows, group_rows, (have > 0 ? have : 148) * 4ll, 1);
+    if (!row_kernels(cfg)) return join_split(cfg->rows, group_rows, (have > 0 ? have : 148) * 4ll, 1);
     s = backward_shape(cfg->width);
-    const int64_t blocks = resident(cfg, true, true, s);
-    return join_split(cfg->rows, group_rows, blocks / s.cluster, s.teams);
+    const int64_t blocks = resident(cfg, true, vec, s);
+    return join_split(cfg->rows, group_rows, blocks, s.teams);
 }
 static void take_split(JoinArgs &a, const JoinSplit &s) {
     a.group_rows = s.group_rows;
@@ -328,10 +367,10 @@ int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs
     return LUTB_OK;
 }
 
-static bool all_aligned16(std::initializer_list<const void *> list) {
+static bool all_aligned(uintptr_t to, std::initializer_list<const void *> list) {
     uintptr_t all = 0;
     for (const void *p : list) all |= reinterpret_cast<uintptr_t>(p);
-    return all % 16 == 0;
+    return all % to == 0;
 }
 
 static int check_join(const lutb_join_cfg *c) {
@@ -409,14 +448,14 @@ extern "C" int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const 
     JoinArgs a = join_args(cfg);
     a.x = x; a.f = f; a.gate = gate; a.aw = after_weight; a.ab = after_bias; a.bw = before_weight; a.bb = before_bias;
     a.h = h; a.y = y; a.stats = reinterpret_cast<float4 *>(stats); a.random = random; a.gate_rows = cfg->gate_rows;
-    const bool vec = cfg->width % kRowElems == 0 && all_aligned16({x, f, gate, after_weight, after_bias, before_weight, before_bias, h, y});
+    const bool vec = cfg->width % kRowElems == 0 && all_aligned(16, {x, f, gate, after_weight, after_bias, before_weight, before_bias}) && all_aligned(32, {h, y});
     RowShape shape{};
     const JoinSplit split = split_forward(cfg, vec, shape);
     take_split(a, split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return by_types(cfg, [&](auto xt, auto ft) -> int {
         KernelScope scope(K_JOIN_FORWARD, s);
-        if (cfg->width <= kRowMaxWidth) return join_rows<decltype(xt), decltype(ft)>(false, vec, a, shape, split.blocks, s);
+        if (row_kernels(cfg)) return join_rows<decltype(xt), decltype(ft)>(false, vec, a, shape, split.blocks, s);
         join_forward_kernel<decltype(xt), decltype(ft)><<<split.blocks, kRowThreads, 0, s>>>(a);
         LUTB_LAUNCH_CHECK();
         return (int)LUTB_OK;
@@ -426,10 +465,15 @@ extern "C" int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const 
 extern "C" size_t lutb_join_backward_workspace(const lutb_join_cfg *cfg) {
     using namespace lutb;
     if (check_join(cfg) || cfg->rows == 0) return 0;
-    RowShape shape{};
-    const JoinSplit plain = split_backward(cfg, false, shape), gated = split_backward(cfg, true, shape);
-    const int64_t blocks = plain.blocks > gated.blocks ? plain.blocks : gated.blocks;
-    return (size_t)((4 * blocks + (cfg->gate_rows > 1 ? gated.chunks : 0)) * cfg->width) * sizeof(float);
+    size_t floats = 0;
+    for (int vec = 0; vec < 2; vec++)
+        for (int gated = 0; gated < 2; gated++) {
+            RowShape shape{};
+            const JoinSplit split = split_backward(cfg, gated != 0, vec != 0, shape);
+            const size_t need = (size_t)(4 * split.blocks + (gated && cfg->gate_rows > 1 ? split.chunks : 0)) * cfg->width;
+            floats = need > floats ? need : floats;
+        }
+    return floats * sizeof(float);
 }
 
 extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const void *f, const void *gate, const void *after_weight,
@@ -467,11 +511,13 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     a.stats = reinterpret_cast<float4 *>(const_cast<float *>(stats)); a.random = random;
     a.dh = dh; a.dy = dy; a.dx = dx; a.df = df; a.dgate = dgate;
     const bool gate_summed = dgate != nullptr && cfg->gate_rows > 1;
+    const bool vec = cfg->width % kRowElems == 0 &&
+                     all_aligned(16, {x, f, gate, after_weight, after_bias, before_weight, dh, dy}) && all_aligned(32, {dx, df, dgate});
     RowShape shape{};
-    const JoinSplit split = split_backward(cfg, dgate != nullptr, shape);
+    const JoinSplit split = split_backward(cfg, dgate != nullptr, vec, shape);
     take_split(a, split);
     a.gate_direct = gate_summed && split.per_group == 1;
-    const bool gate_parts = gate_summed && !(a.gate_direct && cfg->width <= kRowMaxWidth);   // (the kernel for wide rows sums there in any case)
+    const bool gate_parts = gate_summed && !(a.gate_direct && row_kernels(cfg));   // (the kernel for wide rows sums there in any case)
     SumList l{};
     float *at = static_cast<float *>(workspace);
     size_t need = 0;
@@ -490,12 +536,10 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     LUTB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need * sizeof(float)), LUTB_ERR_WORKSPACE,
                  "workspace of %zu bytes needed", need * sizeof(float));
     LUTB_REQUIRE(reinterpret_cast<uintptr_t>(workspace) % 16 == 0, LUTB_ERR_ALIGN, "workspace must be 16-byte aligned");
-    const bool vec = cfg->width % kRowElems == 0 &&
-                     all_aligned16({x, f, gate, after_weight, after_bias, before_weight, dh, dy, dx, df, dgate});
     return by_types(cfg, [&](auto xt, auto ft) -> int {
         {
             KernelScope scope(K_JOIN_BACKWARD, s);
-            if (cfg->width <= kRowMaxWidth) {
+            if (row_kernels(cfg)) {
                 if (int rc = join_rows<decltype(xt), decltype(ft)>(true, vec, a, shape, split.blocks, s)) return rc;
             } else {
                 join_backward_kernel<decltype(xt), decltype(ft)><<<split.blocks, kRowThreads, 0, s>>>(a);

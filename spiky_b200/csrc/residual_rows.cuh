@@ -6,9 +6,10 @@
 // formula of Chan, Golub and LeVeque, 1979, so that no square is taken about a mean that is far off).  What a team does depends on the width
 // alone, so that a row's result does not depend on the rows beside it.
 //
-// Rows in 16-byte aligned arrays of a multiple of eight elements (VEC): a group is eight neighbours, a thread fetches the groups of the next
-// rows with 16-byte asynchronous copies into slots of shared memory of its own (no barrier), and one generator block decides a group's mask.
-// Other rows: a thread's elements are a team apart, so that a warp's loads are neighbours, and the mask's bytes go through shared memory.
+// The next rows are fetched into shared memory with 16-byte asynchronous copies.  Rows of a multiple of eight elements in aligned arrays (VEC): a
+// group is eight neighbours, a warp fetches what its threads will read (no barrier of the block), and one generator block decides a group's
+// mask.  Other rows: the team fetches the aligned 16-byte pieces that its row touches, a thread's elements are a team apart, so that a
+// warp reads and stores neighbours, and the mask's bytes go through shared memory too.
 #pragma once
 
 #include <atomic>
@@ -21,6 +22,7 @@ namespace lutb {
 constexpr int kRowElems = 8;
 constexpr int kBackwardThreads = 256, kForwardThreads = 512, kRowMaxCluster = 8;
 constexpr int64_t kRowMaxWidth = 16384;   // 512 threads of four groups forward, eight blocks of 256 threads of one group backward
+constexpr int64_t kRowMaxRows = 1 << 30;  // (row numbers of 32 bits)
 
 
 enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_CLUSTER = 2, TEAM_ANY = 3 };   // ANY: told at run time (rows that are not VEC)
@@ -136,12 +138,12 @@ __device__ __forceinline__ void unpack8(const uint4 *part, float2 *v) {
 }
 template <class T>
 __device__ __forceinline__ void store8(T *p, const float2 *v) {
-    uint4 *q = reinterpret_cast<uint4 *>(p);
-    if constexpr (sizeof(T) == 4) {
-        q[0] = make_uint4(__float_as_uint(v[0].x), __float_as_uint(v[0].y), __float_as_uint(v[1].x), __float_as_uint(v[1].y));
-        q[1] = make_uint4(__float_as_uint(v[2].x), __float_as_uint(v[2].y), __float_as_uint(v[3].x), __float_as_uint(v[3].y));
+    if constexpr (sizeof(T) == 4) {   // (one store of a whole 32-byte sector; two of 16 bytes would each take half of every sector)
+        asm volatile("st.global.v8.f32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "f"(v[0].x), "f"(v[0].y), "f"(v[1].x), "f"(v[1].y),
+                     "f"(v[2].x), "f"(v[2].y), "f"(v[3].x), "f"(v[3].y)
+                     : "memory");
     } else {
-        q[0] = make_uint4(word_of(v[0], T()), word_of(v[1], T()), word_of(v[2], T()), word_of(v[3], T()));
+        *reinterpret_cast<uint4 *>(p) = make_uint4(word_of(v[0], T()), word_of(v[1], T()), word_of(v[2], T()), word_of(v[3], T()));
     }
 }
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
@@ -159,7 +161,7 @@ struct RowSlots {
 struct RowPlace {
     int t, team, teams, which;   // thread in its team; threads of a team, teams, this one
     int cluster, rank;
-    int64_t first;               // the block's first column
+    int first, limit;            // the block's columns: first .. limit - 1
     uint32_t valid;              // which elements exist: a bit a group (VEC) or an element
     uint32_t turn;               // exchanges so far
     float width, inverse;        // of a row, in elements
@@ -168,8 +170,8 @@ struct RowPlace {
 
 // Column k of group g.
 template <bool VEC>
-__device__ __forceinline__ int64_t row_column(const RowPlace &p, int g, int k) {
-    return VEC ? p.first + (int64_t)(g * p.team + p.t) * 8 + k : p.first + p.t + (int64_t)(g * 8 + k) * p.team;
+__device__ __forceinline__ int row_column(const RowPlace &p, int g, int k) {
+    return VEC ? p.first + (g * p.team + p.t) * 8 + k : p.first + p.t + (g * 8 + k) * p.team;
 }
 template <bool VEC>
 __device__ __forceinline__ bool row_valid(const RowPlace &p, int g, int k) { return p.valid >> (VEC ? g : g * 8 + k) & 1; }
@@ -180,42 +182,42 @@ __device__ __forceinline__ void cluster_sync() {
 // (no memory is handed over: nothing is waited for but the blocks themselves)
 __device__ __forceinline__ void cluster_meet() { asm volatile("barrier.cluster.arrive.relaxed;\n\tbarrier.cluster.wait;" ::: "memory"); }
 
-template <bool VEC, int G, class Slots>
+template <bool VEC, int G, int TEAM, class Slots>
 __device__ __forceinline__ RowPlace row_place(const JoinArgs &a, const RowShape &s, Slots &slots) {
     RowPlace p;
     const int tid = threadIdx.x;
     p.team = s.team;
-    p.teams = s.teams;
-    p.which = tid / s.team;
+    p.teams = TEAM == TEAM_BLOCK || TEAM == TEAM_CLUSTER ? 1 : s.teams;
+    p.which = p.teams == 1 ? 0 : tid / s.team;
     p.t = tid - p.which * s.team;
-    p.cluster = s.cluster;
-    p.rank = s.cluster > 1 ? (int)(blockIdx.x % s.cluster) : 0;
-    p.first = (int64_t)p.rank * s.slice;
+    p.cluster = TEAM == TEAM_WARP || TEAM == TEAM_BLOCK ? 1 : s.cluster;
+    p.rank = p.cluster > 1 ? (int)(blockIdx.x % p.cluster) : 0;
+    p.first = p.rank * s.slice;
+    p.limit = (int)min((int64_t)p.first + s.slice, a.width);
     p.width = (float)a.width;
     p.inverse = 1.0f / p.width;
     p.turn = 0;
     p.waits = true;
     p.valid = 0;
-    const int64_t limit = min(p.first + s.slice, a.width);
     int count = 0;
 #pragma unroll
     for (int g = 0; g < G; g++) {
         if (VEC) {
-            if (row_column<VEC>(p, g, 0) < limit) p.valid |= 1u << g, count += 8;
+            if (row_column<VEC>(p, g, 0) < p.limit) p.valid |= 1u << g, count += 8;
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                if (row_column<VEC>(p, g, k) < limit) p.valid |= 1u << (g * 8 + k), count++;
+                if (row_column<VEC>(p, g, k) < p.limit) p.valid |= 1u << (g * 8 + k), count++;
         }
     }
-    if (s.team > 32) {
+    if (TEAM != TEAM_WARP && s.team > 32) {
         constexpr int kAll = sizeof(slots.a[0]) / sizeof(float), kWarps = sizeof(slots.count) / sizeof(float);
         for (int k = tid; k < kAll; k += blockDim.x) slots.a[0][k] = slots.a[1][k] = slots.b[0][k] = slots.b[1][k] = 0.0f;
         if (tid < kWarps) slots.count[tid] = 0.0f;
         count = __reduce_add_sync(0xffffffffu, count);
         __syncthreads();
         if ((tid & 31) == 0) slots.count[tid >> 5] = (float)count;
-        if (s.cluster > 1) {
+        if (p.cluster > 1) {
             if (tid == 0) {
                 mbar_init(smem_u32(&slots.arrived[0]), 1);
                 mbar_init(smem_u32(&slots.arrived[1]), 1);
@@ -430,15 +432,15 @@ __device__ __forceinline__ void param8(const RowPlace &p, int g, const void *fro
 
 // The rows of a block in turn: chunk by chunk, `teams` rows at a time.
 struct RowCursor {
-    int64_t chunk, base, end;
+    int chunk, base, end;
     __device__ __forceinline__ void enter(const JoinArgs &a) {
-        if (chunk >= a.chunks) return;
-        const int64_t group = chunk / a.per_group;
-        base = group * a.group_rows + (chunk - group * a.per_group) * a.chunk_rows;
-        end = min(base + a.chunk_rows, min((group + 1) * a.group_rows, a.rows));
+        if (chunk >= (int)a.chunks) return;
+        const int per = (int)a.per_group, group = chunk / per, rows = (int)a.group_rows;
+        base = group * rows + (chunk - group * per) * (int)a.chunk_rows;
+        end = min(base + (int)a.chunk_rows, (group + 1) * rows);
     }
-    __device__ __forceinline__ bool more(const JoinArgs &a) const { return chunk < a.chunks; }
-    __device__ __forceinline__ void next(const JoinArgs &a, int teams, int64_t stride) {
+    __device__ __forceinline__ bool more(const JoinArgs &a) const { return chunk < (int)a.chunks; }
+    __device__ __forceinline__ void next(const JoinArgs &a, int teams, int stride) {
         base += teams;
         if (base >= end) {
             chunk += stride;
@@ -447,45 +449,109 @@ struct RowCursor {
     }
 };
 
-// The next rows' elements, in this thread's slots of shared memory.  With one stage a row is fetched when its turn comes.
+template <int TEAM>
+__device__ __forceinline__ void team_barrier(const RowPlace &p) {
+    if (within_warp<TEAM>(p))
+        __syncwarp();
+    else
+        __syncthreads();
+}
+
+// Bytes of the next rows' elements of one array in a stage.  Rows that are not VEC: a place of 32 bytes more than a row's for each team, for the aligned
+// pieces at its two ends.
+__host__ __device__ inline int ring_row_bytes(int slice, int size) { return (slice * size + 15) / 16 * 16 + 32; }
+__host__ __device__ inline int ring_bytes(bool vec, const RowShape &s, int size) {
+    return vec ? s.groups * kRowElems * size * s.threads : s.teams * ring_row_bytes(s.slice, size);
+}
+
+// With one stage a row is fetched when its turn comes, else one or two rows ahead.  The current row can be read to the end of its turn.
+template <bool VEC, int G, int TEAM>
 struct RowRing {
-    uint4 *at;          // [stage][part][thread], from this thread's first
-    int parts, threads, stages;
-    int fill, take;
-    template <int N>
-    __device__ __forceinline__ void fetch(int part, const void *from) const {
-        const uint32_t to = smem_u32(at + (fill * parts + part) * threads);
+    unsigned char *at;
+    int stage_bytes, stages, fill, take;
+
+    // What this thread fetches of a row of one array, whose place in a stage begins at `part`.
+    template <class T>
+    __device__ __forceinline__ void fetch(const RowPlace &p, const RowShape &s, int part, const T *from, int64_t row, const JoinArgs &a) const {
+        const uint32_t to = smem_u32(at) + fill * stage_bytes + part;
+        constexpr int kEach = 16 / sizeof(T);
+        if constexpr (VEC) {
+            // 16-byte pieces of a warp's (or a smaller team's) part of the row, one after another over its threads; those of eight 4-byte
+            // elements are two, swapped in every other four pairs, so that the threads' reads of their two pieces meet no bank twice
+            const int wide = min(p.team, 32), u = p.t & (wide - 1);
 #pragma unroll
-        for (int q = 0; q < N; q++) copy16(to + q * threads * 16, static_cast<const uint4 *>(from) + q);
+            for (int g = 0; g < G; g++) {
+                const int first = p.first + (g * p.team + p.t - u) * 8;
+                const uint32_t place = to + (g * (int)blockDim.x + threadIdx.x - u) * (kParts<T> * 16);
+#pragma unroll
+                for (int q = 0; q < kParts<T>; q++) {
+                    const int c = q * wide + u, column = first + c * kEach;
+                    if (column < p.limit) copy16(place + (kParts<T> == 2 ? c ^ (c >> 3 & 1) : c) * 16, from + row * a.width + column);
+                }
+            }
+        } else {
+            const int64_t begin = row * a.width + p.first, total = a.rows * a.width;
+            const unsigned char *const bytes = reinterpret_cast<const unsigned char *>(from);
+            const int ahead = (int)(reinterpret_cast<uintptr_t>(from + begin) & 15);   // of the row in its first piece
+            const int pieces = (ahead + (p.limit - p.first) * (int)sizeof(T) + 15) / 16;
+            const uint32_t place = to + p.which * ring_row_bytes(s.slice, sizeof(T));
+            for (int c = p.t; c < pieces; c += p.team) {
+                const int64_t offset = begin * (int64_t)sizeof(T) - ahead + c * 16;   // from the array's begin
+                if (offset >= 0 && offset + 16 <= total * (int64_t)sizeof(T)) {
+                    copy16(place + c * 16, bytes + offset);
+                } else {   // a piece that the array does not fill: its elements one by one
+                    T *const own = reinterpret_cast<T *>(at + fill * stage_bytes + part + p.which * ring_row_bytes(s.slice, sizeof(T)) + c * 16);
+                    const int64_t element = (begin * (int64_t)sizeof(T) - ahead) / (int64_t)sizeof(T) + c * kEach;
+#pragma unroll
+                    for (int e = 0; e < kEach; e++)
+                        if (element + e >= 0 && element + e < total) own[e] = from[element + e];
+                }
+            }
+        }
     }
     __device__ __forceinline__ void filled() {
         asm volatile("cp.async.commit_group;" ::: "memory");
         fill = fill + 1 == stages ? 0 : fill + 1;
     }
-    __device__ __forceinline__ void ready() const {
+    // The current row's elements are there, for the team; what was read of the row before may be overwritten.
+    __device__ __forceinline__ void ready(const RowPlace &p) const {
         if (stages == 3)
             asm volatile("cp.async.wait_group 1;" ::: "memory");
         else
             asm volatile("cp.async.wait_group 0;" ::: "memory");
+        if (VEC)
+            __syncwarp();
+        else
+            team_barrier<TEAM>(p);
     }
     __device__ __forceinline__ void taken() { take = take + 1 == stages ? 0 : take + 1; }
+    // Eight elements; 0 where there are none.
     template <class T>
-    __device__ __forceinline__ void get(int part, float2 *v) const {
-        uint4 w[kParts<T>];
+    __device__ __forceinline__ void get(const RowPlace &p, const RowShape &s, int g, int part, const T *from, int64_t begin, bool on, float2 *v) const {
+        const unsigned char *const stage = at + take * stage_bytes + part;
+        if constexpr (VEC) {
+            if (!on || !row_valid<VEC>(p, g, 0)) {
+                zero8(v);
+                return;
+            }
+            const int wide = min(p.team, 32), u = p.t & (wide - 1), turned = kParts<T> == 2 ? u >> 2 & 1 : 0;
+            const uint4 *const own = reinterpret_cast<const uint4 *>(stage) + (g * (int)blockDim.x + threadIdx.x - u) * kParts<T> + kParts<T> * u;
+            uint4 w[kParts<T>];
 #pragma unroll
-        for (int q = 0; q < kParts<T>; q++) w[q] = at[(take * parts + part + q) * threads];
-        unpack8<T>(w, v);
+            for (int q = 0; q < kParts<T>; q++) w[q] = own[q ^ turned];
+            unpack8<T>(w, v);
+        } else {
+            const int ahead = (int)(reinterpret_cast<uintptr_t>(from + begin + p.first) & 15) / (int)sizeof(T);
+            const T *const own = reinterpret_cast<const T *>(stage + p.which * ring_row_bytes(s.slice, sizeof(T))) + ahead - p.first;
+            float e[8];
+#pragma unroll
+            for (int k = 0; k < 8; k++) e[k] = on && row_valid<VEC>(p, g, k) ? to_f32(own[row_column<VEC>(p, g, k)]) : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
+        }
     }
 };
 
-template <class T, bool VEC>
-__device__ __forceinline__ void load_apart(const RowPlace &p, int g, const T *row, bool on, float2 *v) {
-    float e[8];
-#pragma unroll
-    for (int k = 0; k < 8; k++) e[k] = on && row_valid<VEC>(p, g, k) ? to_f32(row[row_column<VEC>(p, g, k)]) : 0.0f;
-#pragma unroll
-    for (int k = 0; k < 4; k++) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
-}
 template <class T, bool VEC>
 __device__ __forceinline__ void store_row(const RowPlace &p, int g, T *row, const float2 *v) {
     if constexpr (VEC) {
@@ -497,26 +563,28 @@ __device__ __forceinline__ void store_row(const RowPlace &p, int g, T *row, cons
     }
 }
 
-// The masks of a thread's groups, eight bits each.  Rows that are not VEC: the team's generator blocks as bytes in shared memory, two sets
-// in turn, so that one barrier a row is enough.
+// The masks of a thread's groups, eight bits each.  Rows that are not VEC: the team's generator blocks as bytes in shared memory, written before
+// the row's barrier and read after it, two sets in turn.
 template <bool VEC, int G>
-__device__ __forceinline__ uint32_t row_mask(const RowPlace &p, const JoinArgs &a, const DropKey &key, int64_t row, uint8_t *bytes, uint32_t set) {
-    const int64_t at = row * a.width + p.first;
-    uint32_t kept = 0;
+__device__ __forceinline__ uint32_t form_mask(const RowPlace &p, const JoinArgs &a, const DropKey &key, int64_t row, uint8_t *bytes, uint32_t set) {
+    const uint64_t block = (uint64_t)(row * a.width + p.first) >> 3;
     if (VEC) {
+        uint32_t kept = 0;
 #pragma unroll
-        for (int g = 0; g < G; g++) kept |= keep_bits((uint64_t)(at >> 3) + g * p.team + p.t, key, a.drop) << (8 * g);
+        for (int g = 0; g < G; g++) kept |= keep_bits(block + g * p.team + p.t, key, a.drop) << (8 * g);
         return kept;
     }
     uint8_t *own = bytes + ((int)set * p.teams + p.which) * (G * p.team + 1);
-    const int off = (int)(at & 7);
 #pragma unroll
-    for (int g = 0; g < G; g++) own[g * p.team + p.t] = (uint8_t)keep_bits((uint64_t)(at >> 3) + g * p.team + p.t, key, a.drop);
-    if (p.t == 0) own[G * p.team] = (uint8_t)keep_bits((uint64_t)(at >> 3) + G * p.team, key, a.drop);
-    if (p.team <= 32)
-        __syncwarp();
-    else
-        __syncthreads();
+    for (int g = 0; g < G; g++) own[g * p.team + p.t] = (uint8_t)keep_bits(block + g * p.team + p.t, key, a.drop);
+    if (p.t == 0) own[G * p.team] = (uint8_t)keep_bits(block + G * p.team, key, a.drop);
+    return 0;
+}
+template <int G>
+__device__ __forceinline__ uint32_t read_mask(const RowPlace &p, const JoinArgs &a, int64_t row, const uint8_t *bytes, uint32_t set) {
+    const uint8_t *own = bytes + ((int)set * p.teams + p.which) * (G * p.team + 1);
+    const int off = (int)((row * a.width + p.first) & 7);
+    uint32_t kept = 0;
 #pragma unroll
     for (int k = 0; k < 8 * G; k++) {
         const int e = off + p.t + k * p.team;
@@ -525,86 +593,75 @@ __device__ __forceinline__ uint32_t row_mask(const RowPlace &p, const JoinArgs &
     return kept;
 }
 template <int G, int THREADS>
-constexpr size_t kMaskBytes = 2 * (G * THREADS + THREADS);   // two sets, a byte a group and one a team
+constexpr size_t kMaskBytes = 2 * (G * THREADS + THREADS);   // two sets, a byte a group and one more a team
 
 // ------------------------------------------------------------------------------------------------ forward
 // BRANCH: 0 no branch (the norm alone), 1 a branch, 2 a branch with a norm of its own.  NEXT: the norm before the next block.
-template <class X, class F>
-constexpr int kForwardParts = kParts<X> + kParts<F>;   // of a group: x, f; two more for a gate of each element
 template <int G, int TEAM>
 constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : G == 1 ? 256 : kForwardThreads;
 
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int G, int TEAM>
 __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
     constexpr int kThreads = kThreadsOf<G, TEAM>;
-    extern __shared__ uint4 dynamic[];
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) RowSlots<TEAM == TEAM_WARP ? 4 : kThreads / 32, 1> slots;
     __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<G, kThreads>];
-    RowPlace p = row_place<VEC, G>(a, shape, slots);
+    RowPlace p = row_place<VEC, G, TEAM>(a, shape, slots);
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
-    const bool gate_each = BRANCH && a.gate_rows == 1;
-    constexpr int kX = 0, kF = kParts<X>, kGate = kForwardParts<X, F>;
-    const int parts = kForwardParts<X, F> + (gate_each ? 2 : 0);
-    RowRing ring{dynamic + threadIdx.x, G * parts, (int)blockDim.x, shape.stages, 0, 0};
-    const int64_t stride = gridDim.x;
-    RowCursor load{(int64_t)blockIdx.x, 0, 0}, here = load;
-    load.enter(a);
-    here = load;
+    const bool gate_each = BRANCH && a.gate_rows == 1, gate_f32 = sizeof(F) == 4 || a.gate_f32;
+    const int part_f = ring_bytes(VEC, shape, sizeof(X)), part_gate = part_f + (BRANCH ? ring_bytes(VEC, shape, sizeof(F)) : 0);
+    RowRing<VEC, G, TEAM> ring{dynamic, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0), shape.stages, 0, 0};
     const X *const x_in = static_cast<const X *>(a.x);
     const F *const f_in = static_cast<const F *>(a.f);
+    RowCursor load{(int)blockIdx.x, 0, 0}, here;
+    load.enter(a);
+    here = load;
     auto fetch = [&]() {
-        if (VEC) {
-            if (load.more(a)) {
-                const int64_t row = load.base + p.which, at = row * a.width;
-                if (row < load.end) {
-#pragma unroll
-                    for (int g = 0; g < G; g++) {
-                        if (!row_valid<VEC>(p, g, 0)) break;
-                        const int64_t c = at + row_column<VEC>(p, g, 0);
-                        ring.fetch<kParts<X>>(g * parts + kX, x_in + c);
-                        if (BRANCH) ring.fetch<kParts<F>>(g * parts + kF, f_in + c);
-                        if (gate_each) {
-                            if (sizeof(F) == 4 || a.gate_f32)
-                                ring.fetch<2>(g * parts + kGate, static_cast<const float *>(a.gate) + c);
-                            else
-                                ring.fetch<kParts<F>>(g * parts + kGate, static_cast<const F *>(a.gate) + c);
-                        }
-                    }
+        if (load.more(a)) {
+            const int64_t row = load.base + p.which;
+            if (row < load.end) {
+                ring.template fetch<X>(p, shape, 0, x_in, row, a);
+                if (BRANCH) ring.template fetch<F>(p, shape, part_f, f_in, row, a);
+                if (gate_each) {
+                    if (gate_f32)
+                        ring.template fetch<float>(p, shape, part_gate, static_cast<const float *>(a.gate), row, a);
+                    else
+                        ring.template fetch<F>(p, shape, part_gate, static_cast<const F *>(a.gate), row, a);
                 }
-                load.next(a, p.teams, stride);
             }
-            ring.filled();
+            load.next(a, p.teams, gridDim.x);
         }
+        ring.filled();
     };
     for (int s = 1; s < shape.stages; s++) fetch();
     uint32_t set = 0;
-    int64_t gate_at = 0, gate_end = 0;   // the gate row in use, the first row of another one
-    for (; here.more(a); here.next(a, p.teams, stride)) {
-        const int64_t row = here.base + p.which, at = row * a.width;
+    int64_t gate_at = 0;   // the gate row in use
+    int gate_end = 0;      // the first row of another one
+    for (; here.more(a); here.next(a, p.teams, gridDim.x)) {
+        const int row = here.base + p.which;
+        const int64_t at = row * a.width;
         const bool on = row < here.end;
         if (BRANCH && a.gate_rows > 1 && on && row >= gate_end) {
-            const int64_t gate_row = row / a.gate_rows;
-            gate_end = (gate_row + 1) * a.gate_rows;
+            const int gate_row = row / (int)a.gate_rows;
+            gate_end = (gate_row + 1) * (int)a.gate_rows;
             gate_at = gate_row * a.width;
         }
         uint32_t kept = 0xffffffffu;
-        if (BRANCH && a.drop.on) kept = row_mask<VEC, G>(p, a, key, row, masks, set);
+        if (BRANCH && a.drop.on) kept = form_mask<VEC, G>(p, a, key, row, masks, set);
+        if (shape.stages == 1) {
+            team_barrier<TEAM>(p);
+            fetch();
+        }
+        ring.ready(p);
+        if (!VEC && BRANCH && a.drop.on) kept = read_mask<G>(p, a, row, masks, set);
         set ^= 1;
+        if (shape.stages > 1) fetch();
         float2 v[G][4];
         float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
-        if (VEC) {
-            if (shape.stages == 1) fetch();
-            ring.ready();
-        }
         if (BRANCH) {
 #pragma unroll
             for (int g = 0; g < G; g++) {
-                if (VEC) {
-                    ring.get<F>(g * parts + kF, v[g]);
-                    if (!on || !row_valid<VEC>(p, g, 0)) zero8(v[g]);
-                } else {
-                    load_apart<F, VEC>(p, g, f_in + at, on, v[g]);
-                }
+                ring.template get<F>(p, shape, g, part_f, f_in, at, on, v[g]);
                 if (a.drop.on) drop8(v[g], kept >> (8 * g), a.drop.scale);
             }
         }
@@ -624,41 +681,23 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
 #pragma unroll
         for (int g = 0; g < G; g++) {
             float2 x[4];
-            if (VEC) {
-                ring.get<X>(g * parts + kX, x);
-                if (!on || !row_valid<VEC>(p, g, 0)) zero8(x);
-            } else {
-                load_apart<X, VEC>(p, g, x_in + at, on, x);
-            }
+            ring.template get<X>(p, shape, g, 0, x_in, at, on, x);
             if (BRANCH) {
                 float2 gate[4];
-                if (!gate_each) {
-                    param8<F, VEC>(p, g, a.gate, a.gate_f32, gate_at, 1.0f, gate);
-                } else if (VEC) {
-                    if (sizeof(F) == 4 || a.gate_f32)
-                        ring.get<float>(g * parts + kGate, gate);
-                    else
-                        ring.get<F>(g * parts + kGate, gate);
-                    if (!on || !row_valid<VEC>(p, g, 0)) zero8(gate);
-                } else if (a.gate_f32) {
-                    load_apart<float, VEC>(p, g, static_cast<const float *>(a.gate) + at, on, gate);
-                } else {
-                    load_apart<F, VEC>(p, g, static_cast<const F *>(a.gate) + at, on, gate);
-                }
+                if (!gate_each)
+                    param8<F, VEC>(p, g, a.gate, gate_f32, gate_at, 1.0f, gate);
+                else if (gate_f32)
+                    ring.template get<float>(p, shape, g, part_gate, static_cast<const float *>(a.gate), at, on, gate);
+                else
+                    ring.template get<F>(p, shape, g, part_gate, static_cast<const F *>(a.gate), at, on, gate);
 #pragma unroll
                 for (int k = 0; k < 4; k++) v[g][k] = fma2(mul2(gate[k], both(a.branch)), v[g][k], mul2(x[k], both(a.skip)));
+                if (on) store_row<X, VEC>(p, g, static_cast<X *>(a.h) + at, v[g]);
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; k++) v[g][k] = x[k];
             }
         }
-        if (VEC) {
-            ring.taken();
-            if (shape.stages > 1) fetch();
-        }
-        if (BRANCH && on)
-#pragma unroll
-            for (int g = 0; g < G; g++) store_row<X, VEC>(p, g, static_cast<X *>(a.h) + at, v[g]);
         if (NEXT) {
             const float2 s = row_stats<VEC, G, TEAM>(p, slots, v, a.before == LUTB_NORM_LAYER, a.eps);
             st.z = s.x;
@@ -675,23 +714,23 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
                 }
         }
         if (a.stats && on && p.t == 0) a.stats[row] = st;
+        ring.taken();
     }
 }
 
 // ------------------------------------------------------------------------------------------------ backward
-template <class X, class F>
-constexpr int kBackwardParts = 2 * kParts<X> + 2 * kParts<F>;   // x, dh, f, dy; two more for a gate of each element
 constexpr int kBackwardParams = 4;   // aw, ab, bw, gate
 
-// See join_backward_kernel for the formulas.  A thread's sums over its rows stay in registers to the end (of the chunk, for a gate row).
+// See join_backward_kernel for the formulas.  A thread's sums over its rows stay in registers to the end (of the chunk, for a gate row); what a step
+// needs of the row is read from shared memory at that step, so that three sets of eight values are live at most beside the forty sums.
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int TEAM>
 __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel(const JoinArgs a, const RowShape shape) {
     constexpr bool kTeams = TEAM == TEAM_WARP || TEAM == TEAM_ANY, kClusters = TEAM == TEAM_CLUSTER || TEAM == TEAM_ANY;
-    extern __shared__ uint4 dynamic[];
+    extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) RowSlots<kBackwardThreads / 32, kClusters ? kRowMaxCluster : 1> slots;
     __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<1, kBackwardThreads>];
     __shared__ float2 joined[kTeams ? 4 * kBackwardThreads : 1];   // the teams' sums of a block
-    RowPlace p = row_place<VEC, 1>(a, shape, slots);
+    RowPlace p = row_place<VEC, 1, TEAM>(a, shape, slots);
     const int threads = blockDim.x, tid = threadIdx.x;
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
     // parameters in slots of this thread's own: [parameter][half][thread]
@@ -716,38 +755,40 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
         keep_param(1, a.ab, a.params_f32, 0, 0.0f, 1.0f);
     }
     if (NEXT) keep_param(2, a.bw, a.params_f32, 0, 1.0f, 1.0f);
-    const bool gate_each = BRANCH && a.gate_rows == 1, gate_summed = BRANCH && a.dgate && a.gate_rows > 1;
-    int64_t gate_end = 0;   // first row of another gate row
+    const bool gate_each = BRANCH && a.gate_rows == 1, gate_summed = BRANCH && a.dgate && a.gate_rows > 1, gate_f32 = sizeof(F) == 4 || a.gate_f32;
+    int gate_end = 0;   // first row of another gate row
     if (BRANCH && a.gate_rows == 0) keep_param(3, nullptr, true, 0, 1.0f, a.branch);
 
-    RowRing ring{dynamic + 2 * kBackwardParams * threads + tid, kBackwardParts<X, F> + (gate_each ? 2 : 0), threads, shape.stages, 0, 0};
-    constexpr int kDh = kParts<X>, kF = 2 * kParts<X>, kDy = kF + kParts<F>, kGate = kDy + kParts<F>;
-    const int64_t stride = gridDim.x / shape.cluster, own = blockIdx.x / shape.cluster;
-    RowCursor load{own, 0, 0}, here = load;
-    load.enter(a);
-    here = load;
     const X *const x_in = static_cast<const X *>(a.x), *const dh_in = static_cast<const X *>(a.dh);
     const F *const f_in = static_cast<const F *>(a.f), *const dy_in = static_cast<const F *>(a.dy);
+    const int bytes_x = ring_bytes(VEC, shape, sizeof(X)), bytes_f = ring_bytes(VEC, shape, sizeof(F));
+    const int part_dh = NEXT ? bytes_x : 0, part_f = part_dh + bytes_x, part_dy = part_f + (BRANCH ? bytes_f : 0), part_gate = part_dy + (NEXT ? bytes_f : 0);
+    RowRing<VEC, 1, TEAM> ring{dynamic + 2 * kBackwardParams * 16 * threads, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0),
+                               shape.stages, 0, 0};
+    const int stride = gridDim.x / p.cluster, own = blockIdx.x / p.cluster;
+    RowCursor load{own, 0, 0}, here;
+    load.enter(a);
+    here = load;
     auto fetch = [&]() {
-        if (VEC) {
-            if (load.more(a)) {
-                const int64_t row = load.base + p.which, at = row * a.width + row_column<VEC>(p, 0, 0);
-                if (row < load.end && p.valid) {
-                    if (NEXT) ring.fetch<kParts<X>>(0, x_in + at);
-                    if (dh_in) ring.fetch<kParts<X>>(kDh, dh_in + at);
-                    if (BRANCH) ring.fetch<kParts<F>>(kF, f_in + at);
-                    if (NEXT) ring.fetch<kParts<F>>(kDy, dy_in + at);
-                    if (gate_each) {
-                        if (sizeof(F) == 4 || a.gate_f32)
-                            ring.fetch<2>(kGate, static_cast<const float *>(a.gate) + at);
-                        else
-                            ring.fetch<kParts<F>>(kGate, static_cast<const F *>(a.gate) + at);
-                    }
+        if (load.more(a)) {
+            const int64_t row = load.base + p.which;
+            if (row < load.end) {
+                if (BRANCH) ring.template fetch<F>(p, shape, part_f, f_in, row, a);
+                if (NEXT) {
+                    ring.template fetch<X>(p, shape, 0, x_in, row, a);
+                    ring.template fetch<F>(p, shape, part_dy, dy_in, row, a);
                 }
-                load.next(a, p.teams, stride);
+                if (dh_in) ring.template fetch<X>(p, shape, part_dh, dh_in, row, a);
+                if (gate_each) {
+                    if (gate_f32)
+                        ring.template fetch<float>(p, shape, part_gate, static_cast<const float *>(a.gate), row, a);
+                    else
+                        ring.template fetch<F>(p, shape, part_gate, static_cast<const F *>(a.gate), row, a);
+                }
             }
-            ring.filled();
+            load.next(a, p.teams, stride);
         }
+        ring.filled();
     };
     constexpr int kSums = 5;   // daw, dab, dbw, dbb, gate
     float2 sums[kSums][4];
@@ -769,107 +810,101 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
         for (int c = tid; c < (int)a.width; c += threads) {
             float s = 0.0f;
             for (int w = 0; w < p.teams; w++) s += all[w * p.team * 8 + c];
-            put((int64_t)c, s);
+            put(c, s);
         }
     };
     for (int s = 1; s < shape.stages; s++) fetch();
     uint32_t set = 0;
     while (here.more(a)) {
-        const int64_t row = here.base + p.which, at = row * a.width, chunk = here.chunk;
+        const int row = here.base + p.which, chunk = here.chunk;
+        const int64_t at = row * a.width;
         const bool on = row < here.end;
         const float4 st = on ? a.stats[row] : make_float4(0.0f, 1.0f, 0.0f, 1.0f);
         if (BRANCH && a.gate_rows > 1 && on && row >= gate_end) {
-            const int64_t gate_row = row / a.gate_rows;
-            gate_end = (gate_row + 1) * a.gate_rows;
-            keep_param(3, a.gate, a.gate_f32, gate_row * a.width, 1.0f, a.branch);
+            const int gate_row = row / (int)a.gate_rows;
+            gate_end = (gate_row + 1) * (int)a.gate_rows;
+            keep_param(3, a.gate, gate_f32, gate_row * a.width, 1.0f, a.branch);
         }
-        uint32_t kept = 0xffu;
-        if (BRANCH && a.drop.on) kept = row_mask<VEC, 1>(p, a, key, row, masks, set);
-        set ^= 1;
-        float2 d[4], t[4], z[4], g[4];   // dh, the branch, the stream, dy
-        if (VEC) {
-            if (shape.stages == 1) fetch();
-            ring.ready();
-            if (NEXT) ring.get<X>(0, z);
-            if (dh_in) ring.get<X>(kDh, d);
-            if (BRANCH) ring.get<F>(kF, t);
-            if (NEXT) ring.get<F>(kDy, g);
-        } else {
-            if (NEXT) load_apart<X, VEC>(p, 0, x_in + at, on, z);
-            if (dh_in) load_apart<X, VEC>(p, 0, dh_in + at, on, d);
-            if (BRANCH) load_apart<F, VEC>(p, 0, f_in + at, on, t);
-            if (NEXT) load_apart<F, VEC>(p, 0, dy_in + at, on, g);
-        }
-        if (dh_in == nullptr || (VEC && (!on || !p.valid))) zero8(d);
-        if (VEC && (!on || !p.valid)) {
-            if (NEXT) zero8(z);
-            if (BRANCH) zero8(t);
-            if (NEXT) zero8(g);
-        }
-        float2 gate[4], w[4];
-        if (BRANCH) {
-            if (!gate_each)
-                param(3, gate);
-            else {
-                if (VEC) {
-                    if (sizeof(F) == 4 || a.gate_f32)
-                        ring.get<float>(kGate, gate);
-                    else
-                        ring.get<F>(kGate, gate);
-                    if (!on || !p.valid) zero8(gate);
-                } else if (a.gate_f32) {
-                    load_apart<float, VEC>(p, 0, static_cast<const float *>(a.gate) + at, on, gate);
-                } else {
-                    load_apart<F, VEC>(p, 0, static_cast<const F *>(a.gate) + at, on, gate);
-                }
-#pragma unroll
-                for (int k = 0; k < 4; k++) gate[k] = mul2(gate[k], both(a.branch));
+        auto gate_of = [&](float2 *v) {   // times the branch's scale
+            if (!gate_each) {
+                param(3, v);
+                return;
             }
-        }
-        if (VEC) {
-            ring.taken();
-            if (shape.stages > 1) fetch();
-        }
-        float2 n[4];   // the branch after its norm; t becomes its normalised values
-        if (BRANCH) {
-            if (a.drop.on) drop8(t, kept, a.drop.scale);
-            if (BRANCH == 2) {
-                float2 shift[4];
-                param(0, w);
-                param(1, shift);
+            if (gate_f32)
+                ring.template get<float>(p, shape, 0, part_gate, static_cast<const float *>(a.gate), at, on, v);
+            else
+                ring.template get<F>(p, shape, 0, part_gate, static_cast<const F *>(a.gate), at, on, v);
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    t[k] = mul2(add2(t[k], both(-st.x)), both(st.y));
-                    n[k] = fma2(t[k], w[k], shift[k]);
-                }
+            for (int k = 0; k < 4; k++) v[k] = mul2(v[k], both(a.branch));
+        };
+        uint32_t kept = 0xffu;
+        if (BRANCH && a.drop.on) kept = form_mask<VEC, 1>(p, a, key, row, masks, set);
+        if (shape.stages == 1) {
+            team_barrier<TEAM>(p);
+            fetch();
+        }
+        ring.ready(p);
+        if (!VEC && BRANCH && a.drop.on) kept = read_mask<1>(p, a, row, masks, set);
+        set ^= 1;
+        if (shape.stages > 1) fetch();
+        float2 t[4];   // the branch, from its norm on normalised
+        if (BRANCH) {
+            ring.template get<F>(p, shape, 0, part_f, f_in, at, on, t);
+            if (a.drop.on) drop8(t, kept, a.drop.scale);
+            if (BRANCH == 2)
+#pragma unroll
+                for (int k = 0; k < 4; k++) t[k] = mul2(add2(t[k], both(-st.x)), both(st.y));
+        }
+        auto branch_out = [&](float2 *n) {   // the branch after its norm
+            if (BRANCH == 2) {
+                float2 w[4], b[4];
+                param(0, w);
+                param(1, b);
+#pragma unroll
+                for (int k = 0; k < 4; k++) n[k] = fma2(t[k], w[k], b[k]);
             } else {
 #pragma unroll
                 for (int k = 0; k < 4; k++) n[k] = t[k];
             }
-        }
+        };
+        float2 d[4];   // the gradient on its way
         if (NEXT) {
-            float2 u[4], s1 = make_float2(0.0f, 0.0f), bw[4];
-            param(2, bw);
+            float2 z[4], u[4], s1 = make_float2(0.0f, 0.0f);   // the stream normalised, dy bw
+            ring.template get<X>(p, shape, 0, 0, x_in, at, on, z);
+            if (BRANCH) {
+                float2 n[4], gate[4];
+                branch_out(n);
+                gate_of(gate);
+#pragma unroll
+                for (int k = 0; k < 4; k++) z[k] = fma2(gate[k], n[k], mul2(z[k], both(a.skip)));
+            }
+            float2 g[4];
+            ring.template get<F>(p, shape, 0, part_dy, dy_in, at, on, g);
+            param(2, u);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                if (BRANCH) z[k] = fma2(gate[k], n[k], mul2(z[k], both(a.skip)));
                 z[k] = mul2(add2(z[k], both(-st.z)), both(st.w));
-                u[k] = mul2(g[k], bw[k]);
+                u[k] = mul2(g[k], u[k]);
                 s1 = fma2(u[k], z[k], s1);
             }
             const bool layer = a.before == LUTB_NORM_LAYER;
             const float2 c = row_sums<TEAM>(p, slots, s1.x + s1.y, layer ? total(u) : 0.0f, layer, [&]() {
+                if (!on) return;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
-                    if (on) {
-                        sums[2][k] = fma2(g[k], z[k], sums[2][k]);
-                        sums[3][k] = add2(sums[3][k], g[k]);
-                    }
+                    sums[2][k] = fma2(g[k], z[k], sums[2][k]);
+                    sums[3][k] = add2(sums[3][k], g[k]);
                 }
             });
             const float c1 = -c.x * p.inverse, c2 = layer ? -c.y * p.inverse : 0.0f;
+            if (dh_in)
+                ring.template get<X>(p, shape, 0, part_dh, dh_in, at, on, d);
+            else
+                zero8(d);
 #pragma unroll
             for (int k = 0; k < 4; k++) d[k] = fma2(both(st.w), fma2(z[k], both(c1), add2(u[k], both(c2))), d[k]);
+        } else {
+            ring.template get<X>(p, shape, 0, part_dh, dh_in, at, on, d);
         }
         if (a.dx && on) {
             float2 o[4];
@@ -878,59 +913,65 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
             store_row<X, VEC>(p, 0, static_cast<X *>(a.dx) + at, o);
         }
         if (BRANCH) {
-            if (gate_each && a.dgate && on) {
-                float2 o[4];
+            if (a.dgate && on) {
+                float2 n[4];
+                branch_out(n);
+                if (gate_summed) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) o[k] = mul2(mul2(d[k], both(a.branch)), n[k]);
-                if (sizeof(F) == 4 || a.gate_f32)
-                    store_row<float, VEC>(p, 0, static_cast<float *>(a.dgate) + at, o);
-                else
-                    store_row<F, VEC>(p, 0, static_cast<F *>(a.dgate) + at, o);
-            }
-            if (gate_summed && on) {
+                    for (int k = 0; k < 4; k++) sums[4][k] = fma2(d[k], n[k], sums[4][k]);
+                } else {
 #pragma unroll
-                for (int k = 0; k < 4; k++) sums[4][k] = fma2(d[k], n[k], sums[4][k]);
-            }
-#pragma unroll
-            for (int k = 0; k < 4; k++) d[k] = mul2(d[k], gate[k]);
-            if (BRANCH == 2) {
-                float2 v[4], s1 = make_float2(0.0f, 0.0f);
-#pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    v[k] = mul2(d[k], w[k]);
-                    if (!VEC) {
-                        v[k].x = row_valid<VEC>(p, 0, 2 * k) ? v[k].x : 0.0f;
-                        v[k].y = row_valid<VEC>(p, 0, 2 * k + 1) ? v[k].y : 0.0f;
-                    }
-                    s1 = fma2(v[k], t[k], s1);
+                    for (int k = 0; k < 4; k++) n[k] = mul2(mul2(d[k], both(a.branch)), n[k]);
+                    if (gate_f32)
+                        store_row<float, VEC>(p, 0, static_cast<float *>(a.dgate) + at, n);
+                    else
+                        store_row<F, VEC>(p, 0, static_cast<F *>(a.dgate) + at, n);
                 }
-                const bool layer = a.after == LUTB_NORM_LAYER, here_too = VEC ? p.valid != 0 : true;
-                const float2 c = row_sums<TEAM>(p, slots, here_too ? s1.x + s1.y : 0.0f, layer && here_too ? total(v) : 0.0f, layer, [&]() {
+            }
+            {
+                float2 gate[4];
+                gate_of(gate);
+#pragma unroll
+                for (int k = 0; k < 4; k++) d[k] = mul2(d[k], gate[k]);
+            }
+            if (BRANCH == 2) {
+                float2 s1 = make_float2(0.0f, 0.0f), w[4];
+                param(0, w);
+                if (on)
 #pragma unroll
                     for (int k = 0; k < 4; k++) {
-                        if (on) {
-                            sums[0][k] = fma2(d[k], t[k], sums[0][k]);
-                            sums[1][k] = add2(sums[1][k], d[k]);
-                        }
+                        sums[0][k] = fma2(d[k], t[k], sums[0][k]);
+                        sums[1][k] = add2(sums[1][k], d[k]);
                     }
-                });
+#pragma unroll
+                for (int k = 0; k < 4; k++) {
+                    d[k] = mul2(d[k], w[k]);
+                    if (!VEC) {
+                        d[k].x = row_valid<VEC>(p, 0, 2 * k) ? d[k].x : 0.0f;
+                        d[k].y = row_valid<VEC>(p, 0, 2 * k + 1) ? d[k].y : 0.0f;
+                    }
+                    s1 = fma2(d[k], t[k], s1);
+                }
+                const bool layer = a.after == LUTB_NORM_LAYER, some = !VEC || p.valid;
+                const float2 c = row_sums<TEAM>(p, slots, some ? s1.x + s1.y : 0.0f, layer && some ? total(d) : 0.0f, layer, []() {});
                 const float c1 = -c.x * p.inverse, c2 = layer ? -c.y * p.inverse : 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; k++) d[k] = mul2(both(st.y), fma2(t[k], both(c1), add2(v[k], both(c2))));
+                for (int k = 0; k < 4; k++) d[k] = mul2(both(st.y), fma2(t[k], both(c1), add2(d[k], both(c2))));
             }
             if (a.df && on) {
                 if (a.drop.on) drop8(d, kept, a.drop.scale);
                 store_row<F, VEC>(p, 0, static_cast<F *>(a.df) + at, d);
             }
         }
+        ring.taken();
         here.next(a, p.teams, stride);
         if (gate_summed && here.chunk != chunk) {   // (the same for the whole block)
             const int64_t out = (a.gate_direct ? chunk / a.per_group : chunk) * a.width;
-            hand_out(sums[4], [&](int64_t c, float v) {
+            hand_out(sums[4], [&](int c, float v) {
                 v *= a.branch;
                 if (!a.gate_direct)
                     a.gate_sums[out + c] = v;
-                else if (sizeof(F) == 4 || a.gate_f32)
+                else if (a.gate_f32)
                     static_cast<float *>(a.dgate)[out + c] = v;
                 else
                     static_cast<F *>(a.dgate)[out + c] = from_f32<F>(v);
@@ -942,23 +983,25 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     for (int s = 0; s < 4; s++) {
         if ((s < 2 ? BRANCH == 2 : NEXT) && a.sums[s]) {
             float *to = a.sums[s] + own * a.width;
-            hand_out(sums[s], [&](int64_t c, float v) { to[c] = v; });
+            hand_out(sums[s], [&](int c, float v) { to[c] = v; });
         }
     }
     if (over_cluster<TEAM>(p)) cluster_meet();   // (no block is gone while another may store into it)
 }
 
 // ------------------------------------------------------------------------------------------------ launches
+int resident_clusters(const void *kernel, const RowShape &s, size_t smem);
 int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs &a, const RowShape &s, int clusters, size_t smem, cudaStream_t stream);
 
-// Shared memory of a block besides the kernel's own arrays.
+// Shared memory of a block besides the kernel's own arrays, for any join of these types.
 template <class X, class F>
 size_t join_rows_smem(bool backward, bool vec, const RowShape &s, bool gate_each) {
-    const int gate = gate_each ? 2 : 0;
-    size_t parts = backward ? 2 * kBackwardParams : 0;
-    if (vec) parts += (size_t)s.stages * (backward ? kBackwardParts<X, F> + gate : s.groups * (kForwardParts<X, F> + gate));
-    return parts * 16 * s.threads;
+    const size_t x = ring_bytes(vec, s, sizeof(X)), f = ring_bytes(vec, s, sizeof(F)), gate = gate_each ? ring_bytes(vec, s, 4) : 0;
+    return (backward ? 2 * kBackwardParams * 16 * s.threads : 0) + s.stages * ((backward ? 2 : 1) * (x + f) + gate);
 }
+// Clusters of a backward kernel that are resident at a time, as the driver counts them; 0 where it cannot be asked.
+template <class X, class F>
+int join_rows_clusters(const RowShape &s, size_t smem);
 template <class X, class F, int BRANCH, bool NEXT>
 const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
 #define LUTB_FORWARD(VEC, G, TEAM) reinterpret_cast<const void *>(&join_rows_forward_kernel<X, F, BRANCH, NEXT, VEC, G, TEAM>)
@@ -997,6 +1040,10 @@ int join_rows_wait_errors(int *count);
     template <>                                                                                                                     \
     int join_rows<X, F>(bool backward, bool vec, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream) {        \
         return launch_join_rows<X, F>(backward, vec, a, s, clusters, stream);                                                      \
+    }                                                                                                                               \
+    template <>                                                                                                                     \
+    int join_rows_clusters<X, F>(const RowShape &s, size_t smem) {                                                                  \
+        return resident_clusters(join_rows_kernel<X, F, 2, true>(true, true, s), s, smem);                                          \
     }                                                                                                                               \
     template <>                                                                                                                     \
     int join_rows_wait_errors<X, F>(int *count) {                                                                                   \
