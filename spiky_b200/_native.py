@@ -228,6 +228,31 @@ def layer_calls():
     return _layer_calls
 
 
+_residual_calls = None
+RESIDUAL_CALLS_PATH = os.path.join(_HERE, "lib", "_residual_calls.so")
+
+
+def residual_calls():
+    """The extension module of the native host side of the residual-stream operators (host/residual_calls.cpp), set up; raises
+    RuntimeError or ImportError when it is missing or was built against another torch."""
+    global _residual_calls
+    if _residual_calls is None:
+        if not os.path.exists(RESIDUAL_CALLS_PATH):
+            raise RuntimeError(f"{RESIDUAL_CALLS_PATH} is missing: build it with `python -m spiky_b200.build`")
+        import importlib.util
+
+        import torch
+        spec = importlib.util.spec_from_file_location("_residual_calls", RESIDUAL_CALLS_PATH)
+        module = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(module)
+        if module.torch_version != torch.__version__.split("+")[0]:   # (it uses torch's own data structures)
+            raise RuntimeError(f"{RESIDUAL_CALLS_PATH} was built against torch {module.torch_version}, this is {torch.__version__}")
+        handle = lib()
+        module.setup({name: ctypes.cast(getattr(handle, name), _vp).value for name in SIGNATURES if name.startswith(("lutb_dropout", "lutb_join"))}, check)
+        _residual_calls = module
+    return _residual_calls
+
+
 class LutbError(RuntimeError):
     pass
 

@@ -1,5 +1,5 @@
-"""Builds libspiky_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and _layer_calls.so (the native host side of
-layer calls, host/layer_calls.cpp, against the installed torch) with the host compiler.
+"""Builds libspiky_b200.so (the C-ABI CUDA library) in-tree with nvcc for sm_100a, and _layer_calls.so and _residual_calls.so (the native
+host sides of layer calls and of the residual-stream operators, host/, against the installed torch) with the host compiler.
 
     python -m spiky_b200.build [--force] [--verbose]
 
@@ -65,19 +65,20 @@ def _extra_flags(src):
     return flags
 
 
-HOST_SRC = os.path.join(HERE, "host", "layer_calls.cpp")
-HOST_LIB = os.path.join(LIBDIR, "_layer_calls.so")
+HOST_DIR = os.path.join(HERE, "host")
+HOST_MODULES = ("_layer_calls", "_residual_calls")
 
 
-def _build_host(force):
-    """The extension module; rebuilt when its source, the C ABI's header or torch itself is newer."""
+def _build_host(name, force):
+    """An extension module (host/<name without its underscore>.cpp); rebuilt when its source, a header or torch itself is newer."""
     import sysconfig
 
     import torch
     root = os.path.dirname(torch.__file__)
-    header = os.path.join(HERE, "..", "include", "spiky_b200.h")
-    if not force and os.path.exists(HOST_LIB) and os.path.getmtime(HOST_LIB) >= _newest(
-            [HOST_SRC, header, os.path.join(root, "version.py")]):
+    source, module = os.path.join(HOST_DIR, name[1:] + ".cpp"), os.path.join(LIBDIR, name + ".so")
+    headers = [os.path.join(HOST_DIR, "call_checks.h"), os.path.join(HERE, "..", "include", "spiky_b200.h")]
+    if not force and os.path.exists(module) and os.path.getmtime(module) >= _newest(
+            [source, os.path.join(root, "version.py")] + headers):
         return
     gxx = "/usr/bin/g++" if os.path.exists("/usr/bin/g++") else "g++"
     cuda = os.path.join(os.path.dirname(os.path.dirname(_nvcc())), "include")
@@ -85,10 +86,10 @@ def _build_host(force):
     for d in (os.path.join(root, "include"), os.path.join(root, "include", "torch", "csrc", "api", "include"), cuda,
               sysconfig.get_paths()["include"]):
         cmd += ["-isystem", d]
-    cmd += [HOST_SRC, "-o", HOST_LIB, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
+    cmd += [source, "-o", module, "-L" + os.path.join(root, "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_python"]
     p = subprocess.run(cmd, capture_output=True, text=True)
     if p.returncode != 0:
-        raise RuntimeError("host compiler failed for %s:\n%s\n%s" % (HOST_SRC, p.stdout, p.stderr))
+        raise RuntimeError("host compiler failed for %s:\n%s\n%s" % (source, p.stdout, p.stderr))
 
 
 def _newest(paths):
@@ -103,7 +104,8 @@ def build(force=False, verbose=False):
     objdir = os.path.join(LIBDIR, "obj")
     os.makedirs(objdir, exist_ok=True)
     if not force and os.path.exists(LIB) and os.path.getmtime(LIB) >= _newest(sources + headers):
-        _build_host(force)
+        for name in HOST_MODULES:
+            _build_host(name, force)
         return LIB
     nvcc = _nvcc()
     hdr_time = _newest(headers) if headers else 0.0
@@ -118,10 +120,11 @@ def build(force=False, verbose=False):
             raise RuntimeError("nvcc failed for %s:\n%s\n%s" % (src, p.stdout, p.stderr))
         return obj, "== %s\n%s%s" % (os.path.basename(src), p.stdout, p.stderr)
 
-    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources)) + 1) as ex:
-        host = ex.submit(_build_host, force)
+    with concurrent.futures.ThreadPoolExecutor(max_workers=min(8, len(sources)) + len(HOST_MODULES)) as ex:
+        hosts = [ex.submit(_build_host, name, force) for name in HOST_MODULES]
         results = list(ex.map(compile_one, sources))
-        host.result()
+        for host in hosts:
+            host.result()
     objs = [r[0] for r in results]
     log = "".join(r[1] for r in results)
     if log:

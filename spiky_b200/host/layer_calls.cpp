@@ -14,17 +14,14 @@
 #include <torch/extension.h>
 #include <torch/version.h>
 
-#include <ATen/FuncTorchTLS.h>
-#include <ATen/PythonTorchFunctionTLS.h>
-#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_cpp_function.h>
 #include <torch/csrc/autograd/saved_variable.h>
-#include <torch/csrc/jit/frontend/tracer.h>
 
 #include "../../include/spiky_b200.h"
+#include "call_checks.h"
 
 namespace {
 
@@ -67,16 +64,6 @@ std::vector<std::pair<PyObject *, PyObject *>> layer_methods, manager_methods;  
 std::vector<PyObject *> layer_hooks;
 std::vector<PyObject *> layer_parts;   // names of what a layer's backward pass reads
 
-struct Ref {   // owned reference
-    PyObject *p = nullptr;
-    explicit Ref(PyObject *q = nullptr) : p(q) {}
-    Ref(const Ref &) = delete;
-    Ref &operator=(const Ref &) = delete;
-    ~Ref() { Py_XDECREF(p); }
-    PyObject *get() const { return p; }
-    explicit operator bool() const { return p != nullptr; }
-};
-
 PyObject *instance_dict(PyObject *o) {   // borrowed
     PyObject **d = _PyObject_GetDictPtr(o);
     return d ? *d : nullptr;
@@ -97,11 +84,6 @@ bool methods_untouched(PyObject *o, PyObject *dict, const std::vector<std::pair<
 bool exact_tensor(PyObject *o) {
     return o != nullptr && ((PyObject *)Py_TYPE(o) == tensor_class || (PyObject *)Py_TYPE(o) == parameter_class);
 }
-[[noreturn]] void raise_current() {
-    python_error e;
-    e.persist();
-    throw std::move(e);
-}
 void check(int status) {
     if (status == 0) return;
     Ref r(PyObject_CallFunction(check_status, "i", status));   // raises what the Python route raises
@@ -109,18 +91,6 @@ void check(int status) {
 }
 
 // ------------------------------------------------------------------------------------------------ what a call needs
-bool plain_cuda(const Tensor &t, at::ScalarType type, c10::DeviceIndex device) {
-    if (!t.defined() || t.layout() != at::kStrided || t.scalar_type() != type || !t.is_cuda() || t.device().index() != device) return false;
-    const auto keys = t.unsafeGetTensorImpl()->key_set();
-    return !keys.has_any(c10::python_ks) && !keys.has(c10::DispatchKey::FuncTorchGradWrapper) && !keys.has(c10::DispatchKey::FuncTorchBatched) &&
-           !keys.has(c10::DispatchKey::Functionalize) && !keys.has(c10::DispatchKey::Batched) && !t.is_neg() && !t.is_conj() && !t._is_zerotensor();
-}
-bool ordinary_context() {
-    return !torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::any_modes_set() && !at::impl::torch_function_mode_enabled() &&
-           (at::functorch::functorchTLSAccessor() == nullptr ||   // (it stays after the first transform; a key is there while one is active)
-            !c10::impl::tls_is_dispatch_key_included(c10::DispatchKey::FuncTorchDynamicLayerFrontMode));
-}
-
 enum Mode { NONSEQ, CONCAT, PRODUCT };
 
 struct Call {

@@ -10,19 +10,44 @@ No counterpart in the reference, whose transformer composes torch's dropout, ``B
   block, and in the same pass ``y = N'(h)``, the norm before the next block.
 
 float32, bfloat16 and float16; a float32 stream may carry a 16-bit branch.  Sums, norms and their statistics are float32, every
-output is rounded once.  ``CounterDropout``, ``RowNorm`` and ``ResidualJoin`` are the modules; ``LUTTransformer`` uses them.
+output is rounded once.  ``CounterDropout``, ``RowNorm`` and ``ResidualJoin`` are the modules; ``LUTTransformer`` uses them.  Ordinary calls run through
+the native host side (host/residual_calls.cpp); the functions here define them all and take the rest.
 
 Argument mistakes raise ``ValueError``, mistakes of type or device ``RuntimeError``; there is no CPU path.  Tensors that are not
 contiguous are copied.  Work goes to torch's current stream of the tensors' device.
 """
 import ctypes
 import math
+import warnings
 
 import torch
 import torch.nn as nn
 
 from . import _native
 from ._native import JoinCfg
+
+_calls = None   # the native host side (host/residual_calls.cpp), once a call has asked for it
+
+
+class _PythonRoute:
+    """What stands in for the native host side where there is none: leaves every call to the functions below."""
+
+    @staticmethod
+    def join(*args):
+        return None
+
+    dropout = take = join
+
+
+def _native_calls():
+    global _calls
+    try:
+        _calls = _native.residual_calls()
+    except (ImportError, RuntimeError) as e:
+        warnings.warn(f"residual operators take the Python route, at about twice the host time: {e}", RuntimeWarning, stacklevel=4)
+        _calls = _PythonRoute
+    return _calls
+
 
 _TYPES = {torch.float32: _native.F32, torch.bfloat16: _native.BF16, torch.float16: _native.F16}
 _NORMS = {None: _native.NORM_NONE, "rms": _native.NORM_RMS, "layer": _native.NORM_LAYER}
@@ -71,6 +96,9 @@ def dropout_state(seed, device, offset=0):
 
 def take_dropout_state(state, count):
     """A copy of ``state`` for ``count`` dropouts (their sites 0 .. count - 1); the offset in ``state`` moves on by ``count``."""
+    used = (_calls or _native_calls()).take(state, count)
+    if used is not None:
+        return used
     _check_dropout(1.0, state, 0, state.device if isinstance(state, torch.Tensor) else None)
     if not state.is_cuda:
         raise RuntimeError("state must be on CUDA: spiky_b200 has no CPU path")
@@ -112,6 +140,9 @@ def counter_dropout(x, p, state, site=0):
     dropped is 0 even where ``x`` is infinite or NaN.  The backward pass reads ``state`` again: leave it as it was until then
     (``take_dropout_state`` hands out copies).
     """
+    y = (_calls or _native_calls()).dropout(x, p, state, site)
+    if y is not None:
+        return y
     p, site = float(p), int(site)
     _check_data(x, "x")
     _check_dropout(p, state, site, x.device)
@@ -247,6 +278,9 @@ def _join(x, branch, branch_type, after, aw, ab, gate, skip_scale, branch_scale,
 def row_norm(x, weight=None, bias=None, kind="rms", eps=1e-6, dtype=None):
     """``N(x) * weight + bias`` over the last dimension: ``kind`` 'rms' is ``x / sqrt(mean(x^2) + eps)``, 'layer' is
     ``(x - mean) / sqrt(mean((x - mean)^2) + eps)``.  ``dtype``: the result's, that of ``x`` or a 16-bit type of a float32 ``x``."""
+    got = (_calls or _native_calls()).join(x, None, dtype, None, None, None, None, 1.0, 1.0, 0.0, None, 0, kind, weight, bias, eps)
+    if got is not None:
+        return got[1]
     if kind is None:
         raise ValueError("kind is 'rms' or 'layer'")
     _check_data(x, "x")
@@ -266,6 +300,10 @@ def residual_join(x, branch, *, branch_norm=None, branch_weight=None, branch_bia
     """
     if branch is None:
         raise RuntimeError("branch must be a tensor")
+    got = (_calls or _native_calls()).join(x, branch, None, branch_norm, branch_weight, branch_bias, gate, skip_scale, branch_scale, dropout, state,
+                                           site, next_norm, next_weight, next_bias, eps)
+    if got is not None:
+        return got[0] if next_norm is None else got
     _check_data(branch, "branch")
     h, y = _join(x, branch, branch.dtype, branch_norm, branch_weight, branch_bias, gate, skip_scale, branch_scale, dropout, state, site,
                  next_norm, next_weight, next_bias, eps)
