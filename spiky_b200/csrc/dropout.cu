@@ -32,15 +32,15 @@ __global__ void __launch_bounds__(256) dropout_kernel(int64_t first, int64_t n, 
 #pragma unroll
                 for (int q = 0; q < kParts<T>; q++)
                     if (8 * (b + 256 * k) < n) in[k][q] = reinterpret_cast<const uint4 *>(x + 8 * (b + 256 * k))[q];
-            uint32_t kept[kSide];
+            DropDigits digits[kSide];
 #pragma unroll
-            for (int k = 0; k < kSide; k++) kept[k] = keep_bits((uint64_t)(b + 256 * k), key, rule);
+            for (int k = 0; k < kSide; k++) digits[k] = drop_digits((uint64_t)(b + 256 * k), key, rule);
 #pragma unroll
             for (int k = 0; k < kSide; k++) {
                 if (8 * (b + 256 * k) >= n) break;
                 float2 v[4];
                 unpack8<T>(in[k], v);
-                drop8(v, kept[k], rule.scale);
+                drop8(v, digits[k], rule.scale);
                 store8(y + 8 * (b + 256 * k), v);
             }
         }

@@ -56,27 +56,36 @@ __device__ __forceinline__ uint4 philox_block(uint64_t block, uint32_t second, c
     return make_uint4(c0, c1, c2, c3);
 }
 
-// Which of the elements 8 * block .. 8 * block + 7 stay, as bits.  One block of 128 bits decides eight elements but for one in 8192 of these
-// groups, where a digit ties and a second block is formed: 32-bit probabilities at the cost of 16-bit ones.
-__device__ __forceinline__ uint32_t keep_bits(uint64_t block, const DropKey &key, const DropRule &rule) {
+// The digits of the elements 8 * block .. 8 * block + 7: element 2k stays when word k << 16 is above `above`, element 2k + 1 when word k is.  One block of
+// 128 bits decides eight elements but for one in 8192 of these groups, where a digit ties and a second block is formed: 32-bit
+// probabilities at the cost of 16-bit ones.
+struct DropDigits {
+    uint32_t w[4], above;
+};
+__device__ __forceinline__ DropDigits drop_digits(uint64_t block, const DropKey &key, const DropRule &rule) {
     const uint4 v = philox_block(block, 0, key);
-    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t kept = 0, tied = 0;
-#pragma unroll
-    for (int k = 0; k < 4; k++) {
-        kept |= ((w[k] << 16) > rule.above ? 1u : 0u) << (2 * k) | (w[k] > rule.above ? 2u : 0u) << (2 * k);
-        const uint32_t d = w[k] ^ rule.tie;   // a half of zero where the digits agree
-        tied |= (d - 0x00010001u) & ~d & 0x80008000u;
-    }
-    if (tied && rule.ties) {
+    DropDigits d{{v.x, v.y, v.z, v.w}, rule.above};
+    // the smaller halves of the words' differences from T's upper digit: 0 where a digit ties
+    const uint32_t near = __vimin3_u16x2(d.w[0] ^ rule.tie, d.w[1] ^ rule.tie, __vminu2(d.w[2] ^ rule.tie, d.w[3] ^ rule.tie));
+    if ((near < 0x10000u || (near & 0xffffu) == 0u) && rule.ties) {
         const uint4 s = philox_block(block, 1, key);
-        const uint32_t q[4] = {s.x, s.y, s.z, s.w};
+        const uint32_t q[4] = {s.x, s.y, s.z, s.w}, tie = rule.tie & 0xffffu;
 #pragma unroll
         for (int k = 0; k < 4; k++) {
-            if ((w[k] & 0xffffu) == (rule.tie & 0xffffu) && (q[k] & 0xffffu) >= rule.low) kept |= 1u << (2 * k);
-            if ((w[k] >> 16) == (rule.tie & 0xffffu) && (q[k] >> 16) >= rule.low) kept |= 2u << (2 * k);
+            const uint32_t lo = d.w[k] & 0xffffu, hi = d.w[k] >> 16;
+            const bool keep_lo = lo == tie ? (q[k] & 0xffffu) >= rule.low : (lo << 16) > rule.above;
+            const bool keep_hi = hi == tie ? (q[k] >> 16) >= rule.low : d.w[k] > rule.above;
+            d.w[k] = (keep_lo ? 0xffffu : 0u) | (keep_hi ? 0xffff0000u : 0u);
         }
+        d.above = 0x7fffffffu;
     }
+    return d;
+}
+__device__ __forceinline__ uint32_t keep_bits(uint64_t block, const DropKey &key, const DropRule &rule) {
+    const DropDigits d = drop_digits(block, key, rule);
+    uint32_t kept = 0;
+#pragma unroll
+    for (int k = 0; k < 4; k++) kept |= ((d.w[k] << 16) > d.above ? 1u : 0u) << (2 * k) | (d.w[k] > d.above ? 2u : 0u) << (2 * k);
     return kept;
 }
 

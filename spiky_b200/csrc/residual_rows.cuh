@@ -102,8 +102,9 @@ __device__ __forceinline__ void zero8(float2 *v) {
 __device__ __forceinline__ void drop8(float2 *v, uint32_t kept, float scale) {
 #pragma unroll
     for (int k = 0; k < 4; k++) {
-        v[k].x = (kept >> (2 * k) & 1) ? v[k].x * scale : 0.0f;
-        v[k].y = (kept >> (2 * k) & 2) ? v[k].y * scale : 0.0f;
+        v[k] = mul2(v[k], both(scale));
+        v[k].x = (kept >> (2 * k) & 1) ? v[k].x : 0.0f;
+        v[k].y = (kept >> (2 * k) & 2) ? v[k].y : 0.0f;
     }
 }
 
@@ -147,6 +148,19 @@ __device__ __forceinline__ void store8(T *p, const float2 *v) {
     }
 }
 __device__ __forceinline__ void copy16(uint32_t to, const void *from) { asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory"); }
+
+__device__ __forceinline__ void drop8(float2 *v, const DropDigits &d, float scale) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) {
+        v[k] = mul2(v[k], both(scale));
+        v[k].x = (d.w[k] << 16) > d.above ? v[k].x : 0.0f;
+        v[k].y = d.w[k] > d.above ? v[k].y : 0.0f;
+    }
+}
+// (16 bytes, or zeros where there are none to fetch)
+__device__ __forceinline__ void copy16_or_zeros(uint32_t to, const void *from, bool some) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(some ? 16 : 0) : "memory");
+}
 
 // ------------------------------------------------------------------------------------------------ a thread's place
 // Values that warps exchange: of two numbers each, two sets in turn (a set is written again only after the barrier of the next one, which a
@@ -341,13 +355,17 @@ __device__ __forceinline__ float2 row_sums(RowPlace &p, Slots &slots, float a, f
     p.turn++;
     return s;
 }
-// Mean (0 for an RMS norm) and reciprocal deviation of the row's values; values of no element are 0.
+// Mean (0 for an RMS norm) and reciprocal deviation of the row's values.  Values of no element do not count (in rows that are not VEC
+// they are 0).
 template <bool VEC, int G, int TEAM, class Slots>
 __device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const float2 (*v)[4], bool layer, float eps) {
     auto sum = [&]() {
         float s = 0.0f;
 #pragma unroll
-        for (int g = 0; g < G; g++) s += total(v[g]);
+        for (int g = 0; g < G; g++) {
+            const float one = total(v[g]);
+            s += !VEC || row_valid<VEC>(p, g, 0) ? one : 0.0f;
+        }
         return s;
     };
     auto squares = [&](float mean) {
@@ -364,7 +382,10 @@ __device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const flo
                 }
                 q = fma2(d, d, q);
             }
-            if (VEC && !row_valid<VEC>(p, g, 0)) q = make_float2(0.0f, 0.0f);
+            if (VEC) {
+                q.x = row_valid<VEC>(p, g, 0) ? q.x : 0.0f;
+                q.y = row_valid<VEC>(p, g, 0) ? q.y : 0.0f;
+            }
             s = add2(s, q);
         }
         return s.x + s.y;
@@ -402,17 +423,11 @@ __device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const flo
     return make_float2(mean, rsqrtf(s * p.inverse + eps));
 }
 
-// Eight of a parameter's values: `none` where there is no such parameter, 0 for columns beyond the row.
+// Eight of a parameter's values.  VEC: a group beyond the row reads another one's; else values of no element are 0.
 template <class F, bool VEC>
-__device__ __forceinline__ void param8(const RowPlace &p, int g, const void *from, bool f32, int64_t at, float none, float2 *v) {
+__device__ __forceinline__ void param8(const RowPlace &p, int g, const void *from, bool f32, int64_t at, float2 *v) {
     if constexpr (VEC) {
-        if (from == nullptr || !row_valid<VEC>(p, g, 0)) {
-            const float e = row_valid<VEC>(p, g, 0) ? none : 0.0f;
-#pragma unroll
-            for (int k = 0; k < 4; k++) v[k] = both(e);
-            return;
-        }
-        const int64_t c = at + row_column<VEC>(p, g, 0);
+        const int64_t c = at + min(row_column<VEC>(p, g, 0), p.limit - 8);
         if (sizeof(F) == 4 || f32) {
             const uint4 *q = reinterpret_cast<const uint4 *>(static_cast<const float *>(from) + c);
             const uint4 part[2] = {__ldg(q), __ldg(q + 1)};
@@ -424,10 +439,38 @@ __device__ __forceinline__ void param8(const RowPlace &p, int g, const void *fro
     } else {
         float e[8];
 #pragma unroll
-        for (int k = 0; k < 8; k++) e[k] = row_valid<VEC>(p, g, k) ? join_param<F>(from, f32, at + row_column<VEC>(p, g, k), none) : 0.0f;
+        for (int k = 0; k < 8; k++) e[k] = row_valid<VEC>(p, g, k) ? join_param<F>(from, f32, at + row_column<VEC>(p, g, k), 0.0f) : 0.0f;
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
     }
+}
+// v = v w + b, for what there is of them (one test for all groups).
+template <class F, bool VEC, int G>
+__device__ __forceinline__ void affine(const RowPlace &p, const void *weight, const void *bias, bool f32, float2 (*v)[4]) {
+    auto each = [&](bool of_f32) {
+        if (weight != nullptr) {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                float2 w[4];
+                param8<F, VEC>(p, g, weight, of_f32, 0, w);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = mul2(v[g][k], w[k]);
+            }
+        }
+        if (bias != nullptr) {
+#pragma unroll
+            for (int g = 0; g < G; g++) {
+                float2 b[4];
+                param8<F, VEC>(p, g, bias, of_f32, 0, b);
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = add2(v[g][k], b[k]);
+            }
+        }
+    };
+    if (sizeof(F) == 4 || f32)
+        each(true);
+    else
+        each(false);
 }
 
 // The rows of a block in turn: chunk by chunk, `teams` rows at a time.
@@ -464,32 +507,49 @@ __host__ __device__ inline int ring_bytes(bool vec, const RowShape &s, int size)
     return vec ? s.groups * kRowElems * size * s.threads : s.teams * ring_row_bytes(s.slice, size);
 }
 
-// With one stage a row is fetched when its turn comes, else one or two rows ahead.  The current row can be read to the end of its turn.
+// The current row and those that are fetched.  With one stage a row is fetched when its turn comes, else one or two rows ahead.  The current row can be
+// read to the end of its turn.
+//
+// VEC: a warp has a place of its own, [stage][array][group][piece], in which arrays and groups begin at constants (AT, in parts of 512 bytes).  A
+// warp's (or a smaller team's) 16-byte pieces of a group go side by side over its threads; those of 4-byte elements are two a
+// thread, swapped in every other four pairs, so that the threads' reads of their two pieces meet no bank twice.
 template <bool VEC, int G, int TEAM>
 struct RowRing {
-    unsigned char *at;
-    int stage_bytes, stages, fill, take;
+    unsigned char *at;          // VEC: this warp's place, else the block's
+    int stage_bytes, stages, fill, take;   // VEC: of this warp; fill and take count bytes
+    int u, wide;                // VEC: thread among those that share pieces, how many they are
+    int mine, swapped;          // VEC: this thread's own pieces (in bytes, for one part), and whether its two are swapped
 
-    // What this thread fetches of a row of one array, whose place in a stage begins at `part`.
-    template <class T>
-    __device__ __forceinline__ void fetch(const RowPlace &p, const RowShape &s, int part, const T *from, int64_t row, const JoinArgs &a) const {
-        const uint32_t to = smem_u32(at) + fill * stage_bytes + part;
+    __device__ __forceinline__ RowRing(unsigned char *memory, const RowPlace &p, int bytes_of_block, int n) : at(memory), stages(n), fill(0), take(0) {
+        stage_bytes = bytes_of_block;
+        if (VEC) {
+            const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+            stage_bytes = bytes_of_block / (int)(blockDim.x >> 5);
+            at = memory + warp * n * stage_bytes;
+            wide = min(p.team, 32);
+            u = lane & (wide - 1);
+            mine = (lane - u) * 16;
+            swapped = u >> 2 & 1;
+        }
+    }
+    // What this thread fetches of a row of one array.
+    template <class T, int AT>
+    __device__ __forceinline__ void fetch(const RowPlace &p, const RowShape &s, int part, const T *from, int64_t row, bool some, const JoinArgs &a) const {
         constexpr int kEach = 16 / sizeof(T);
         if constexpr (VEC) {
-            // 16-byte pieces of a warp's (or a smaller team's) part of the row, one after another over its threads; those of eight 4-byte
-            // elements are two, swapped in every other four pairs, so that the threads' reads of their two pieces meet no bank twice
-            const int wide = min(p.team, 32), u = p.t & (wide - 1);
+            const T *const begin = from + (some ? row * a.width : 0);
+            const uint32_t to = smem_u32(at) + fill + AT * 512 + mine * kParts<T>;
 #pragma unroll
-            for (int g = 0; g < G; g++) {
-                const int first = p.first + (g * p.team + p.t - u) * 8;
-                const uint32_t place = to + (g * (int)blockDim.x + threadIdx.x - u) * (kParts<T> * 16);
+            for (int g = 0; g < G; g++)
 #pragma unroll
                 for (int q = 0; q < kParts<T>; q++) {
-                    const int c = q * wide + u, column = first + c * kEach;
-                    if (column < p.limit) copy16(place + (kParts<T> == 2 ? c ^ (c >> 3 & 1) : c) * 16, from + row * a.width + column);
+                    const int c = q * wide + u, column = p.first + (g * p.team + p.t - u) * 8 + c * kEach;
+                    const bool there = some && column < p.limit;
+                    copy16_or_zeros(to + g * kParts<T> * 512 + (kParts<T> == 2 ? c ^ (c >> 3 & 1) : c) * 16, begin + (there ? column : 0), there);
                 }
-            }
         } else {
+            if (!some) return;
+            const uint32_t to = smem_u32(at) + fill + part;
             const int64_t begin = row * a.width + p.first, total = a.rows * a.width;
             const unsigned char *const bytes = reinterpret_cast<const unsigned char *>(from);
             const int ahead = (int)(reinterpret_cast<uintptr_t>(from + begin) & 15);   // of the row in its first piece
@@ -500,7 +560,7 @@ struct RowRing {
                 if (offset >= 0 && offset + 16 <= total * (int64_t)sizeof(T)) {
                     copy16(place + c * 16, bytes + offset);
                 } else {   // a piece that the array does not fill: its elements one by one
-                    T *const own = reinterpret_cast<T *>(at + fill * stage_bytes + part + p.which * ring_row_bytes(s.slice, sizeof(T)) + c * 16);
+                    T *const own = reinterpret_cast<T *>(at + fill + part + p.which * ring_row_bytes(s.slice, sizeof(T)) + c * 16);
                     const int64_t element = (begin * (int64_t)sizeof(T) - ahead) / (int64_t)sizeof(T) + c * kEach;
 #pragma unroll
                     for (int e = 0; e < kEach; e++)
@@ -511,7 +571,7 @@ struct RowRing {
     }
     __device__ __forceinline__ void filled() {
         asm volatile("cp.async.commit_group;" ::: "memory");
-        fill = fill + 1 == stages ? 0 : fill + 1;
+        fill = fill + stage_bytes == stages * stage_bytes ? 0 : fill + stage_bytes;
     }
     // The current row's elements are there, for the team; what was read of the row before may be overwritten.
     __device__ __forceinline__ void ready(const RowPlace &p) const {
@@ -524,23 +584,22 @@ struct RowRing {
         else
             team_barrier<TEAM>(p);
     }
-    __device__ __forceinline__ void taken() { take = take + 1 == stages ? 0 : take + 1; }
+    __device__ __forceinline__ void taken() { take = take + stage_bytes == stages * stage_bytes ? 0 : take + stage_bytes; }
     // Eight elements; 0 where there are none.
-    template <class T>
+    template <class T, int AT>
     __device__ __forceinline__ void get(const RowPlace &p, const RowShape &s, int g, int part, const T *from, int64_t begin, bool on, float2 *v) const {
-        const unsigned char *const stage = at + take * stage_bytes + part;
         if constexpr (VEC) {
-            if (!on || !row_valid<VEC>(p, g, 0)) {
-                zero8(v);
-                return;
-            }
-            const int wide = min(p.team, 32), u = p.t & (wide - 1), turned = kParts<T> == 2 ? u >> 2 & 1 : 0;
-            const uint4 *const own = reinterpret_cast<const uint4 *>(stage) + (g * (int)blockDim.x + threadIdx.x - u) * kParts<T> + kParts<T> * u;
+            const uint4 *const own = reinterpret_cast<const uint4 *>(at + take + mine * kParts<T> + u * (kParts<T> * 16)) + (AT + g * kParts<T>)*32;
             uint4 w[kParts<T>];
-#pragma unroll
-            for (int q = 0; q < kParts<T>; q++) w[q] = own[q ^ turned];
+            if constexpr (kParts<T> == 2) {
+                w[0] = own[swapped];
+                w[1] = own[1 - swapped];
+            } else {
+                w[0] = own[0];
+            }
             unpack8<T>(w, v);
         } else {
+            const unsigned char *const stage = at + take + part;
             const int ahead = (int)(reinterpret_cast<uintptr_t>(from + begin + p.first) & 15) / (int)sizeof(T);
             const T *const own = reinterpret_cast<const T *>(stage + p.which * ring_row_bytes(s.slice, sizeof(T))) + ahead - p.first;
             float e[8];
@@ -553,7 +612,7 @@ struct RowRing {
 };
 
 template <class T, bool VEC>
-__device__ __forceinline__ void store_row(const RowPlace &p, int g, T *row, const float2 *v) {
+__device__ __forceinline__ void store_row(const RowPlace &p, int g, T *row, const float2 *v) {   // (only where there is a row)
     if constexpr (VEC) {
         if (row_valid<VEC>(p, g, 0)) store8(row + row_column<VEC>(p, g, 0), v);
     } else {
@@ -563,25 +622,18 @@ __device__ __forceinline__ void store_row(const RowPlace &p, int g, T *row, cons
     }
 }
 
-// The masks of a thread's groups, eight bits each.  Rows that are not VEC: the team's generator blocks as bytes in shared memory, written before
-// the row's barrier and read after it, two sets in turn.
-template <bool VEC, int G>
-__device__ __forceinline__ uint32_t form_mask(const RowPlace &p, const JoinArgs &a, const DropKey &key, int64_t row, uint8_t *bytes, uint32_t set) {
+// The masks of a thread's groups.  Rows that are not VEC: the team's generator blocks as bytes in shared memory, written before the row's barrier and
+// read after it, two sets in turn.
+template <int G>
+__device__ __forceinline__ void form_masks(const RowPlace &p, const JoinArgs &a, const DropKey &key, int64_t row, uint8_t *bytes, uint32_t set) {
     const uint64_t block = (uint64_t)(row * a.width + p.first) >> 3;
-    if (VEC) {
-        uint32_t kept = 0;
-#pragma unroll
-        for (int g = 0; g < G; g++) kept |= keep_bits(block + g * p.team + p.t, key, a.drop) << (8 * g);
-        return kept;
-    }
     uint8_t *own = bytes + ((int)set * p.teams + p.which) * (G * p.team + 1);
 #pragma unroll
     for (int g = 0; g < G; g++) own[g * p.team + p.t] = (uint8_t)keep_bits(block + g * p.team + p.t, key, a.drop);
     if (p.t == 0) own[G * p.team] = (uint8_t)keep_bits(block + G * p.team, key, a.drop);
-    return 0;
 }
 template <int G>
-__device__ __forceinline__ uint32_t read_mask(const RowPlace &p, const JoinArgs &a, int64_t row, const uint8_t *bytes, uint32_t set) {
+__device__ __forceinline__ uint32_t read_masks(const RowPlace &p, const JoinArgs &a, int64_t row, const uint8_t *bytes, uint32_t set) {
     const uint8_t *own = bytes + ((int)set * p.teams + p.which) * (G * p.team + 1);
     const int off = (int)((row * a.width + p.first) & 7);
     uint32_t kept = 0;
@@ -610,7 +662,8 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
     const bool gate_each = BRANCH && a.gate_rows == 1, gate_f32 = sizeof(F) == 4 || a.gate_f32;
     const int part_f = ring_bytes(VEC, shape, sizeof(X)), part_gate = part_f + (BRANCH ? ring_bytes(VEC, shape, sizeof(F)) : 0);
-    RowRing<VEC, G, TEAM> ring{dynamic, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0), shape.stages, 0, 0};
+    constexpr int kF = G * kParts<X>, kGate = kF + (BRANCH ? G * kParts<F> : 0);
+    RowRing<VEC, G, TEAM> ring(dynamic, p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0), shape.stages);
     const X *const x_in = static_cast<const X *>(a.x);
     const F *const f_in = static_cast<const F *>(a.f);
     RowCursor load{(int)blockIdx.x, 0, 0}, here;
@@ -619,15 +672,14 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
     auto fetch = [&]() {
         if (load.more(a)) {
             const int64_t row = load.base + p.which;
-            if (row < load.end) {
-                ring.template fetch<X>(p, shape, 0, x_in, row, a);
-                if (BRANCH) ring.template fetch<F>(p, shape, part_f, f_in, row, a);
-                if (gate_each) {
-                    if (gate_f32)
-                        ring.template fetch<float>(p, shape, part_gate, static_cast<const float *>(a.gate), row, a);
-                    else
-                        ring.template fetch<F>(p, shape, part_gate, static_cast<const F *>(a.gate), row, a);
-                }
+            const bool some = row < load.end;
+            ring.template fetch<X, 0>(p, shape, 0, x_in, row, some, a);
+            if (BRANCH) ring.template fetch<F, kF>(p, shape, part_f, f_in, row, some, a);
+            if (gate_each) {
+                if (gate_f32)
+                    ring.template fetch<float, kGate>(p, shape, part_gate, static_cast<const float *>(a.gate), row, some, a);
+                else
+                    ring.template fetch<F, kGate>(p, shape, part_gate, static_cast<const F *>(a.gate), row, some, a);
             }
             load.next(a, p.teams, gridDim.x);
         }
@@ -646,23 +698,31 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
             gate_end = (gate_row + 1) * (int)a.gate_rows;
             gate_at = gate_row * a.width;
         }
-        uint32_t kept = 0xffffffffu;
-        if (BRANCH && a.drop.on) kept = form_mask<VEC, G>(p, a, key, row, masks, set);
+        const bool drop = BRANCH && a.drop.on;
+        if (!VEC && drop) form_masks<G>(p, a, key, row, masks, set);
         if (shape.stages == 1) {
             team_barrier<TEAM>(p);
             fetch();
         }
         ring.ready(p);
-        if (!VEC && BRANCH && a.drop.on) kept = read_mask<G>(p, a, row, masks, set);
+        uint32_t kept = 0;
+        if (!VEC && drop) kept = read_masks<G>(p, a, row, masks, set);
         set ^= 1;
         if (shape.stages > 1) fetch();
         float2 v[G][4];
         float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
         if (BRANCH) {
 #pragma unroll
-            for (int g = 0; g < G; g++) {
-                ring.template get<F>(p, shape, g, part_f, f_in, at, on, v[g]);
-                if (a.drop.on) drop8(v[g], kept >> (8 * g), a.drop.scale);
+            for (int g = 0; g < G; g++) ring.template get<F, kF>(p, shape, g, part_f, f_in, at, on, v[g]);
+            if (drop) {
+                const uint64_t block = (uint64_t)(at + p.first) >> 3;
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    if (VEC)
+                        drop8(v[g], drop_digits(block + g * p.team + p.t, key, a.drop), a.drop.scale);
+                    else
+                        drop8(v[g], kept >> (8 * g), a.drop.scale);
+                }
             }
         }
         if (BRANCH == 2) {
@@ -670,48 +730,60 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
             st.x = s.x;
             st.y = s.y;
 #pragma unroll
-            for (int g = 0; g < G; g++) {
-                float2 w[4], b[4];
-                param8<F, VEC>(p, g, a.aw, a.params_f32, 0, 1.0f, w);
-                param8<F, VEC>(p, g, a.ab, a.params_f32, 0, 0.0f, b);
+            for (int g = 0; g < G; g++)
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[g][k] = fma2(mul2(add2(v[g][k], both(-s.x)), both(s.y)), w[k], b[k]);
+                for (int k = 0; k < 4; k++) v[g][k] = mul2(add2(v[g][k], both(-s.x)), both(s.y));
+            affine<F, VEC, G>(p, a.aw, a.ab, a.params_f32, v);
+        }
+        if (BRANCH) {
+            auto gated = [&](auto get) {
+#pragma unroll
+                for (int g = 0; g < G; g++) {
+                    float2 gate[4];
+                    get(g, gate);
+#pragma unroll
+                    for (int k = 0; k < 4; k++) v[g][k] = mul2(v[g][k], gate[k]);
+                }
+            };
+            if (gate_each) {
+                if (gate_f32)
+                    gated([&](int g, float2 *e) { ring.template get<float, kGate>(p, shape, g, part_gate, static_cast<const float *>(a.gate), at, on, e); });
+                else
+                    gated([&](int g, float2 *e) { ring.template get<F, kGate>(p, shape, g, part_gate, static_cast<const F *>(a.gate), at, on, e); });
+            } else if (a.gate != nullptr) {
+                if (gate_f32)
+                    gated([&](int g, float2 *e) { param8<F, VEC>(p, g, a.gate, true, gate_at, e); });
+                else
+                    gated([&](int g, float2 *e) { param8<F, VEC>(p, g, a.gate, false, gate_at, e); });
             }
         }
 #pragma unroll
         for (int g = 0; g < G; g++) {
             float2 x[4];
-            ring.template get<X>(p, shape, g, 0, x_in, at, on, x);
-            if (BRANCH) {
-                float2 gate[4];
-                if (!gate_each)
-                    param8<F, VEC>(p, g, a.gate, gate_f32, gate_at, 1.0f, gate);
-                else if (gate_f32)
-                    ring.template get<float>(p, shape, g, part_gate, static_cast<const float *>(a.gate), at, on, gate);
-                else
-                    ring.template get<F>(p, shape, g, part_gate, static_cast<const F *>(a.gate), at, on, gate);
+            ring.template get<X, 0>(p, shape, g, 0, x_in, at, on, x);
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[g][k] = fma2(mul2(gate[k], both(a.branch)), v[g][k], mul2(x[k], both(a.skip)));
-                if (on) store_row<X, VEC>(p, g, static_cast<X *>(a.h) + at, v[g]);
-            } else {
+            for (int k = 0; k < 4; k++) v[g][k] = BRANCH ? fma2(v[g][k], both(a.branch), mul2(x[k], both(a.skip))) : x[k];
+            if (!VEC && BRANCH) {
 #pragma unroll
-                for (int k = 0; k < 4; k++) v[g][k] = x[k];
+                for (int k = 0; k < 4; k++) {
+                    v[g][k].x = row_valid<VEC>(p, g, 2 * k) ? v[g][k].x : 0.0f;
+                    v[g][k].y = row_valid<VEC>(p, g, 2 * k + 1) ? v[g][k].y : 0.0f;
+                }
             }
+            if (BRANCH && on) store_row<X, VEC>(p, g, static_cast<X *>(a.h) + at, v[g]);
         }
         if (NEXT) {
             const float2 s = row_stats<VEC, G, TEAM>(p, slots, v, a.before == LUTB_NORM_LAYER, a.eps);
             st.z = s.x;
             st.w = s.y;
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = mul2(add2(v[g][k], both(-s.x)), both(s.y));
+            affine<F, VEC, G>(p, a.bw, a.bb, a.params_f32, v);
             if (on)
 #pragma unroll
-                for (int g = 0; g < G; g++) {
-                    float2 w[4], b[4];
-                    param8<F, VEC>(p, g, a.bw, a.params_f32, 0, 1.0f, w);
-                    param8<F, VEC>(p, g, a.bb, a.params_f32, 0, 0.0f, b);
-#pragma unroll
-                    for (int k = 0; k < 4; k++) w[k] = fma2(mul2(add2(v[g][k], both(-s.x)), both(s.y)), w[k], b[k]);
-                    store_row<F, VEC>(p, g, static_cast<F *>(a.y) + at, w);
-                }
+                for (int g = 0; g < G; g++) store_row<F, VEC>(p, g, static_cast<F *>(a.y) + at, v[g]);
         }
         if (a.stats && on && p.t == 0) a.stats[row] = st;
         ring.taken();
@@ -733,18 +805,26 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     RowPlace p = row_place<VEC, 1, TEAM>(a, shape, slots);
     const int threads = blockDim.x, tid = threadIdx.x;
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
-    // parameters in slots of this thread's own: [parameter][half][thread]
-    float4 *const params = reinterpret_cast<float4 *>(dynamic) + tid;
+    // parameters in slots of this thread's own: [warp][parameter][half][lane]
+    float4 *const params = reinterpret_cast<float4 *>(dynamic) + (tid >> 5) * (2 * kBackwardParams * 32) + (tid & 31);
+    auto keep = [&](int which, const float2 *v) {
+        params[(2 * which) * 32] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
+        params[(2 * which + 1) * 32] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+    };
     auto keep_param = [&](int which, const void *from, bool f32, int64_t at, float none, float scale) {
         float2 v[4];
-        param8<F, VEC>(p, 0, from, f32, at, none, v);
+        if (from != nullptr) {
+            param8<F, VEC>(p, 0, from, f32, at, v);
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = both(none);
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = mul2(v[k], both(scale));
-        params[(2 * which) * threads] = make_float4(v[0].x, v[0].y, v[1].x, v[1].y);
-        params[(2 * which + 1) * threads] = make_float4(v[2].x, v[2].y, v[3].x, v[3].y);
+        keep(which, v);
     };
     auto param = [&](int which, float2 *v) {
-        const float4 lo = params[(2 * which) * threads], hi = params[(2 * which + 1) * threads];
+        const float4 lo = params[(2 * which) * 32], hi = params[(2 * which + 1) * 32];
         v[0] = make_float2(lo.x, lo.y);
         v[1] = make_float2(lo.z, lo.w);
         v[2] = make_float2(hi.x, hi.y);
@@ -763,8 +843,9 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     const F *const f_in = static_cast<const F *>(a.f), *const dy_in = static_cast<const F *>(a.dy);
     const int bytes_x = ring_bytes(VEC, shape, sizeof(X)), bytes_f = ring_bytes(VEC, shape, sizeof(F));
     const int part_dh = NEXT ? bytes_x : 0, part_f = part_dh + bytes_x, part_dy = part_f + (BRANCH ? bytes_f : 0), part_gate = part_dy + (NEXT ? bytes_f : 0);
-    RowRing<VEC, 1, TEAM> ring{dynamic + 2 * kBackwardParams * 16 * threads, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0),
-                               shape.stages, 0, 0};
+    constexpr int kDh = NEXT ? kParts<X> : 0, kF = kDh + kParts<X>, kDy = kF + (BRANCH ? kParts<F> : 0), kGate = kDy + (NEXT ? kParts<F> : 0);
+    RowRing<VEC, 1, TEAM> ring(dynamic + 2 * kBackwardParams * 16 * threads, p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0),
+                               shape.stages);
     const int stride = gridDim.x / p.cluster, own = blockIdx.x / p.cluster;
     RowCursor load{own, 0, 0}, here;
     load.enter(a);
@@ -772,19 +853,18 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     auto fetch = [&]() {
         if (load.more(a)) {
             const int64_t row = load.base + p.which;
-            if (row < load.end) {
-                if (BRANCH) ring.template fetch<F>(p, shape, part_f, f_in, row, a);
-                if (NEXT) {
-                    ring.template fetch<X>(p, shape, 0, x_in, row, a);
-                    ring.template fetch<F>(p, shape, part_dy, dy_in, row, a);
-                }
-                if (dh_in) ring.template fetch<X>(p, shape, part_dh, dh_in, row, a);
-                if (gate_each) {
-                    if (gate_f32)
-                        ring.template fetch<float>(p, shape, part_gate, static_cast<const float *>(a.gate), row, a);
-                    else
-                        ring.template fetch<F>(p, shape, part_gate, static_cast<const F *>(a.gate), row, a);
-                }
+            const bool some = row < load.end;
+            if (BRANCH) ring.template fetch<F, kF>(p, shape, part_f, f_in, row, some, a);
+            if (NEXT) {
+                ring.template fetch<X, 0>(p, shape, 0, x_in, row, some, a);
+                ring.template fetch<F, kDy>(p, shape, part_dy, dy_in, row, some, a);
+            }
+            if (dh_in) ring.template fetch<X, kDh>(p, shape, part_dh, dh_in, row, some, a);
+            if (gate_each) {
+                if (gate_f32)
+                    ring.template fetch<float, kGate>(p, shape, part_gate, static_cast<const float *>(a.gate), row, some, a);
+                else
+                    ring.template fetch<F, kGate>(p, shape, part_gate, static_cast<const F *>(a.gate), row, some, a);
             }
             load.next(a, p.teams, stride);
         }
@@ -831,25 +911,30 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
                 return;
             }
             if (gate_f32)
-                ring.template get<float>(p, shape, 0, part_gate, static_cast<const float *>(a.gate), at, on, v);
+                ring.template get<float, kGate>(p, shape, 0, part_gate, static_cast<const float *>(a.gate), at, on, v);
             else
-                ring.template get<F>(p, shape, 0, part_gate, static_cast<const F *>(a.gate), at, on, v);
+                ring.template get<F, kGate>(p, shape, 0, part_gate, static_cast<const F *>(a.gate), at, on, v);
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] = mul2(v[k], both(a.branch));
         };
         uint32_t kept = 0xffu;
-        if (BRANCH && a.drop.on) kept = form_mask<VEC, 1>(p, a, key, row, masks, set);
+        if (BRANCH && a.drop.on) {
+            if (VEC)
+                kept = keep_bits(((uint64_t)(at + p.first) >> 3) + p.t, key, a.drop);
+            else
+                form_masks<1>(p, a, key, row, masks, set);
+        }
         if (shape.stages == 1) {
             team_barrier<TEAM>(p);
             fetch();
         }
         ring.ready(p);
-        if (!VEC && BRANCH && a.drop.on) kept = read_mask<1>(p, a, row, masks, set);
+        if (!VEC && BRANCH && a.drop.on) kept = read_masks<1>(p, a, row, masks, set);
         set ^= 1;
         if (shape.stages > 1) fetch();
         float2 t[4];   // the branch, from its norm on normalised
         if (BRANCH) {
-            ring.template get<F>(p, shape, 0, part_f, f_in, at, on, t);
+            ring.template get<F, kF>(p, shape, 0, part_f, f_in, at, on, t);
             if (a.drop.on) drop8(t, kept, a.drop.scale);
             if (BRANCH == 2)
 #pragma unroll
@@ -870,7 +955,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
         float2 d[4];   // the gradient on its way
         if (NEXT) {
             float2 z[4], u[4], s1 = make_float2(0.0f, 0.0f);   // the stream normalised, dy bw
-            ring.template get<X>(p, shape, 0, 0, x_in, at, on, z);
+            ring.template get<X, 0>(p, shape, 0, 0, x_in, at, on, z);
             if (BRANCH) {
                 float2 n[4], gate[4];
                 branch_out(n);
@@ -879,7 +964,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
                 for (int k = 0; k < 4; k++) z[k] = fma2(gate[k], n[k], mul2(z[k], both(a.skip)));
             }
             float2 g[4];
-            ring.template get<F>(p, shape, 0, part_dy, dy_in, at, on, g);
+            ring.template get<F, kDy>(p, shape, 0, part_dy, dy_in, at, on, g);
             param(2, u);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
@@ -898,13 +983,13 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
             });
             const float c1 = -c.x * p.inverse, c2 = layer ? -c.y * p.inverse : 0.0f;
             if (dh_in)
-                ring.template get<X>(p, shape, 0, part_dh, dh_in, at, on, d);
+                ring.template get<X, kDh>(p, shape, 0, part_dh, dh_in, at, on, d);
             else
                 zero8(d);
 #pragma unroll
             for (int k = 0; k < 4; k++) d[k] = fma2(both(st.w), fma2(z[k], both(c1), add2(u[k], both(c2))), d[k]);
         } else {
-            ring.template get<X>(p, shape, 0, part_dh, dh_in, at, on, d);
+            ring.template get<X, kDh>(p, shape, 0, part_dh, dh_in, at, on, d);
         }
         if (a.dx && on) {
             float2 o[4];
