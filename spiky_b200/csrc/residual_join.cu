@@ -306,11 +306,11 @@ static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, RowSh
         int device, threads, cluster, clusters;
         size_t smem;
     };
-    static thread_local Asked kept[9] = {};
-    Asked &k = kept[cfg->stream_type * 3 + cfg->branch_type];
+    static thread_local Asked kept[2][9] = {};
+    Asked &k = kept[backward][cfg->stream_type * 3 + cfg->branch_type];
     if (info.sm_count > 0 && (k.clusters == 0 || k.device != info.device || k.threads != s.threads || k.cluster != s.cluster || k.smem != dynamic))
         k = {info.device, s.threads, s.cluster,
-             by_types(cfg, [&](auto xt, auto ft) { return join_rows_clusters<decltype(xt), decltype(ft)>(s, dynamic); }), dynamic};
+             by_types(cfg, [&](auto xt, auto ft) { return join_rows_clusters<decltype(xt), decltype(ft)>(backward, s, dynamic); }), dynamic};
     return info.sm_count > 0 && k.clusters > 0 ? k.clusters : sm * blocks / s.cluster;
 }
 static bool row_kernels(const lutb_join_cfg *cfg) { return cfg->width <= kRowMaxWidth && cfg->rows <= kRowMaxRows; }

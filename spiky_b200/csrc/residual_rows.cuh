@@ -1,7 +1,7 @@
 // Row kernels of the residual joins: a row's elements stay in registers from the first sum to the last store.
 //
-// A thread has groups of eight elements of a row.  A team of threads has a row: a warp or a part of one, or a block, in the backward pass beyond
-// 2048 elements a cluster of up to eight blocks; sums over a row go through shuffles, shared memory and the cluster's shared memory
+// A thread has groups of eight elements of a row.  A team of threads has a row: a warp or a part of one, a block, or beyond 4096 elements
+// (backward 2048) a cluster of up to eight blocks; sums over a row go through shuffles, shared memory and the cluster's shared memory
 // accordingly, one exchange for each norm and direction (a norm's mean and squares are combined from the warps' own by the pairwise
 // formula of Chan, Golub and LeVeque, 1979, so that no square is taken about a mean that is far off).  What a team does depends on the width
 // alone, so that a row's result does not depend on the rows beside it.
@@ -20,8 +20,8 @@
 namespace lutb {
 
 constexpr int kRowElems = 8;
-constexpr int kBackwardThreads = 256, kForwardThreads = 512, kRowMaxCluster = 8;
-constexpr int64_t kRowMaxWidth = 16384;   // 512 threads of four groups forward, eight blocks of 256 threads of one group backward
+constexpr int kBackwardThreads = 256, kHeldThreads = 512, kOddThreads = 512, kRowMaxCluster = 8;
+constexpr int64_t kRowMaxWidth = 16384;   // backward eight blocks of 256 threads of one group; forward four of 256 of two, or 512 threads of four
 constexpr int64_t kRowMaxRows = 1 << 30;  // (row numbers of 32 bits)
 
 
@@ -32,6 +32,7 @@ struct RowShape {
     int team, teams, threads;   // threads of a row in a block, rows a block has at a time, threads of a block
     int cluster, slice;         // blocks of a row, columns of a block
     int kind;                   // RowTeam
+    int pad;                    // bytes between the places of two stages of a warp
     int stages;                 // rows whose elements a thread has room for in shared memory: this one and those that are fetched
 };
 inline void shape_team(RowShape &s, int64_t width, int block) {
@@ -50,21 +51,28 @@ inline void shape_team(RowShape &s, int64_t width, int block) {
         s.kind = s.cluster > 1 ? TEAM_CLUSTER : TEAM_BLOCK;
     }
 }
-// Forward: up to 256 elements one group a thread, up to 1024 four, always within a warp; then blocks.  Rows that are not VEC have one group up to
+// Forward.  VEC: up to 256 elements one group a thread, up to 1024 four, always within a warp, with the parameters read for each row (20 KB at most, which
+// stay in L1); beyond, two groups with the parameters in registers and slots of shared memory: read again for each row they came from L2, 20 bytes an element
+// against the rows' own 8 at 16 bits (12288 x 8192 bf16 with all of them: 313 us so, 200 us held).  Rows that are not VEC have one group up to
 // 2048, where a warp's loads cover more neighbours.
 inline RowShape forward_shape(int64_t width, bool vec) {
     RowShape s{};
     s.cluster = 1;
-    s.groups = width <= (vec ? 256 : 2048) ? 1 : 4;
+    s.groups = vec ? (width <= 256 ? 1 : width <= 1024 ? 4 : 2) : width <= 2048 ? 1 : 4;
+    if (vec)
+        while (width > (int64_t)s.cluster * 2 * kRowElems * kHeldThreads) s.cluster *= 2;
     shape_team(s, width, 128);
     return s;
 }
-// Backward: one group, whose five sums over the rows take forty registers.
+// Backward: one group, whose five sums over the rows take forty registers.  Stages of a block's or cluster's rows 16 bytes apart measured faster
+// than end to end (32768 x 1024 fp32 145 against 165 us, 12288 x 8192 bf16 558 against 575), those of a warp's rows did not (65536 x 256: 78 against
+// 75), nor did the forward pass's.
 inline RowShape backward_shape(int64_t width) {
     RowShape s{};
     s.cluster = s.groups = 1;
     while (width > (int64_t)s.cluster * kRowElems * kBackwardThreads) s.cluster *= 2;
     shape_team(s, width, kBackwardThreads);
+    s.pad = s.kind == TEAM_WARP ? 0 : 16;
     return s;
 }
 
@@ -157,18 +165,14 @@ __device__ __forceinline__ void drop8(float2 *v, const DropDigits &d, float scal
         v[k].y = d.w[k] > d.above ? v[k].y : 0.0f;
     }
 }
-// (16 bytes, or zeros where there are none to fetch)
-__device__ __forceinline__ void copy16_or_zeros(uint32_t to, const void *from, bool some) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(some ? 16 : 0) : "memory");
-}
-
 // ------------------------------------------------------------------------------------------------ a thread's place
 // Values that warps exchange: of two numbers each, two sets in turn (a set is written again only after the barrier of the next one, which a
 // thread reaches when it has read this one).
 template <int WARPS, int CLUSTER>
 struct RowSlots {
+    static constexpr int kWarps = WARPS;
     float a[2][WARPS * CLUSTER], b[2][WARPS * CLUSTER];
-    float count[WARPS];    // elements of the warps
+    float count[WARPS * CLUSTER];   // elements of the warps
     uint64_t arrived[2];   // clusters: all blocks' values of a set have come
 };
 
@@ -213,24 +217,33 @@ __device__ __forceinline__ RowPlace row_place(const JoinArgs &a, const RowShape 
     p.turn = 0;
     p.waits = true;
     p.valid = 0;
-    int count = 0;
 #pragma unroll
     for (int g = 0; g < G; g++) {
         if (VEC) {
-            if (row_column<VEC>(p, g, 0) < p.limit) p.valid |= 1u << g, count += 8;
+            if (row_column<VEC>(p, g, 0) < p.limit) p.valid |= 1u << g;
         } else {
 #pragma unroll
             for (int k = 0; k < 8; k++)
-                if (row_column<VEC>(p, g, k) < p.limit) p.valid |= 1u << (g * 8 + k), count++;
+                if (row_column<VEC>(p, g, k) < p.limit) p.valid |= 1u << (g * 8 + k);
         }
     }
     if (TEAM != TEAM_WARP && s.team > 32) {
-        constexpr int kAll = sizeof(slots.a[0]) / sizeof(float), kWarps = sizeof(slots.count) / sizeof(float);
+        constexpr int kAll = sizeof(slots.a[0]) / sizeof(float), kWarps = Slots::kWarps;
         for (int k = tid; k < kAll; k += blockDim.x) slots.a[0][k] = slots.a[1][k] = slots.b[0][k] = slots.b[1][k] = 0.0f;
-        if (tid < kWarps) slots.count[tid] = 0.0f;
-        count = __reduce_add_sync(0xffffffffu, count);
+        constexpr int kCounts = sizeof(slots.count) / sizeof(float);
+        for (int k = tid; k < kCounts; k += blockDim.x) {   // elements of the row's warps, other blocks' too (VEC: their groups' 256 columns)
+            const int rank = k / kWarps, warp = k - rank * kWarps, end = (int)min((int64_t)(rank + 1) * s.slice, a.width);
+            int n = 0;
+            if (rank < p.cluster && warp < (s.team >> 5)) {
+#pragma unroll
+                for (int g = 0; g < (VEC ? G : 8 * G); g++) {
+                    const int step = VEC ? 8 : 1, begin = rank * s.slice + (g * s.team + warp * 32) * step;
+                    n += max(0, min(end - begin, 32 * step));
+                }
+            }
+            slots.count[k] = (float)n;
+        }
         __syncthreads();
-        if ((tid & 31) == 0) slots.count[tid >> 5] = (float)count;
         if (p.cluster > 1) {
             if (tid == 0) {
                 mbar_init(smem_u32(&slots.arrived[0]), 1);
@@ -258,6 +271,17 @@ __device__ __forceinline__ float team_sum(float v, int team) {   // teams of a w
     }
     return v;
 }
+// Both sums over the warp: one exchange sends each half of the lanes its value, the others add one value a lane; all lanes have both in the end.
+__device__ __forceinline__ void warp_sums(float &a, float &b) {
+    const bool upper = threadIdx.x & 16;
+    float v = upper ? b : a;
+    v += __shfl_xor_sync(0xffffffffu, upper ? a : b, 16);
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    const float other = __shfl_xor_sync(0xffffffffu, v, 16);
+    a = upper ? other : v;
+    b = upper ? v : other;
+}
 template <int TEAM>
 __device__ __forceinline__ bool within_warp(const RowPlace &p) { return TEAM == TEAM_WARP || (TEAM == TEAM_ANY && p.team <= 32); }
 template <int TEAM>
@@ -281,7 +305,7 @@ __device__ __forceinline__ void publish(const RowPlace &p, Slots &slots, float a
     const int warps = p.team >> 5;
     if (threadIdx.x == 0) mbar_arrive_expect_tx(smem_u32(&slots.arrived[set]), (uint32_t)(8 * warps * p.cluster));
     if (lane < p.cluster) {
-        const int at = p.rank * (kBackwardThreads / 32) + warp;
+        const int at = p.rank * Slots::kWarps + warp;
         uint32_t to_a = smem_u32(&slots.a[set][at]), to_b = smem_u32(&slots.b[set][at]), bar = smem_u32(&slots.arrived[set]);
         asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(to_a) : "r"(lane));
         asm("mapa.shared::cluster.u32 %0, %0, %1;" : "+r"(to_b) : "r"(lane));
@@ -331,11 +355,12 @@ __device__ __forceinline__ float slot_sum(const float *from) {
 }
 template <int TEAM, class Slots>
 __device__ __forceinline__ float all_slots(const RowPlace &p, const float *from) {
-    constexpr int kWarps = sizeof(Slots::count) / sizeof(float);
-    float s = slot_sum<kWarps>(from);
-    if (over_cluster<TEAM>(p))
-        for (int r = 1; r < p.cluster; r++) s += slot_sum<kWarps>(from + r * kWarps);
-    return s;
+    constexpr int kWarps = Slots::kWarps;
+    if (!over_cluster<TEAM>(p)) return slot_sum<kWarps>(from);
+    const int lane = threadIdx.x & 31, n = p.cluster * kWarps;   // 16, 32 or 64 slots, one or two a lane
+    float v = lane < n ? from[lane] : 0.0f;
+    if (n > 32) v += from[lane + 32];
+    return warp_sum(v);
 }
 // Sums of two values over the row; `between` runs while the others arrive.
 template <int TEAM, class Slots, class Fn>
@@ -346,14 +371,28 @@ __device__ __forceinline__ float2 row_sums(RowPlace &p, Slots &slots, float a, f
         between();
         return make_float2(a, b);
     }
-    a = warp_sum(a);
-    if (second) b = warp_sum(b);
+    if (second)
+        warp_sums(a, b);
+    else
+        a = warp_sum(a);
     publish<TEAM>(p, slots, a, b);
     between();
     collect<TEAM>(p, slots);
-    const float2 s = make_float2(all_slots<TEAM, Slots>(p, slots.a[p.turn & 1]), second ? all_slots<TEAM, Slots>(p, slots.b[p.turn & 1]) : 0.0f);
+    const float *const sa = slots.a[p.turn & 1], *const sb = slots.b[p.turn & 1];
     p.turn++;
-    return s;
+    if (over_cluster<TEAM>(p) && second) {   // the slots' values over the lanes, then as before
+        constexpr int kWarps = Slots::kWarps;
+        const int lane = threadIdx.x & 31, n = p.cluster * kWarps;   // 16, 32 or 64 slots, one or two a lane
+        a = lane < n ? sa[lane] : 0.0f;
+        b = lane < n ? sb[lane] : 0.0f;
+        if (n > 32) {
+            a += sa[lane + 32];
+            b += sb[lane + 32];
+        }
+        warp_sums(a, b);
+        return make_float2(a, b);
+    }
+    return make_float2(all_slots<TEAM, Slots>(p, sa), second ? all_slots<TEAM, Slots>(p, sb) : 0.0f);
 }
 // Mean (0 for an RMS norm) and reciprocal deviation of the row's values.  Values of no element do not count (in rows that are not VEC
 // they are 0).
@@ -394,30 +433,42 @@ __device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const flo
         const float mean = layer ? team_sum(sum(), p.team) / p.width : 0.0f;
         return make_float2(mean, rsqrtf(team_sum(squares(mean), p.team) * p.inverse + eps));
     }
-    const int set = p.turn & 1;
+    const int set = p.turn & 1, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    constexpr int kWarps = Slots::kWarps;
     float mean = 0.0f, s;
     if (layer) {
-        const float count = slots.count[threadIdx.x >> 5];
+        const float count = slots.count[p.rank * kWarps + warp];
         mean = count > 0.0f ? warp_sum(sum()) / count : 0.0f;
     }
     publish<TEAM>(p, slots, warp_sum(squares(mean)), mean);
     collect<TEAM>(p, slots);
-    s = all_slots<TEAM, Slots>(p, slots.a[set]);
     mean = 0.0f;
-    if (layer) {
-        constexpr int kWarps = sizeof(Slots::count) / sizeof(float);
-        float m[kWarps], n[kWarps];
-#pragma unroll
-        for (int k = 0; k < kWarps; k++) {
-            m[k] = slots.b[set][k];
-            n[k] = slots.count[k];
-            mean = fmaf(m[k], n[k], mean);
+    if (over_cluster<TEAM>(p)) {   // the row's warps over the lanes, 16 or 32 of them
+        static_assert(TEAM != TEAM_CLUSTER || sizeof(slots.a[0]) <= 32 * sizeof(float) || G == 1, "a slot a lane");
+        const bool some = lane < p.cluster * kWarps;
+        s = some ? slots.a[set][lane] : 0.0f;
+        if (layer) {
+            const float m = some ? slots.b[set][lane] : 0.0f, n = some ? slots.count[lane] : 0.0f;
+            mean = warp_sum(m * n) / p.width;
+            s = fmaf(n * (m - mean), m - mean, s);
         }
-        mean /= p.width;
-        float between = 0.0f;
+        s = warp_sum(s);
+    } else {
+        s = slot_sum<kWarps>(slots.a[set]);
+        if (layer) {
+            float m[kWarps], n[kWarps];
 #pragma unroll
-        for (int k = 0; k < kWarps; k++) between = fmaf(n[k] * (m[k] - mean), m[k] - mean, between);
-        s += between;
+            for (int k = 0; k < kWarps; k++) {
+                m[k] = slots.b[set][k];
+                n[k] = slots.count[k];
+                mean = fmaf(m[k], n[k], mean);
+            }
+            mean /= p.width;
+            float between = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kWarps; k++) between = fmaf(n[k] * (m[k] - mean), m[k] - mean, between);
+            s += between;
+        }
     }
     p.turn++;
     return make_float2(mean, rsqrtf(s * p.inverse + eps));
@@ -532,20 +583,19 @@ struct RowRing {
             swapped = u >> 2 & 1;
         }
     }
-    // What this thread fetches of a row of one array.
+    // What this thread fetches of a row of one array.  VEC: pieces that the row does not have are another one's.
     template <class T, int AT>
     __device__ __forceinline__ void fetch(const RowPlace &p, const RowShape &s, int part, const T *from, int64_t row, bool some, const JoinArgs &a) const {
         constexpr int kEach = 16 / sizeof(T);
         if constexpr (VEC) {
-            const T *const begin = from + (some ? row * a.width : 0);
+            const T *const begin = from + row * a.width;
             const uint32_t to = smem_u32(at) + fill + AT * 512 + mine * kParts<T>;
 #pragma unroll
             for (int g = 0; g < G; g++)
 #pragma unroll
                 for (int q = 0; q < kParts<T>; q++) {
                     const int c = q * wide + u, column = p.first + (g * p.team + p.t - u) * 8 + c * kEach;
-                    const bool there = some && column < p.limit;
-                    copy16_or_zeros(to + g * kParts<T> * 512 + (kParts<T> == 2 ? c ^ (c >> 3 & 1) : c) * 16, begin + (there ? column : 0), there);
+                    copy16(to + g * kParts<T> * 512 + (kParts<T> == 2 ? c ^ (c >> 3 & 1) : c) * 16, begin + min(column, p.limit - kEach));
                 }
         } else {
             if (!some) return;
@@ -585,7 +635,7 @@ struct RowRing {
             team_barrier<TEAM>(p);
     }
     __device__ __forceinline__ void taken() { take = take + stage_bytes == stages * stage_bytes ? 0 : take + stage_bytes; }
-    // Eight elements; 0 where there are none.
+    // Eight elements; where there are none: 0, in VEC rows those of another group or row.
     template <class T, int AT>
     __device__ __forceinline__ void get(const RowPlace &p, const RowShape &s, int g, int part, const T *from, int64_t begin, bool on, float2 *v) const {
         if constexpr (VEC) {
@@ -649,30 +699,36 @@ constexpr size_t kMaskBytes = 2 * (G * THREADS + THREADS);   // two sets, a byte
 
 // ------------------------------------------------------------------------------------------------ forward
 // BRANCH: 0 no branch (the norm alone), 1 a branch, 2 a branch with a norm of its own.  NEXT: the norm before the next block.
+// The parameters that a forward kernel keeps in shared memory.
+__host__ __device__ inline int held_bytes(const RowShape &s) { return s.kind == TEAM_WARP ? 0 : 2 * s.groups * kRowElems * 4 * s.threads; }
 template <int G, int TEAM>
-constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : G == 1 ? 256 : kForwardThreads;
+constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : TEAM == TEAM_ANY ? (G == 4 ? kOddThreads : 256) : kHeldThreads;
+constexpr int kForwardCluster = 2;
 
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int G, int TEAM>
 __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
     constexpr int kThreads = kThreadsOf<G, TEAM>;
+    constexpr bool kHeld = TEAM == TEAM_BLOCK || TEAM == TEAM_CLUSTER;   // the parameters stay in registers
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ __align__(16) RowSlots<TEAM == TEAM_WARP ? 4 : kThreads / 32, 1> slots;
+    __shared__ __align__(16) RowSlots<TEAM == TEAM_WARP ? 4 : kThreads / 32, TEAM == TEAM_CLUSTER ? kForwardCluster : 1> slots;
     __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<G, kThreads>];
     RowPlace p = row_place<VEC, G, TEAM>(a, shape, slots);
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
     const bool gate_each = BRANCH && a.gate_rows == 1, gate_f32 = sizeof(F) == 4 || a.gate_f32;
+    constexpr bool sure = kHeld;   // (a row in every turn)
     const int part_f = ring_bytes(VEC, shape, sizeof(X)), part_gate = part_f + (BRANCH ? ring_bytes(VEC, shape, sizeof(F)) : 0);
     constexpr int kF = G * kParts<X>, kGate = kF + (BRANCH ? G * kParts<F> : 0);
-    RowRing<VEC, G, TEAM> ring(dynamic, p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0), shape.stages);
+    RowRing<VEC, G, TEAM> ring(dynamic + (kHeld ? held_bytes(shape) : 0), p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0), shape.stages);
     const X *const x_in = static_cast<const X *>(a.x);
     const F *const f_in = static_cast<const F *>(a.f);
-    RowCursor load{(int)blockIdx.x, 0, 0}, here;
+    const int stride = gridDim.x / p.cluster;
+    RowCursor load{(int)blockIdx.x / p.cluster, 0, 0}, here;
     load.enter(a);
     here = load;
     auto fetch = [&]() {
         if (load.more(a)) {
-            const int64_t row = load.base + p.which;
-            const bool some = row < load.end;
+            const bool some = sure || load.base + p.which < load.end;
+            const int64_t row = some ? load.base + p.which : load.end - 1;
             ring.template fetch<X, 0>(p, shape, 0, x_in, row, some, a);
             if (BRANCH) ring.template fetch<F, kF>(p, shape, part_f, f_in, row, some, a);
             if (gate_each) {
@@ -681,22 +737,73 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
                 else
                     ring.template fetch<F, kGate>(p, shape, part_gate, static_cast<const F *>(a.gate), row, some, a);
             }
-            load.next(a, p.teams, gridDim.x);
+            load.next(a, p.teams, stride);
         }
         ring.filled();
     };
     for (int s = 1; s < shape.stages; s++) fetch();
     uint32_t set = 0;
+    // Held: the norm after the block with the gate and the branch's scale in it, in registers; the norm before the next block in slots of this
+    // thread's own, [warp][weight, bias][group][half][lane] (all of them in registers spilled).
+    constexpr int H = kHeld ? G : 1;
+    float2 aw[H][4], ab[H][4];
+    float4 *const slot = reinterpret_cast<float4 *>(dynamic) + (threadIdx.x >> 5) * (4 * H * 32) + (threadIdx.x & 31);
+    auto hold = [&](const void *from, bool f32, int64_t at, float none, float2 (*v)[4]) {
+#pragma unroll
+        for (int g = 0; g < H; g++) {
+            if (from != nullptr) {
+                param8<F, VEC>(p, g, from, f32, at, v[g]);
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = both(none);
+            }
+        }
+    };
+    auto hold_branch = [&](int64_t gate_at) {
+        if (BRANCH == 2) {
+            hold(a.aw, a.params_f32, 0, 1.0f, aw);
+            hold(a.ab, a.params_f32, 0, 0.0f, ab);
+        } else {
+            hold(nullptr, true, 0, 1.0f, aw);
+        }
+#pragma unroll
+        for (int g = 0; g < H; g++) {
+            float2 gate[4] = {both(1.0f), both(1.0f), both(1.0f), both(1.0f)};
+            if (a.gate != nullptr && !gate_each) param8<F, VEC>(p, g, a.gate, gate_f32, gate_at, gate);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                gate[k] = mul2(gate[k], both(a.branch));
+                aw[g][k] = mul2(aw[g][k], gate[k]);
+                if (BRANCH == 2) ab[g][k] = mul2(ab[g][k], gate[k]);
+            }
+        }
+    };
+    if (kHeld) {
+        if (BRANCH) hold_branch(0);
+        if (NEXT) {
+            float2 v[H][4];
+#pragma unroll
+            for (int n = 0; n < 2; n++) {
+                hold(n ? a.bb : a.bw, a.params_f32, 0, n ? 0.0f : 1.0f, v);
+#pragma unroll
+                for (int g = 0; g < H; g++) {
+                    slot[((n * H + g) * 2) * 32] = make_float4(v[g][0].x, v[g][0].y, v[g][1].x, v[g][1].y);
+                    slot[((n * H + g) * 2 + 1) * 32] = make_float4(v[g][2].x, v[g][2].y, v[g][3].x, v[g][3].y);
+                }
+            }
+        }
+    }
     int64_t gate_at = 0;   // the gate row in use
     int gate_end = 0;      // the first row of another one
-    for (; here.more(a); here.next(a, p.teams, gridDim.x)) {
+    for (; here.more(a); here.next(a, p.teams, stride)) {
         const int row = here.base + p.which;
         const int64_t at = row * a.width;
-        const bool on = row < here.end;
+        const bool on = sure || row < here.end;
         if (BRANCH && a.gate_rows > 1 && on && row >= gate_end) {
             const int gate_row = row / (int)a.gate_rows;
             gate_end = (gate_row + 1) * (int)a.gate_rows;
             gate_at = gate_row * a.width;
+            if (kHeld) hold_branch(gate_at);
         }
         const bool drop = BRANCH && a.drop.on;
         if (!VEC && drop) form_masks<G>(p, a, key, row, masks, set);
@@ -733,7 +840,13 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
             for (int g = 0; g < G; g++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) v[g][k] = mul2(add2(v[g][k], both(-s.x)), both(s.y));
-            affine<F, VEC, G>(p, a.aw, a.ab, a.params_f32, v);
+            if (!kHeld) affine<F, VEC, G>(p, a.aw, a.ab, a.params_f32, v);
+        }
+        if (kHeld && BRANCH) {
+#pragma unroll
+            for (int g = 0; g < G; g++)
+#pragma unroll
+                for (int k = 0; k < 4; k++) v[g][k] = BRANCH == 2 ? fma2(v[g][k], aw[g % H][k], ab[g % H][k]) : mul2(v[g][k], aw[g % H][k]);
         }
         if (BRANCH) {
             auto gated = [&](auto get) {
@@ -750,7 +863,7 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
                     gated([&](int g, float2 *e) { ring.template get<float, kGate>(p, shape, g, part_gate, static_cast<const float *>(a.gate), at, on, e); });
                 else
                     gated([&](int g, float2 *e) { ring.template get<F, kGate>(p, shape, g, part_gate, static_cast<const F *>(a.gate), at, on, e); });
-            } else if (a.gate != nullptr) {
+            } else if (!kHeld && a.gate != nullptr) {
                 if (gate_f32)
                     gated([&](int g, float2 *e) { param8<F, VEC>(p, g, a.gate, true, gate_at, e); });
                 else
@@ -762,7 +875,8 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
             float2 x[4];
             ring.template get<X, 0>(p, shape, g, 0, x_in, at, on, x);
 #pragma unroll
-            for (int k = 0; k < 4; k++) v[g][k] = BRANCH ? fma2(v[g][k], both(a.branch), mul2(x[k], both(a.skip))) : x[k];
+            for (int k = 0; k < 4; k++)
+                v[g][k] = !BRANCH ? x[k] : kHeld ? fma2(x[k], both(a.skip), v[g][k]) : fma2(v[g][k], both(a.branch), mul2(x[k], both(a.skip)));
             if (!VEC && BRANCH) {
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -780,14 +894,25 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>
             for (int g = 0; g < G; g++)
 #pragma unroll
                 for (int k = 0; k < 4; k++) v[g][k] = mul2(add2(v[g][k], both(-s.x)), both(s.y));
-            affine<F, VEC, G>(p, a.bw, a.bb, a.params_f32, v);
+            if (kHeld) {
+#pragma unroll
+                for (int g = 0; g < G; g++)
+#pragma unroll
+                    for (int half = 0; half < 2; half++) {
+                        const float4 w = slot[((g % H) * 2 + half) * 32], b = slot[((H + g % H) * 2 + half) * 32];
+                        v[g][2 * half] = fma2(v[g][2 * half], make_float2(w.x, w.y), make_float2(b.x, b.y));
+                        v[g][2 * half + 1] = fma2(v[g][2 * half + 1], make_float2(w.z, w.w), make_float2(b.z, b.w));
+                    }
+            }
+            if (!kHeld) affine<F, VEC, G>(p, a.bw, a.bb, a.params_f32, v);
             if (on)
 #pragma unroll
                 for (int g = 0; g < G; g++) store_row<F, VEC>(p, g, static_cast<F *>(a.y) + at, v[g]);
         }
-        if (a.stats && on && p.t == 0) a.stats[row] = st;
+        if (a.stats && on && p.t == 0 && p.rank == 0) a.stats[row] = st;
         ring.taken();
     }
+    if (over_cluster<TEAM>(p)) cluster_meet();   // (no block is gone while another may store into it)
 }
 
 // ------------------------------------------------------------------------------------------------ backward
@@ -843,8 +968,9 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     const F *const f_in = static_cast<const F *>(a.f), *const dy_in = static_cast<const F *>(a.dy);
     const int bytes_x = ring_bytes(VEC, shape, sizeof(X)), bytes_f = ring_bytes(VEC, shape, sizeof(F));
     const int part_dh = NEXT ? bytes_x : 0, part_f = part_dh + bytes_x, part_dy = part_f + (BRANCH ? bytes_f : 0), part_gate = part_dy + (NEXT ? bytes_f : 0);
+    constexpr bool sure = TEAM == TEAM_BLOCK || TEAM == TEAM_CLUSTER;   // (a row in every turn)
     constexpr int kDh = NEXT ? kParts<X> : 0, kF = kDh + kParts<X>, kDy = kF + (BRANCH ? kParts<F> : 0), kGate = kDy + (NEXT ? kParts<F> : 0);
-    RowRing<VEC, 1, TEAM> ring(dynamic + 2 * kBackwardParams * 16 * threads, p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0),
+    RowRing<VEC, 1, TEAM> ring(dynamic + 2 * kBackwardParams * 16 * threads, p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0) + shape.pad * (threads / 32),
                                shape.stages);
     const int stride = gridDim.x / p.cluster, own = blockIdx.x / p.cluster;
     RowCursor load{own, 0, 0}, here;
@@ -852,8 +978,8 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     here = load;
     auto fetch = [&]() {
         if (load.more(a)) {
-            const int64_t row = load.base + p.which;
-            const bool some = row < load.end;
+            const bool some = sure || load.base + p.which < load.end;
+            const int64_t row = some ? load.base + p.which : load.end - 1;
             if (BRANCH) ring.template fetch<F, kF>(p, shape, part_f, f_in, row, some, a);
             if (NEXT) {
                 ring.template fetch<X, 0>(p, shape, 0, x_in, row, some, a);
@@ -898,8 +1024,8 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     while (here.more(a)) {
         const int row = here.base + p.which, chunk = here.chunk;
         const int64_t at = row * a.width;
-        const bool on = row < here.end;
-        const float4 st = on ? a.stats[row] : make_float4(0.0f, 1.0f, 0.0f, 1.0f);
+        const bool on = sure || row < here.end;
+        const float4 st = a.stats[on ? row : here.end - 1];
         if (BRANCH && a.gate_rows > 1 && on && row >= gate_end) {
             const int gate_row = row / (int)a.gate_rows;
             gate_end = (gate_row + 1) * (int)a.gate_rows;
@@ -972,8 +1098,8 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
                 u[k] = mul2(g[k], u[k]);
                 s1 = fma2(u[k], z[k], s1);
             }
-            const bool layer = a.before == LUTB_NORM_LAYER;
-            const float2 c = row_sums<TEAM>(p, slots, s1.x + s1.y, layer ? total(u) : 0.0f, layer, [&]() {
+            const bool layer = a.before == LUTB_NORM_LAYER, some = !VEC || p.valid;
+            const float2 c = row_sums<TEAM>(p, slots, some ? s1.x + s1.y : 0.0f, layer && some ? total(u) : 0.0f, layer, [&]() {
                 if (!on) return;
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
@@ -1082,11 +1208,11 @@ int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs
 template <class X, class F>
 size_t join_rows_smem(bool backward, bool vec, const RowShape &s, bool gate_each) {
     const size_t x = ring_bytes(vec, s, sizeof(X)), f = ring_bytes(vec, s, sizeof(F)), gate = gate_each ? ring_bytes(vec, s, 4) : 0;
-    return (backward ? 2 * kBackwardParams * 16 * s.threads : 0) + s.stages * ((backward ? 2 : 1) * (x + f) + gate);
+    return (backward ? 2 * kBackwardParams * 16 * s.threads : vec ? held_bytes(s) : 0) + s.stages * ((backward ? 2 : 1) * (x + f) + gate + s.pad * (s.threads / 32));
 }
-// Clusters of a backward kernel that are resident at a time, as the driver counts them; 0 where it cannot be asked.
+// Clusters of a kernel that are resident at a time, as the driver counts them; 0 where it cannot be asked.
 template <class X, class F>
-int join_rows_clusters(const RowShape &s, size_t smem);
+int join_rows_clusters(bool backward, const RowShape &s, size_t smem);
 template <class X, class F, int BRANCH, bool NEXT>
 const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
 #define LUTB_FORWARD(VEC, G, TEAM) reinterpret_cast<const void *>(&join_rows_forward_kernel<X, F, BRANCH, NEXT, VEC, G, TEAM>)
@@ -1097,7 +1223,7 @@ const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
     }
     if (!vec) return s.groups == 1 ? LUTB_FORWARD(false, 1, TEAM_ANY) : LUTB_FORWARD(false, 4, TEAM_ANY);
     if (s.kind == TEAM_WARP) return s.groups == 1 ? LUTB_FORWARD(true, 1, TEAM_WARP) : LUTB_FORWARD(true, 4, TEAM_WARP);
-    return LUTB_FORWARD(true, 4, TEAM_BLOCK);
+    return s.kind == TEAM_BLOCK ? LUTB_FORWARD(true, 2, TEAM_BLOCK) : LUTB_FORWARD(true, 2, TEAM_CLUSTER);
 #undef LUTB_FORWARD
 #undef LUTB_BACKWARD
 }
@@ -1127,8 +1253,8 @@ int join_rows_wait_errors(int *count);
         return launch_join_rows<X, F>(backward, vec, a, s, clusters, stream);                                                      \
     }                                                                                                                               \
     template <>                                                                                                                     \
-    int join_rows_clusters<X, F>(const RowShape &s, size_t smem) {                                                                  \
-        return resident_clusters(join_rows_kernel<X, F, 2, true>(true, true, s), s, smem);                                          \
+    int join_rows_clusters<X, F>(bool backward, const RowShape &s, size_t smem) {                                                   \
+        return resident_clusters(join_rows_kernel<X, F, 2, true>(backward, true, s), s, smem);                                      \
     }                                                                                                                               \
     template <>                                                                                                                     \
     int join_rows_wait_errors<X, F>(int *count) {                                                                                   \
