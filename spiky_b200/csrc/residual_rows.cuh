@@ -20,12 +20,13 @@
 namespace lutb {
 
 constexpr int kRowElems = 8;
-constexpr int kBackwardThreads = 256, kHeldThreads = 512, kOddThreads = 512, kRowMaxCluster = 8;
-constexpr int64_t kRowMaxWidth = 16384;   // backward eight blocks of 256 threads of one group; forward four of 256 of two, or 512 threads of four
+constexpr int kBlockThreads = 256, kWideThreads = 512;   // of a team; a warp's teams share a block of 128 forward, 256 backward
+constexpr int kForwardCluster = 2, kBackwardCluster = 4;
+constexpr int64_t kRowMaxWidth = 16384;   // such clusters of 512 threads, of two groups forward and one backward, or 512 threads of four
 constexpr int64_t kRowMaxRows = 1 << 30;  // (row numbers of 32 bits)
 
 
-enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_CLUSTER = 2, TEAM_ANY = 3 };   // ANY: told at run time (rows that are not VEC)
+enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_ANY = 4 };   // a block of 256 or 512 threads; ANY: told at run time (rows that are not VEC)
 
 struct RowShape {
     int groups;                 // of a thread
@@ -48,7 +49,7 @@ inline void shape_team(RowShape &s, int64_t width, int block) {
     } else {
         s.team = s.threads = (t + 31) / 32 * 32;
         s.teams = 1;
-        s.kind = s.cluster > 1 ? TEAM_CLUSTER : TEAM_BLOCK;
+        s.kind = s.cluster > 1 ? TEAM_CLUSTER : s.threads > kBlockThreads ? TEAM_WIDE : TEAM_BLOCK;
     }
 }
 // Forward.  VEC: up to 256 elements one group a thread, up to 1024 four, always within a warp, with the parameters read for each row (20 KB at most, which
@@ -60,7 +61,7 @@ inline RowShape forward_shape(int64_t width, bool vec) {
     s.cluster = 1;
     s.groups = vec ? (width <= 256 ? 1 : width <= 1024 ? 4 : 2) : width <= 2048 ? 1 : 4;
     if (vec)
-        while (width > (int64_t)s.cluster * 2 * kRowElems * kHeldThreads) s.cluster *= 2;
+        while (width > (int64_t)s.cluster * 2 * kRowElems * kWideThreads) s.cluster *= 2;
     shape_team(s, width, 128);
     return s;
 }
@@ -70,8 +71,8 @@ inline RowShape forward_shape(int64_t width, bool vec) {
 inline RowShape backward_shape(int64_t width) {
     RowShape s{};
     s.cluster = s.groups = 1;
-    while (width > (int64_t)s.cluster * kRowElems * kBackwardThreads) s.cluster *= 2;
-    shape_team(s, width, kBackwardThreads);
+    while (width > (int64_t)s.cluster * kRowElems * kWideThreads) s.cluster *= 2;
+    shape_team(s, width, 256);
     s.pad = s.kind == TEAM_WARP ? 0 : 16;
     return s;
 }
@@ -205,10 +206,10 @@ __device__ __forceinline__ RowPlace row_place(const JoinArgs &a, const RowShape 
     RowPlace p;
     const int tid = threadIdx.x;
     p.team = s.team;
-    p.teams = TEAM == TEAM_BLOCK || TEAM == TEAM_CLUSTER ? 1 : s.teams;
+    p.teams = TEAM == TEAM_WARP || TEAM == TEAM_ANY ? s.teams : 1;
     p.which = p.teams == 1 ? 0 : tid / s.team;
     p.t = tid - p.which * s.team;
-    p.cluster = TEAM == TEAM_WARP || TEAM == TEAM_BLOCK ? 1 : s.cluster;
+    p.cluster = TEAM == TEAM_CLUSTER || TEAM == TEAM_ANY ? s.cluster : 1;
     p.rank = p.cluster > 1 ? (int)(blockIdx.x % p.cluster) : 0;
     p.first = p.rank * s.slice;
     p.limit = (int)min((int64_t)p.first + s.slice, a.width);
@@ -444,7 +445,7 @@ __device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const flo
     collect<TEAM>(p, slots);
     mean = 0.0f;
     if (over_cluster<TEAM>(p)) {   // the row's warps over the lanes, 16 or 32 of them
-        static_assert(TEAM != TEAM_CLUSTER || sizeof(slots.a[0]) <= 32 * sizeof(float) || G == 1, "a slot a lane");
+        static_assert(TEAM != TEAM_CLUSTER || sizeof(slots.a[0]) <= 32 * sizeof(float), "a slot a lane");
         const bool some = lane < p.cluster * kWarps;
         s = some ? slots.a[set][lane] : 0.0f;
         if (layer) {
@@ -702,13 +703,12 @@ constexpr size_t kMaskBytes = 2 * (G * THREADS + THREADS);   // two sets, a byte
 // The parameters that a forward kernel keeps in shared memory.
 __host__ __device__ inline int held_bytes(const RowShape &s) { return s.kind == TEAM_WARP ? 0 : 2 * s.groups * kRowElems * 4 * s.threads; }
 template <int G, int TEAM>
-constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : TEAM == TEAM_ANY ? (G == 4 ? kOddThreads : 256) : kHeldThreads;
-constexpr int kForwardCluster = 2;
+constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : TEAM == TEAM_BLOCK || (TEAM == TEAM_ANY && G == 1) ? kBlockThreads : kWideThreads;
 
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int G, int TEAM>
 __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
     constexpr int kThreads = kThreadsOf<G, TEAM>;
-    constexpr bool kHeld = TEAM == TEAM_BLOCK || TEAM == TEAM_CLUSTER;   // the parameters stay in registers
+    constexpr bool kHeld = TEAM == TEAM_BLOCK || TEAM == TEAM_WIDE || TEAM == TEAM_CLUSTER;   // the parameters stay in registers
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) RowSlots<TEAM == TEAM_WARP ? 4 : kThreads / 32, TEAM == TEAM_CLUSTER ? kForwardCluster : 1> slots;
     __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<G, kThreads>];
@@ -920,13 +920,17 @@ constexpr int kBackwardParams = 4;   // aw, ab, bw, gate
 
 // See join_backward_kernel for the formulas.  A thread's sums over its rows stay in registers to the end (of the chunk, for a gate row); what a step
 // needs of the row is read from shared memory at that step, so that three sets of eight values are live at most beside the forty sums.
+template <int TEAM>
+constexpr int kBackwardThreads = TEAM == TEAM_WARP || TEAM == TEAM_BLOCK ? kBlockThreads : kWideThreads;
+
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int TEAM>
-__global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel(const JoinArgs a, const RowShape shape) {
+__global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads<TEAM>) join_rows_backward_kernel(const JoinArgs a, const RowShape shape) {
+    constexpr int kThreads = kBackwardThreads<TEAM>;
     constexpr bool kTeams = TEAM == TEAM_WARP || TEAM == TEAM_ANY, kClusters = TEAM == TEAM_CLUSTER || TEAM == TEAM_ANY;
     extern __shared__ __align__(16) unsigned char dynamic[];
-    __shared__ __align__(16) RowSlots<kBackwardThreads / 32, kClusters ? kRowMaxCluster : 1> slots;
-    __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<1, kBackwardThreads>];
-    __shared__ float2 joined[kTeams ? 4 * kBackwardThreads : 1];   // the teams' sums of a block
+    __shared__ __align__(16) RowSlots<kThreads / 32, kClusters ? kBackwardCluster : 1> slots;
+    __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<1, kThreads>];
+    __shared__ float2 joined[kTeams ? 4 * kBlockThreads : 1];   // the teams' sums of a block
     RowPlace p = row_place<VEC, 1, TEAM>(a, shape, slots);
     const int threads = blockDim.x, tid = threadIdx.x;
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
@@ -968,7 +972,7 @@ __global__ void __launch_bounds__(kBackwardThreads, 2) join_rows_backward_kernel
     const F *const f_in = static_cast<const F *>(a.f), *const dy_in = static_cast<const F *>(a.dy);
     const int bytes_x = ring_bytes(VEC, shape, sizeof(X)), bytes_f = ring_bytes(VEC, shape, sizeof(F));
     const int part_dh = NEXT ? bytes_x : 0, part_f = part_dh + bytes_x, part_dy = part_f + (BRANCH ? bytes_f : 0), part_gate = part_dy + (NEXT ? bytes_f : 0);
-    constexpr bool sure = TEAM == TEAM_BLOCK || TEAM == TEAM_CLUSTER;   // (a row in every turn)
+    constexpr bool sure = !kTeams;   // (a row in every turn)
     constexpr int kDh = NEXT ? kParts<X> : 0, kF = kDh + kParts<X>, kDy = kF + (BRANCH ? kParts<F> : 0), kGate = kDy + (NEXT ? kParts<F> : 0);
     RowRing<VEC, 1, TEAM> ring(dynamic + 2 * kBackwardParams * 16 * threads, p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0) + shape.pad * (threads / 32),
                                shape.stages);
@@ -1219,17 +1223,20 @@ const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
 #define LUTB_BACKWARD(VEC, TEAM) reinterpret_cast<const void *>(&join_rows_backward_kernel<X, F, BRANCH, NEXT, VEC, TEAM>)
     if (backward) {
         if (!vec) return LUTB_BACKWARD(false, TEAM_ANY);
-        return s.kind == TEAM_WARP ? LUTB_BACKWARD(true, TEAM_WARP) : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(true, TEAM_BLOCK) : LUTB_BACKWARD(true, TEAM_CLUSTER);
+        return s.kind == TEAM_WARP    ? LUTB_BACKWARD(true, TEAM_WARP)
+               : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(true, TEAM_BLOCK)
+               : s.kind == TEAM_WIDE  ? LUTB_BACKWARD(true, TEAM_WIDE)
+                                      : LUTB_BACKWARD(true, TEAM_CLUSTER);
     }
     if (!vec) return s.groups == 1 ? LUTB_FORWARD(false, 1, TEAM_ANY) : LUTB_FORWARD(false, 4, TEAM_ANY);
     if (s.kind == TEAM_WARP) return s.groups == 1 ? LUTB_FORWARD(true, 1, TEAM_WARP) : LUTB_FORWARD(true, 4, TEAM_WARP);
-    return s.kind == TEAM_BLOCK ? LUTB_FORWARD(true, 2, TEAM_BLOCK) : LUTB_FORWARD(true, 2, TEAM_CLUSTER);
+    return s.kind == TEAM_BLOCK ? LUTB_FORWARD(true, 2, TEAM_BLOCK) : s.kind == TEAM_WIDE ? LUTB_FORWARD(true, 2, TEAM_WIDE) : LUTB_FORWARD(true, 2, TEAM_CLUSTER);
 #undef LUTB_FORWARD
 #undef LUTB_BACKWARD
 }
 template <class X, class F>
 int launch_join_rows(bool backward, bool vec, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream) {
-    static std::atomic<uint32_t> opted[2][2][6][6];
+    static std::atomic<uint32_t> opted[2][2][6][8];
     const int kind = (a.f == nullptr ? 0 : a.after == LUTB_NORM_NONE ? 1 : 2) * 2 + (backward ? a.dy != nullptr : a.y != nullptr);
     const void *kernel = kind == 1   ? join_rows_kernel<X, F, 0, true>(backward, vec, s)
                          : kind == 2 ? join_rows_kernel<X, F, 1, false>(backward, vec, s)
