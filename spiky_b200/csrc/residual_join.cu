@@ -201,7 +201,7 @@ __global__ void __launch_bounds__(kRowThreads) join_backward_kernel(const JoinAr
     }
 }
 
-// The blocks' sums into the gradients: 32 columns a block, its warps share the partial sums; always the same order.
+// The blocks' sums into the gradients: 32 lanes of V columns a block, whose warps share the partial sums; always the same order.
 struct SumList {
     const float *from[5];
     void *to[5];
@@ -209,27 +209,62 @@ struct SumList {
     int32_t f32[5];
     int32_t count;      // lists of one row each; the gate's rows follow
 };
-template <class F>
+template <class F, int V>
 __global__ void __launch_bounds__(1024) join_sums_kernel(const SumList l, int64_t width) {
-    __shared__ float part[32][33];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, k = min((int)blockIdx.y, l.count);
-    const int64_t c = blockIdx.x * 32ll + lane, out_row = (int)blockIdx.y - k;
-    const float *from = l.from[k] + out_row * l.parts[k] * width;
-    float s = 0.0f;
-    if (c < width)
-        for (int64_t p = warp; p < l.parts[k]; p += 32) s += from[p * width + c];
-    part[warp][lane] = s;
-    __syncthreads();
-    s = part[lane][warp];
+    __shared__ float all[32][32 * V + 1];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, k = min((int)blockIdx.y, l.count);
+    const int64_t first = (int64_t)blockIdx.x * (32 * V), c = first + lane * V, out_row = (int)blockIdx.y - k;
+    const float *from = l.from[k] + out_row * l.parts[k] * width + c;
+    constexpr int kAhead = 4;   // loads on their way
+    float s[kAhead][V];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    const int64_t col = blockIdx.x * 32ll + warp;
-    if (lane == 0 && col < width) {
-        if (l.f32[k])
-            static_cast<float *>(l.to[k])[out_row * width + col] = s;
-        else
-            static_cast<F *>(l.to[k])[out_row * width + col] = from_f32<F>(s);
+    for (int a = 0; a < kAhead; a++)
+#pragma unroll
+        for (int e = 0; e < V; e++) s[a][e] = 0.0f;
+    if (c < width)
+        for (int64_t p = warp; p < l.parts[k]; p += kAhead * warps)
+#pragma unroll
+            for (int a = 0; a < kAhead; a++) {
+                if (p + a * warps >= l.parts[k]) break;
+                if constexpr (V == 4) {
+                    const float4 v = *reinterpret_cast<const float4 *>(from + (p + a * warps) * width);
+                    s[a][0] += v.x;
+                    s[a][1] += v.y;
+                    s[a][2] += v.z;
+                    s[a][3] += v.w;
+                } else {
+                    s[a][0] += from[(p + a * warps) * width];
+                }
+            }
+#pragma unroll
+    for (int e = 0; e < V; e++) all[warp][lane * V + e] = (s[0][e] + s[1][e]) + (s[2][e] + s[3][e]);
+    __syncthreads();
+    for (int at = threadIdx.x; at < 32 * V; at += blockDim.x) {
+        float sum = 0.0f;
+        for (int w = 0; w < warps; w++) sum += all[w][at];
+        if (first + at < width) {
+            if (l.f32[k])
+                static_cast<float *>(l.to[k])[out_row * width + first + at] = sum;
+            else
+                static_cast<F *>(l.to[k])[out_row * width + first + at] = from_f32<F>(sum);
+        }
     }
+}
+// Wide rows: four columns a lane and as many warps as have four partial sums each; narrow ones: one column and all warps, so that there are more
+// blocks (1024 columns of 592 sums, three lists: 96 blocks).
+template <class F>
+static int launch_sums(const SumList &l, int64_t out_rows, int64_t width, cudaStream_t stream) {
+    int64_t parts = 1;
+    for (int k = 0; k < 5; k++) parts = l.parts[k] > parts ? l.parts[k] : parts;
+    int warps = 4;
+    while (warps < 32 && 4 * warps < parts) warps *= 2;
+    KernelScope scope(K_JOIN_SUMS, stream);
+    if (width % 4 == 0 && width >= 4096)
+        join_sums_kernel<F, 4><<<dim3((unsigned)((width + 127) / 128), (unsigned)out_rows), 32 * warps, 0, stream>>>(l, width);
+    else
+        join_sums_kernel<F, 1><<<dim3((unsigned)((width + 31) / 32), (unsigned)out_rows), 32 * warps, 0, stream>>>(l, width);
+    LUTB_LAUNCH_CHECK();
+    return LUTB_OK;
 }
 
 // `at_once`: rows that a block takes together.
@@ -547,12 +582,7 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
             }
         }
         const int64_t out_rows = l.count + (gate_summed && !a.gate_direct ? split.chunks / split.per_group : 0);
-        if (out_rows) {
-            KernelScope scope(K_JOIN_SUMS, s);
-            const dim3 grid((unsigned)((cfg->width + 31) / 32), (unsigned)out_rows);
-            join_sums_kernel<decltype(ft)><<<grid, 1024, 0, s>>>(l, cfg->width);
-            LUTB_LAUNCH_CHECK();
-        }
+        if (out_rows) return launch_sums<decltype(ft)>(l, out_rows, cfg->width, s);
         return (int)LUTB_OK;
     });
 }

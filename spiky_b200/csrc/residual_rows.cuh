@@ -26,7 +26,7 @@ constexpr int64_t kRowMaxWidth = 16384;   // such clusters of 512 threads, of tw
 constexpr int64_t kRowMaxRows = 1 << 30;  // (row numbers of 32 bits)
 
 
-enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_ANY = 4 };   // a block of 256 or 512 threads; ANY: told at run time (rows that are not VEC)
+enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_ANY = 4 };   // a block of up to 256 or 512 threads; ANY: told at run time (wide rows that are not VEC, backward)
 
 struct RowShape {
     int groups;                 // of a thread
@@ -490,8 +490,12 @@ __device__ __forceinline__ void param8(const RowPlace &p, int g, const void *fro
         }
     } else {
         float e[8];
+        int64_t c = at + row_column<VEC>(p, g, 0);
 #pragma unroll
-        for (int k = 0; k < 8; k++) e[k] = row_valid<VEC>(p, g, k) ? join_param<F>(from, f32, at + row_column<VEC>(p, g, k), 0.0f) : 0.0f;
+        for (int k = 0; k < 8; k++, c += p.team) {
+            e[k] = 0.0f;
+            if (row_valid<VEC>(p, g, k)) e[k] = sizeof(F) == 4 || f32 ? static_cast<const float *>(from)[c] : to_f32(static_cast<const F *>(from)[c]);
+        }
 #pragma unroll
         for (int k = 0; k < 4; k++) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
     }
@@ -600,22 +604,20 @@ struct RowRing {
                 }
         } else {
             if (!some) return;
-            const uint32_t to = smem_u32(at) + fill + part;
-            const int64_t begin = row * a.width + p.first, total = a.rows * a.width;
-            const unsigned char *const bytes = reinterpret_cast<const unsigned char *>(from);
+            const int64_t begin = row * a.width + p.first, total = a.rows * a.width * (int64_t)sizeof(T);
             const int ahead = (int)(reinterpret_cast<uintptr_t>(from + begin) & 15);   // of the row in its first piece
             const int pieces = (ahead + (p.limit - p.first) * (int)sizeof(T) + 15) / 16;
-            const uint32_t place = to + p.which * ring_row_bytes(s.slice, sizeof(T));
-            for (int c = p.t; c < pieces; c += p.team) {
-                const int64_t offset = begin * (int64_t)sizeof(T) - ahead + c * 16;   // from the array's begin
-                if (offset >= 0 && offset + 16 <= total * (int64_t)sizeof(T)) {
-                    copy16(place + c * 16, bytes + offset);
-                } else {   // a piece that the array does not fill: its elements one by one
-                    T *const own = reinterpret_cast<T *>(at + fill + part + p.which * ring_row_bytes(s.slice, sizeof(T)) + c * 16);
-                    const int64_t element = (begin * (int64_t)sizeof(T) - ahead) / (int64_t)sizeof(T) + c * kEach;
-#pragma unroll
-                    for (int e = 0; e < kEach; e++)
-                        if (element + e >= 0 && element + e < total) own[e] = from[element + e];
+            const int64_t offset = begin * (int64_t)sizeof(T) - ahead;   // of that piece, from the array's begin
+            const unsigned char *const bytes = reinterpret_cast<const unsigned char *>(from) + offset;
+            unsigned char *const place = at + fill + part + p.which * ring_row_bytes(s.slice, sizeof(T));
+            if (offset >= 0 && offset + pieces * 16 <= total) {
+                const uint32_t to = smem_u32(place);
+                for (int c = p.t; c < pieces; c += p.team) copy16(to + c * 16, bytes + c * 16);
+            } else {   // pieces that the array does not fill: their elements one by one
+                for (int c = p.t; c < pieces; c += p.team) {
+                    const int64_t o = offset + c * 16;
+                    for (int e = 0; e < 16; e += (int)sizeof(T))
+                        if (o + e >= 0 && o + e < total) *reinterpret_cast<T *>(place + c * 16 + e) = *reinterpret_cast<const T *>(bytes + c * 16 + e);
                 }
             }
         }
@@ -652,10 +654,14 @@ struct RowRing {
         } else {
             const unsigned char *const stage = at + take + part;
             const int ahead = (int)(reinterpret_cast<uintptr_t>(from + begin + p.first) & 15) / (int)sizeof(T);
-            const T *const own = reinterpret_cast<const T *>(stage + p.which * ring_row_bytes(s.slice, sizeof(T))) + ahead - p.first;
+            const T *own = reinterpret_cast<const T *>(stage + p.which * ring_row_bytes(s.slice, sizeof(T))) + ahead + p.t + g * 8 * p.team;
+            const uint32_t valid = on ? p.valid : 0u;
             float e[8];
 #pragma unroll
-            for (int k = 0; k < 8; k++) e[k] = on && row_valid<VEC>(p, g, k) ? to_f32(own[row_column<VEC>(p, g, k)]) : 0.0f;
+            for (int k = 0; k < 8; k++, own += p.team) {
+                e[k] = 0.0f;
+                if (valid >> (g * 8 + k) & 1) e[k] = to_f32(*own);
+            }
 #pragma unroll
             for (int k = 0; k < 4; k++) v[k] = make_float2(e[2 * k], e[2 * k + 1]);
         }
@@ -667,9 +673,10 @@ __device__ __forceinline__ void store_row(const RowPlace &p, int g, T *row, cons
     if constexpr (VEC) {
         if (row_valid<VEC>(p, g, 0)) store8(row + row_column<VEC>(p, g, 0), v);
     } else {
+        T *to = row + row_column<VEC>(p, g, 0);
 #pragma unroll
-        for (int k = 0; k < 8; k++)
-            if (row_valid<VEC>(p, g, k)) row[row_column<VEC>(p, g, k)] = from_f32<T>(k & 1 ? v[k >> 1].y : v[k >> 1].x);
+        for (int k = 0; k < 8; k++, to += p.team)
+            if (row_valid<VEC>(p, g, k)) *to = from_f32<T>(k & 1 ? v[k >> 1].y : v[k >> 1].x);
     }
 }
 
@@ -686,13 +693,10 @@ __device__ __forceinline__ void form_masks(const RowPlace &p, const JoinArgs &a,
 template <int G>
 __device__ __forceinline__ uint32_t read_masks(const RowPlace &p, const JoinArgs &a, int64_t row, const uint8_t *bytes, uint32_t set) {
     const uint8_t *own = bytes + ((int)set * p.teams + p.which) * (G * p.team + 1);
-    const int off = (int)((row * a.width + p.first) & 7);
+    int e = (int)((row * a.width + p.first) & 7) + p.t;
     uint32_t kept = 0;
 #pragma unroll
-    for (int k = 0; k < 8 * G; k++) {
-        const int e = off + p.t + k * p.team;
-        kept |= (uint32_t)(own[e >> 3] >> (e & 7) & 1) << k;
-    }
+    for (int k = 0; k < 8 * G; k++, e += p.team) kept |= ((uint32_t)own[e >> 3] >> (e & 7) & 1u) << k;
     return kept;
 }
 template <int G, int THREADS>
@@ -701,24 +705,26 @@ constexpr size_t kMaskBytes = 2 * (G * THREADS + THREADS);   // two sets, a byte
 // ------------------------------------------------------------------------------------------------ forward
 // BRANCH: 0 no branch (the norm alone), 1 a branch, 2 a branch with a norm of its own.  NEXT: the norm before the next block.
 // The parameters that a forward kernel keeps in shared memory.
-__host__ __device__ inline int held_bytes(const RowShape &s) { return s.kind == TEAM_WARP ? 0 : 2 * s.groups * kRowElems * 4 * s.threads; }
+__host__ __device__ inline int held_bytes(bool vec, const RowShape &s) {
+    return (vec ? s.kind != TEAM_WARP : s.groups == 1) ? 2 * s.groups * kRowElems * 4 * s.threads : 0;
+}
 template <int G, int TEAM>
-constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : TEAM == TEAM_BLOCK || (TEAM == TEAM_ANY && G == 1) ? kBlockThreads : kWideThreads;
+constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : TEAM == TEAM_BLOCK ? kBlockThreads : kWideThreads;
 
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int G, int TEAM>
 __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
     constexpr int kThreads = kThreadsOf<G, TEAM>;
-    constexpr bool kHeld = TEAM == TEAM_BLOCK || TEAM == TEAM_WIDE || TEAM == TEAM_CLUSTER;   // the parameters stay in registers
+    constexpr bool kHeld = VEC ? TEAM != TEAM_WARP : G == 1;   // the parameters are kept
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) RowSlots<TEAM == TEAM_WARP ? 4 : kThreads / 32, TEAM == TEAM_CLUSTER ? kForwardCluster : 1> slots;
     __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<G, kThreads>];
     RowPlace p = row_place<VEC, G, TEAM>(a, shape, slots);
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
     const bool gate_each = BRANCH && a.gate_rows == 1, gate_f32 = sizeof(F) == 4 || a.gate_f32;
-    constexpr bool sure = kHeld;   // (a row in every turn)
+    constexpr bool sure = TEAM == TEAM_BLOCK || TEAM == TEAM_WIDE || TEAM == TEAM_CLUSTER;   // (a row in every turn)
     const int part_f = ring_bytes(VEC, shape, sizeof(X)), part_gate = part_f + (BRANCH ? ring_bytes(VEC, shape, sizeof(F)) : 0);
     constexpr int kF = G * kParts<X>, kGate = kF + (BRANCH ? G * kParts<F> : 0);
-    RowRing<VEC, G, TEAM> ring(dynamic + (kHeld ? held_bytes(shape) : 0), p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0), shape.stages);
+    RowRing<VEC, G, TEAM> ring(dynamic + held_bytes(VEC, shape), p, part_gate + (gate_each ? ring_bytes(VEC, shape, gate_f32 ? 4 : sizeof(F)) : 0), shape.stages);
     const X *const x_in = static_cast<const X *>(a.x);
     const F *const f_in = static_cast<const F *>(a.f);
     const int stride = gridDim.x / p.cluster;
@@ -1212,7 +1218,7 @@ int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs
 template <class X, class F>
 size_t join_rows_smem(bool backward, bool vec, const RowShape &s, bool gate_each) {
     const size_t x = ring_bytes(vec, s, sizeof(X)), f = ring_bytes(vec, s, sizeof(F)), gate = gate_each ? ring_bytes(vec, s, 4) : 0;
-    return (backward ? 2 * kBackwardParams * 16 * s.threads : vec ? held_bytes(s) : 0) + s.stages * ((backward ? 2 : 1) * (x + f) + gate + s.pad * (s.threads / 32));
+    return (backward ? 2 * kBackwardParams * 16 * s.threads : held_bytes(vec, s)) + s.stages * ((backward ? 2 : 1) * (x + f) + gate + s.pad * (s.threads / 32));
 }
 // Clusters of a kernel that are resident at a time, as the driver counts them; 0 where it cannot be asked.
 template <class X, class F>
@@ -1222,13 +1228,13 @@ const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
 #define LUTB_FORWARD(VEC, G, TEAM) reinterpret_cast<const void *>(&join_rows_forward_kernel<X, F, BRANCH, NEXT, VEC, G, TEAM>)
 #define LUTB_BACKWARD(VEC, TEAM) reinterpret_cast<const void *>(&join_rows_backward_kernel<X, F, BRANCH, NEXT, VEC, TEAM>)
     if (backward) {
-        if (!vec) return LUTB_BACKWARD(false, TEAM_ANY);
+        if (!vec) return s.kind == TEAM_WARP ? LUTB_BACKWARD(false, TEAM_WARP) : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(false, TEAM_BLOCK) : LUTB_BACKWARD(false, TEAM_ANY);
         return s.kind == TEAM_WARP    ? LUTB_BACKWARD(true, TEAM_WARP)
                : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(true, TEAM_BLOCK)
                : s.kind == TEAM_WIDE  ? LUTB_BACKWARD(true, TEAM_WIDE)
                                       : LUTB_BACKWARD(true, TEAM_CLUSTER);
     }
-    if (!vec) return s.groups == 1 ? LUTB_FORWARD(false, 1, TEAM_ANY) : LUTB_FORWARD(false, 4, TEAM_ANY);
+    if (!vec) return s.groups > 1 ? LUTB_FORWARD(false, 4, TEAM_WIDE) : s.kind == TEAM_WARP ? LUTB_FORWARD(false, 1, TEAM_WARP) : LUTB_FORWARD(false, 1, TEAM_BLOCK);
     if (s.kind == TEAM_WARP) return s.groups == 1 ? LUTB_FORWARD(true, 1, TEAM_WARP) : LUTB_FORWARD(true, 4, TEAM_WARP);
     return s.kind == TEAM_BLOCK ? LUTB_FORWARD(true, 2, TEAM_BLOCK) : s.kind == TEAM_WIDE ? LUTB_FORWARD(true, 2, TEAM_WIDE) : LUTB_FORWARD(true, 2, TEAM_CLUSTER);
 #undef LUTB_FORWARD
