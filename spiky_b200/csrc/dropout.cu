@@ -18,41 +18,58 @@ DropRule drop_rule(double p) {
     return r;
 }
 
-// A thread takes the eight elements of a generator block, two such blocks (VEC) side by side: their rounds are independent and share the
-// keys.  VEC: whole blocks in 16-byte aligned arrays; the others element by element.
+// A thread takes the eight elements of a generator block; VEC, whole blocks in aligned arrays: two such blocks of 4-byte elements side by side, four of
+// 2-byte ones, whose rounds are independent and share the keys; the others element by element.  Bound: 4-byte types by the memory (67 M
+// values 83 us, 6.4 TB/s, with a block for each 4096 of them; 92 us with the same threads on a grid of eight blocks an SM), 2-byte types by
+// the integer unit beside it, some 75 of its operations for eight elements (four side by side 57 us, two 61, one 67).
+constexpr int64_t kDropMost = 2048ll * INT32_MAX;   // (a grid has 2^31 - 1 blocks, of 2048 elements at least)
+
+template <class T>
+constexpr int kDropSide = sizeof(T) == 4 ? 2 : 4;
+
+// The elements of block b one by one, up to the last.
+template <class T>
+__device__ __forceinline__ void drop_apart(int64_t b, int64_t n, const T *x, T *y, uint32_t kept, float scale) {
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+        const int64_t i = 8 * b + j;
+        if (i < n) y[i] = from_f32<T>((kept >> j & 1) ? to_f32(x[i]) * scale : 0.0f);
+    }
+}
+
 template <class T, bool VEC>
-__global__ void __launch_bounds__(256) dropout_kernel(int64_t first, int64_t n, const T *x, T *y, const int64_t *random, uint64_t site, const DropRule rule) {
+__global__ void __launch_bounds__(256, 4) dropout_kernel(int64_t n, const T *x, T *y, const int64_t *random, uint64_t site, const DropRule rule) {
     const DropKey key = drop_key(random, site);
     if constexpr (VEC) {
-        constexpr int kSide = 2;
-        for (int64_t b = blockIdx.x * (256ll * kSide) + threadIdx.x; 8 * b < n; b += gridDim.x * (256ll * kSide)) {
-            uint4 in[kSide][kParts<T>];
+        constexpr int kSide = kDropSide<T>;
+        const int64_t first = blockIdx.x * (256ll * kSide) + threadIdx.x;
+        uint4 in[kSide][kParts<T>];
 #pragma unroll
-            for (int k = 0; k < kSide; k++)
+        for (int k = 0; k < kSide; k++) {
+            const int64_t b = first + 256 * k;
+            if (8 * b + 8 <= n) {
 #pragma unroll
-                for (int q = 0; q < kParts<T>; q++)
-                    if (8 * (b + 256 * k) < n) in[k][q] = reinterpret_cast<const uint4 *>(x + 8 * (b + 256 * k))[q];
-            DropDigits digits[kSide];
+                for (int q = 0; q < kParts<T>; q++) in[k][q] = reinterpret_cast<const uint4 *>(x + 8 * b)[q];
+            }
+        }
+        DropDigits digits[kSide];
 #pragma unroll
-            for (int k = 0; k < kSide; k++) digits[k] = drop_digits((uint64_t)(b + 256 * k), key, rule);
+        for (int k = 0; k < kSide; k++) digits[k] = drop_digits((uint64_t)(first + 256 * k), key, rule);
 #pragma unroll
-            for (int k = 0; k < kSide; k++) {
-                if (8 * (b + 256 * k) >= n) break;
+        for (int k = 0; k < kSide; k++) {
+            const int64_t b = first + 256 * k;
+            if (8 * b + 8 <= n) {
                 float2 v[4];
                 unpack8<T>(in[k], v);
                 drop8(v, digits[k], rule.scale);
-                store8(y + 8 * (b + 256 * k), v);
+                store8(y + 8 * b, v);
+            } else if (8 * b < n) {
+                drop_apart(b, n, x, y, bits_of(digits[k]), rule.scale);
             }
         }
     } else {
-        for (int64_t b = first / 8 + blockIdx.x * 256ll + threadIdx.x; 8 * b < n; b += gridDim.x * 256ll) {
-            const uint32_t kept = keep_bits((uint64_t)b, key, rule);
-#pragma unroll
-            for (int j = 0; j < 8; j++) {
-                const int64_t i = 8 * b + j;
-                if (i < n) y[i] = from_f32<T>((kept >> j & 1) ? to_f32(x[i]) * rule.scale : 0.0f);
-            }
-        }
+        const int64_t b = blockIdx.x * 256ll + threadIdx.x;
+        if (8 * b < n) drop_apart(b, n, x, y, keep_bits((uint64_t)b, key, rule), rule.scale);
     }
 }
 
@@ -68,19 +85,13 @@ static int launch_dropout(int64_t n, const void *x, void *y, const int64_t *rand
     const T *from = static_cast<const T *>(x);
     T *to = static_cast<T *>(y);
     const bool vec = reinterpret_cast<uintptr_t>(x) % 16 == 0 && reinterpret_cast<uintptr_t>(y) % 32 == 0;
-    const int64_t whole = vec ? n / 8 * 8 : 0, cap = (int64_t)device_info().sm_count * 8;
-    if (whole) {
-        const int64_t blocks = (whole / 8 + 511) / 512;
-        KernelScope scope(K_DROPOUT, stream);
-        dropout_kernel<T, true><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, stream>>>(0, whole, from, to, random, site, rule);
-        LUTB_LAUNCH_CHECK();
-    }
-    if (whole < n) {
-        const int64_t blocks = ((n - whole + 7) / 8 + 255) / 256;
-        KernelScope scope(K_DROPOUT, stream);
-        dropout_kernel<T, false><<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, stream>>>(whole, n, from, to, random, site, rule);
-        LUTB_LAUNCH_CHECK();
-    }
+    const int64_t each = 2048 * (vec ? kDropSide<T> : 1), blocks = (n + each - 1) / each;
+    KernelScope scope(K_DROPOUT, stream);
+    if (vec)
+        dropout_kernel<T, true><<<(unsigned)blocks, 256, 0, stream>>>(n, from, to, random, site, rule);
+    else
+        dropout_kernel<T, false><<<(unsigned)blocks, 256, 0, stream>>>(n, from, to, random, site, rule);
+    LUTB_LAUNCH_CHECK();
     return LUTB_OK;
 }
 
@@ -89,7 +100,7 @@ static int launch_dropout(int64_t n, const void *x, void *y, const int64_t *rand
 extern "C" int lutb_dropout(int type, int64_t n, double p, const int64_t *random, int64_t site, const void *x, void *y, void *stream) {
     using namespace lutb;
     LUTB_REQUIRE(type == LUTB_F32 || type == LUTB_BF16 || type == LUTB_F16, LUTB_ERR_MODE, "unknown element type %d", type);
-    LUTB_REQUIRE(n >= 0, LUTB_ERR_SHAPE, "number of elements < 0");
+    LUTB_REQUIRE(n >= 0 && n <= kDropMost, LUTB_ERR_SHAPE, "number of elements must be between 0 and %lld", (long long)kDropMost);
     LUTB_REQUIRE(p >= 0.0 && p <= 1.0, LUTB_ERR_SHAPE, "dropout probability must be between 0 and 1");
     LUTB_REQUIRE(site >= 0, LUTB_ERR_SHAPE, "site < 0");
     if (n == 0) return LUTB_OK;

@@ -81,12 +81,13 @@ __device__ __forceinline__ DropDigits drop_digits(uint64_t block, const DropKey 
     }
     return d;
 }
-__device__ __forceinline__ uint32_t keep_bits(uint64_t block, const DropKey &key, const DropRule &rule) {
-    const DropDigits d = drop_digits(block, key, rule);
+// Which of the eight stay, as bits.
+__device__ __forceinline__ uint32_t bits_of(const DropDigits &d) {
     uint32_t kept = 0;
 #pragma unroll
     for (int k = 0; k < 4; k++) kept |= ((d.w[k] << 16) > d.above ? 1u : 0u) << (2 * k) | (d.w[k] > d.above ? 2u : 0u) << (2 * k);
     return kept;
 }
+__device__ __forceinline__ uint32_t keep_bits(uint64_t block, const DropKey &key, const DropRule &rule) { return bits_of(drop_digits(block, key, rule)); }
 
 }  // namespace lutb

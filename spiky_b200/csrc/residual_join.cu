@@ -215,34 +215,48 @@ __global__ void __launch_bounds__(1024) join_sums_kernel(const SumList l, int64_
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5, k = min((int)blockIdx.y, l.count);
     const int64_t first = (int64_t)blockIdx.x * (32 * V), c = first + lane * V, out_row = (int)blockIdx.y - k;
     const float *from = l.from[k] + out_row * l.parts[k] * width + c;
-    constexpr int kAhead = 4;   // loads on their way
-    float s[kAhead][V];
+    constexpr int kAhead = 8;   // loads on their way
+    float s[V];
 #pragma unroll
-    for (int a = 0; a < kAhead; a++)
-#pragma unroll
-        for (int e = 0; e < V; e++) s[a][e] = 0.0f;
-    if (c < width)
-        for (int64_t p = warp; p < l.parts[k]; p += kAhead * warps)
-#pragma unroll
-            for (int a = 0; a < kAhead; a++) {
-                if (p + a * warps >= l.parts[k]) break;
-                if constexpr (V == 4) {
-                    const float4 v = *reinterpret_cast<const float4 *>(from + (p + a * warps) * width);
-                    s[a][0] += v.x;
-                    s[a][1] += v.y;
-                    s[a][2] += v.z;
-                    s[a][3] += v.w;
-                } else {
-                    s[a][0] += from[(p + a * warps) * width];
-                }
+    for (int e = 0; e < V; e++) s[e] = 0.0f;
+    if (c < width) {
+        const int64_t parts = l.parts[k], step = (int64_t)warps * width;
+        int64_t p = warp;
+        auto load = [&](int64_t at, float *v) {
+            if constexpr (V == 4) {
+                const float4 q = __ldcs(reinterpret_cast<const float4 *>(from + at));
+                v[0] = q.x;
+                v[1] = q.y;
+                v[2] = q.z;
+                v[3] = q.w;
+            } else {
+                v[0] = __ldcs(from + at);
             }
+        };
+        for (; p + (kAhead - 1) * warps < parts; p += kAhead * warps) {
+            float v[kAhead][V];
 #pragma unroll
-    for (int e = 0; e < V; e++) all[warp][lane * V + e] = (s[0][e] + s[1][e]) + (s[2][e] + s[3][e]);
+            for (int a = 0; a < kAhead; a++) load(p * width + a * step, v[a]);
+#pragma unroll
+            for (int a = 0; a < kAhead; a++)
+#pragma unroll
+                for (int e = 0; e < V; e++) s[e] += v[a][e];
+        }
+        for (; p < parts; p += warps) {
+            float v[V];
+            load(p * width, v);
+#pragma unroll
+            for (int e = 0; e < V; e++) s[e] += v[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) all[warp][lane * V + e] = s[e];
     __syncthreads();
-    for (int at = threadIdx.x; at < 32 * V; at += blockDim.x) {
-        float sum = 0.0f;
-        for (int w = 0; w < warps; w++) sum += all[w][at];
-        if (first + at < width) {
+    for (int at = warp; at < 32 * V; at += warps) {   // a warp a column
+        float sum = lane < warps ? all[lane][at] : 0.0f;
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        if (lane == 0 && first + at < width) {
             if (l.f32[k])
                 static_cast<float *>(l.to[k])[out_row * width + first + at] = sum;
             else
