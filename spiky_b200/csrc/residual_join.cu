@@ -336,7 +336,7 @@ int resident_clusters(const void *kernel, const RowShape &s, size_t smem) {
 
 // Gives the shape its stages (the most of three with which as many threads as registers allow are resident, 512 an SM or, forward, 384; two or one
 // otherwise) and returns how many teams of blocks the device holds: a cluster beyond those would run in a second round.
-static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, RowShape &s) {
+static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, bool alone, RowShape &s) {
     const DeviceInfo info = device_info();
     const int sm = info.sm_count > 0 ? info.sm_count : 148;   // (no device: a size can be asked for all the same)
     const size_t own = backward ? (s.kind == TEAM_WARP ? kBackwardStatic : kBackwardTeamStatic) : vec ? kForwardVecStatic : kForwardStatic;
@@ -344,7 +344,7 @@ static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, RowSh
     int blocks = 1;
     size_t dynamic = 0;
     for (s.stages = 3; s.stages >= 1; s.stages--) {
-        dynamic = by_types(cfg, [&](auto xt, auto ft) { return join_rows_smem<decltype(xt), decltype(ft)>(backward, vec, s, cfg->gate_rows == 1); });
+        dynamic = by_types(cfg, [&](auto xt, auto ft) { return join_rows_smem<decltype(xt), decltype(ft)>(backward, vec, s, alone, cfg->gate_rows == 1); });
         blocks = dynamic > kMaxSmemPerBlock - kBackwardStatic ? 0 : (int)(kMaxSmemPerBlock / (dynamic + own));
         if (blocks >= wanted || (s.stages == 2 && blocks >= 1) || s.stages == 1) break;
     }
@@ -365,19 +365,19 @@ static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, RowSh
 static bool row_kernels(const lutb_join_cfg *cfg) { return cfg->width <= kRowMaxWidth && cfg->rows <= kRowMaxRows; }
 
 // How the rows are dealt, and to what shape of block (unless rows are too wide or too many for the row kernels).
-static JoinSplit split_forward(const lutb_join_cfg *cfg, bool vec, RowShape &s) {
+static JoinSplit split_forward(const lutb_join_cfg *cfg, bool vec, bool alone, RowShape &s) {
     const int have = device_info().sm_count;
     if (!row_kernels(cfg)) return join_split(cfg->rows, cfg->rows, (have > 0 ? have : 148) * 8ll, 1);
     s = forward_shape(cfg->width, vec);
-    const int64_t blocks = resident(cfg, false, vec, s);
+    const int64_t blocks = resident(cfg, false, vec, alone, s);
     return join_split(cfg->rows, cfg->rows, blocks, s.teams);
 }
-static JoinSplit split_backward(const lutb_join_cfg *cfg, bool gate_gradient, bool vec, RowShape &s) {
+static JoinSplit split_backward(const lutb_join_cfg *cfg, bool gate_gradient, bool vec, bool alone, RowShape &s) {
     const int64_t group_rows = gate_gradient && cfg->gate_rows > 1 ? cfg->gate_rows : cfg->rows;
     const int have = device_info().sm_count;
     if (!row_kernels(cfg)) return join_split(cfg->rows, group_rows, (have > 0 ? have : 148) * 4ll, 1);
     s = backward_shape(cfg->width);
-    const int64_t blocks = resident(cfg, true, vec, s);
+    const int64_t blocks = resident(cfg, true, vec, alone, s);
     return join_split(cfg->rows, group_rows, blocks, s.teams);
 }
 static void take_split(JoinArgs &a, const JoinSplit &s) {
@@ -499,7 +499,7 @@ extern "C" int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const 
     a.h = h; a.y = y; a.stats = reinterpret_cast<float4 *>(stats); a.random = random; a.gate_rows = cfg->gate_rows;
     const bool vec = cfg->width % kRowElems == 0 && all_aligned(16, {x, f, gate, after_weight, after_bias, before_weight, before_bias}) && all_aligned(32, {h, y});
     RowShape shape{};
-    const JoinSplit split = split_forward(cfg, vec, shape);
+    const JoinSplit split = split_forward(cfg, vec, f == nullptr, shape);
     take_split(a, split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return by_types(cfg, [&](auto xt, auto ft) -> int {
@@ -516,9 +516,10 @@ extern "C" size_t lutb_join_backward_workspace(const lutb_join_cfg *cfg) {
     if (check_join(cfg) || cfg->rows == 0) return 0;
     size_t floats = 0;
     for (int vec = 0; vec < 2; vec++)
-        for (int gated = 0; gated < 2; gated++) {
+        for (int kind = 0; kind < 3; kind++) {   // a join, one whose gate has a gradient, a norm alone
             RowShape shape{};
-            const JoinSplit split = split_backward(cfg, gated != 0, vec != 0, shape);
+            const bool gated = kind == 1;
+            const JoinSplit split = split_backward(cfg, gated, vec != 0, kind == 2, shape);
             const size_t need = (size_t)(4 * split.blocks + (gated && cfg->gate_rows > 1 ? split.chunks : 0)) * cfg->width;
             floats = need > floats ? need : floats;
         }
@@ -563,7 +564,7 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     const bool vec = cfg->width % kRowElems == 0 &&
                      all_aligned(16, {x, f, gate, after_weight, after_bias, before_weight, dh, dy}) && all_aligned(32, {dx, df, dgate});
     RowShape shape{};
-    const JoinSplit split = split_backward(cfg, dgate != nullptr, vec, shape);
+    const JoinSplit split = split_backward(cfg, dgate != nullptr, vec, f == nullptr, shape);
     take_split(a, split);
     a.gate_direct = gate_summed && split.per_group == 1;
     const bool gate_parts = gate_summed && !(a.gate_direct && row_kernels(cfg));   // (the kernel for wide rows sums there in any case)

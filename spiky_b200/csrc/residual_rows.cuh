@@ -1214,11 +1214,12 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
 int resident_clusters(const void *kernel, const RowShape &s, size_t smem);
 int launch_rows(const void *kernel, std::atomic<uint32_t> &opted, const JoinArgs &a, const RowShape &s, int clusters, size_t smem, cudaStream_t stream);
 
-// Shared memory of a block besides the kernel's own arrays, for any join of these types.
+// Shared memory of a block besides the kernel's own arrays, for any join of these types, or for a norm alone.
 template <class X, class F>
-size_t join_rows_smem(bool backward, bool vec, const RowShape &s, bool gate_each) {
+size_t join_rows_smem(bool backward, bool vec, const RowShape &s, bool alone, bool gate_each) {
     const size_t x = ring_bytes(vec, s, sizeof(X)), f = ring_bytes(vec, s, sizeof(F)), gate = gate_each ? ring_bytes(vec, s, 4) : 0;
-    return (backward ? 2 * kBackwardParams * 16 * s.threads : held_bytes(vec, s)) + s.stages * ((backward ? 2 : 1) * (x + f) + gate + s.pad * (s.threads / 32));
+    const size_t arrays = alone ? (backward ? 2 * x + f : x) : (backward ? 2 : 1) * (x + f) + gate;   // (a place for dh is kept in any case)
+    return (backward ? 2 * kBackwardParams * 16 * s.threads : held_bytes(vec, s)) + s.stages * (arrays + s.pad * (s.threads / 32));
 }
 // Clusters of a kernel that are resident at a time, as the driver counts them; 0 where it cannot be asked.
 template <class X, class F>
@@ -1251,7 +1252,7 @@ int launch_join_rows(bool backward, bool vec, const JoinArgs &a, const RowShape 
                          : kind == 5 ? join_rows_kernel<X, F, 2, true>(backward, vec, s)
                                      : nullptr;
     LUTB_REQUIRE(kernel != nullptr, LUTB_ERR_MODE, "nothing to compute");
-    const size_t smem = join_rows_smem<X, F>(backward, vec, s, a.f != nullptr && a.gate_rows == 1);
+    const size_t smem = join_rows_smem<X, F>(backward, vec, s, a.f == nullptr, a.gate_rows == 1);
     return launch_rows(kernel, opted[backward][vec][kind][backward ? s.kind : 2 * s.kind + (s.groups > 1)], a, s, clusters, smem, stream);
 }
 
