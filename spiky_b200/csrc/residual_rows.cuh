@@ -1074,7 +1074,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             if (a.drop.on) drop8(t, kept, a.drop.scale);
             if (BRANCH == 2)
 #pragma unroll
-                for (int k = 0; k < 4; k++) t[k] = mul2(add2(t[k], both(-st.x)), both(st.y));
+                for (int k = 0; k < 4; k++) t[k] = fma2(t[k], both(st.y), both(-st.x * st.y));
         }
         auto branch_out = [&](float2 *n) {   // the branch after its norm
             if (BRANCH == 2) {
@@ -1104,7 +1104,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             param(2, u);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                z[k] = mul2(add2(z[k], both(-st.z)), both(st.w));
+                z[k] = fma2(z[k], both(st.w), both(-st.z * st.w));
                 u[k] = mul2(g[k], u[k]);
                 s1 = fma2(u[k], z[k], s1);
             }
@@ -1112,10 +1112,10 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             const float2 c = row_sums<TEAM>(p, slots, some ? s1.x + s1.y : 0.0f, layer && some ? total(u) : 0.0f, layer, [&]() {
                 if (!on) return;
 #pragma unroll
-                for (int k = 0; k < 4; k++) {
-                    sums[2][k] = fma2(g[k], z[k], sums[2][k]);
-                    sums[3][k] = add2(sums[3][k], g[k]);
-                }
+                for (int k = 0; k < 4; k++) sums[2][k] = fma2(g[k], z[k], sums[2][k]);
+                if (a.sums[3])
+#pragma unroll
+                    for (int k = 0; k < 4; k++) sums[3][k] = add2(sums[3][k], g[k]);
             });
             const float c1 = -c.x * p.inverse, c2 = layer ? -c.y * p.inverse : 0.0f;
             if (dh_in)
@@ -1123,7 +1123,12 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             else
                 zero8(d);
 #pragma unroll
-            for (int k = 0; k < 4; k++) d[k] = fma2(both(st.w), fma2(z[k], both(c1), add2(u[k], both(c2))), d[k]);
+            for (int k = 0; k < 4; k++) z[k] = fma2(z[k], both(c1), u[k]);
+            if (layer)
+#pragma unroll
+                for (int k = 0; k < 4; k++) z[k] = add2(z[k], both(c2));
+#pragma unroll
+            for (int k = 0; k < 4; k++) d[k] = fma2(both(st.w), z[k], d[k]);
         } else {
             ring.template get<X, kDh>(p, shape, 0, part_dh, dh_in, at, on, d);
         }
@@ -1158,12 +1163,13 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             if (BRANCH == 2) {
                 float2 s1 = make_float2(0.0f, 0.0f), w[4];
                 param(0, w);
-                if (on)
+                if (on) {
 #pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        sums[0][k] = fma2(d[k], t[k], sums[0][k]);
-                        sums[1][k] = add2(sums[1][k], d[k]);
-                    }
+                    for (int k = 0; k < 4; k++) sums[0][k] = fma2(d[k], t[k], sums[0][k]);
+                    if (a.sums[1])
+#pragma unroll
+                        for (int k = 0; k < 4; k++) sums[1][k] = add2(sums[1][k], d[k]);
+                }
 #pragma unroll
                 for (int k = 0; k < 4; k++) {
                     d[k] = mul2(d[k], w[k]);
@@ -1177,7 +1183,12 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
                 const float2 c = row_sums<TEAM>(p, slots, some ? s1.x + s1.y : 0.0f, layer && some ? total(d) : 0.0f, layer, []() {});
                 const float c1 = -c.x * p.inverse, c2 = layer ? -c.y * p.inverse : 0.0f;
 #pragma unroll
-                for (int k = 0; k < 4; k++) d[k] = mul2(both(st.y), fma2(t[k], both(c1), add2(d[k], both(c2))));
+                for (int k = 0; k < 4; k++) d[k] = fma2(t[k], both(c1), d[k]);
+                if (layer)
+#pragma unroll
+                    for (int k = 0; k < 4; k++) d[k] = add2(d[k], both(c2));
+#pragma unroll
+                for (int k = 0; k < 4; k++) d[k] = mul2(d[k], both(st.y));
             }
             if (a.df && on) {
                 if (a.drop.on) drop8(d, kept, a.drop.scale);
