@@ -108,6 +108,12 @@ struct ResidualNode : public torch::autograd::Node {
     }
 };
 
+// What a backward pass is handed can come from hooks: the kernels get nothing that is not what the forward pass had.
+void expect(const Tensor &t, at::ScalarType type, int64_t numel, c10::DeviceIndex device, const char *name) {
+    TORCH_CHECK(plain_cuda(t, type, device) && t.numel() == numel, name, " is not what the forward pass saved: ", numel, " elements of ", type, " on cuda:", (int)device);
+}
+at::ScalarType scalar_type_of(int type) { return type == LUTB_F32 ? at::kFloat : type == LUTB_BF16 ? at::kBFloat16 : at::kHalf; }
+
 // ------------------------------------------------------------------------------------------------ dropout
 Tensor dropout(const Tensor &x, double p, const Tensor &state, int64_t site);
 
@@ -118,6 +124,9 @@ struct DropoutNode : public ResidualNode {
     variable_list apply(variable_list &&grads) override {
         const std::vector<Tensor> s = unpack();
         if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
+        expect(grads[0], grads[0].scalar_type(), grads[0].numel(), grads[0].device().index(), "the gradient");
+        expect(s[0], at::kLong, 2, grads[0].device().index(), "state");
+        TORCH_CHECK(type_of(grads[0].scalar_type()) >= 0 && s[0].is_contiguous(), "the gradient or state is not what the forward pass had");
         return {dropout(grads[0], p, s[0], site)};   // (with a graph of its own where one is asked for)
     }
 };
@@ -187,7 +196,8 @@ enum { X, F, GATE, AW, AB, BW, BB, TENSORS };
 
 struct JoinNode : public ResidualNode {
     lutb_join_cfg cfg;
-    bool has_h = false;
+    bool has_h = false, had[TENSORS] = {};
+    c10::DeviceIndex device = 0;
     std::string name() const override { return "_ResidualJoinBackward"; }
     variable_list apply(variable_list &&grads) override {
         std::vector<Tensor> s = unpack();   // the seven tensors, state, stats
@@ -195,9 +205,21 @@ struct JoinNode : public ResidualNode {
         variable_list out(TENSORS);
         if (!dh.defined() && !dy.defined()) return out;
         const bool again = needs_graph({&dh, &dy});
+        const int64_t all = cfg.rows * cfg.width;
+        const int types[TENSORS] = {cfg.stream_type, cfg.branch_type, cfg.gate_type, cfg.param_type, cfg.param_type, cfg.param_type, cfg.param_type};
+        static const char *const what[TENSORS] = {"x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "next_bias"};
+        for (int k = 0; k < TENSORS; k++)
+            if (had[k]) expect(s[k], scalar_type_of(types[k]), k <= F ? all : k == GATE ? all / cfg.gate_rows : cfg.width, device, what[k]);
+        if (cfg.dropout > 0.0) {
+            expect(s[TENSORS], at::kLong, 2, device, "state");
+            s[TENSORS] = s[TENSORS].contiguous();
+        }
+        expect(s[TENSORS + 1], at::kFloat, 4 * cfg.rows, device, "stats");
+        s[TENSORS + 1] = s[TENSORS + 1].contiguous();
+        if (dh.defined()) expect(dh, scalar_type_of(cfg.stream_type), all, device, "the gradient");
+        if (dy.defined()) expect(dy, scalar_type_of(cfg.branch_type), all, device, "the gradient");
         {
             at::AutoDispatchBelowADInplaceOrView below;
-            const c10::DeviceIndex device = s[X].device().index();
             c10::cuda::CUDAGuard guard(device);
             for (int k = 0; k < TENSORS; k++)
                 if (s[k].defined() && task_should_compute_output(k) && (k < BW || dy.defined())) out[k] = new_like(s[k], s[k].scalar_type());
@@ -310,7 +332,7 @@ PyObject *join_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
         for (int k = 0; k < TENSORS; k++) c[k] = whole(t[k]);
         if (t[F].defined()) h = new_like(x, x.scalar_type());
         if (cfg.before != LUTB_NORM_NONE)
-            y = new_like(x, cfg.branch_type == LUTB_F32 ? at::kFloat : cfg.branch_type == LUTB_BF16 ? at::kBFloat16 : at::kHalf);
+            y = new_like(x, scalar_type_of(cfg.branch_type));
         if (graph) stats = at::empty({cfg.rows, 4}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
         check(lib.join_forward(&cfg, pointer(c[X]), pointer(c[F]), pointer(c[GATE]), pointer(c[AW]), pointer(c[AB]), pointer(c[BW]), pointer(c[BB]),
                                random_of(state), pointer(h), pointer(y), static_cast<float *>(pointer(stats)), stream_on(x.device().index())));
@@ -319,6 +341,8 @@ PyObject *join_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
         auto node = std::shared_ptr<JoinNode>(new JoinNode(), torch::autograd::deleteNode);
         node->cfg = cfg;
         node->has_h = h.defined();
+        node->device = t[X].device().index();
+        for (int k = 0; k < TENSORS; k++) node->had[k] = t[k].defined();
         node->set_next_edges(torch::autograd::collect_next_edges(t[X], t[F], t[GATE], t[AW], t[AB], t[BW], t[BB]));
         for (const Tensor &v : t) node->saved.emplace_back(v, false);
         node->saved.emplace_back(state, false);

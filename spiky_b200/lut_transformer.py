@@ -21,6 +21,9 @@ from .residual import ResidualJoin, RowNorm, counter_dropout as _counter_dropout
 
 
 class LUTTransformer(nn.Module):
+    # (of models that were pickled before these options)
+    norm, counter_dropout, _joined = None, False, False
+
     def __init__(self, vocab_size, embedding_dim, context_size, positional_dim, num_layers, num_heads, n_detectors,
                  n_anchors_per_detector, n_anchors_per_detector_attention=None, no_ffn=False,
                  concatenation_product=True, sliced_product_mode=False, unified_pe=False, do_normalise_weights=False,
@@ -166,11 +169,9 @@ class LUTTransformer(nn.Module):
                 layer.to(device=dev)
         return self
 
-    def _residual_branch(self, z, out, dropout, bn, state, site):
-        if not self.counter_dropout:
-            out = dropout(out)
-        elif state is not None:
-            out = _counter_dropout(out, self.dropout, state, site)
+    @staticmethod
+    def _residual_branch(z, out, dropout, bn):
+        out = dropout(out)
         if bn is not None:
             out = bn(out.reshape(-1, out.shape[-1])).reshape(out.shape)
         return z + out
@@ -178,7 +179,11 @@ class LUTTransformer(nn.Module):
     def _add(self, z, out, block, part, state, site):
         """The stream with a block's output, and what the next block reads of it."""
         if not self._joined:
-            z = self._residual_branch(z, out, block[part + "_dropout"], block[part + "_bn"], state, site)
+            dropout = block[part + "_dropout"]
+            if self.counter_dropout:
+                def dropout(o):
+                    return o if state is None else _counter_dropout(o, self.dropout, state, site)
+            z = self._residual_branch(z, out, dropout, block[part + "_bn"])
             return z, z
         if not self.counter_dropout:
             out = block[part + "_dropout"](out)

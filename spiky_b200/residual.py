@@ -111,8 +111,21 @@ def take_dropout_state(state, count):
     return used
 
 
+def _whole(t):
+    """As the kernels read it: contiguous, no lazy negation."""
+    return None if t is None else t.detach().resolve_neg().contiguous()
+
+
+def _expect(t, like, numel, name):
+    """What a backward pass is handed can come from hooks: the kernels get nothing that is not what the forward pass had."""
+    dtype, device = like
+    if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.numel() != numel or t.layout != torch.strided:
+        raise RuntimeError(f"{name} is not what the forward pass saved: {numel} elements of {dtype} on {device}")
+    return _whole(t)
+
+
 def _dropout(x, p, state, site):
-    x = x.detach().contiguous()
+    x = _whole(x)
     y = torch.empty_like(x)
     with torch.cuda.device(x.device):
         _native.check(_native.lib().lutb_dropout(_TYPES[x.dtype], x.numel(), p, _ptr(state), site, _ptr(x), _ptr(y), _stream(x.device)))
@@ -129,6 +142,7 @@ class _CounterDropout(torch.autograd.Function):
     @staticmethod
     def backward(ctx, dy):
         state, = ctx.saved_tensors
+        _expect(state, (torch.int64, dy.device), 2, "state")
         return counter_dropout(dy, ctx.p, state, ctx.site), None, None, None
 
 
@@ -181,6 +195,8 @@ class _Join(torch.autograd.Function):
     def forward(ctx, cfg, x, branch, gate, aw, ab, bw, bb, state, stats):
         h, y = _join_forward(cfg, x, branch, gate, aw, ab, bw, bb, state, stats)
         ctx.cfg = cfg
+        ctx.had = [None if t is None else ((t.dtype, t.device), t.numel()) for t in (x, branch, gate, aw, ab, bw, bb, state, stats)]
+        ctx.of_grads = [None if t is None else (t.dtype, t.device) for t in (h, y)]
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, branch, gate, aw, ab, bw, bb, state, stats)
         return h, y
@@ -188,10 +204,14 @@ class _Join(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dy):
-        x, branch, gate, aw, ab, bw, bb, state, stats = ctx.saved_tensors
         if dh is None and dy is None:
             return (None,) * 10
         cfg, need = ctx.cfg, ctx.needs_input_grad
+        saved = ctx.saved_tensors
+        names = ("x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "next_bias", "state", "stats")
+        con = [None if had is None else _expect(t, *had, name) for t, had, name in zip(saved, ctx.had, names)]
+        dh, dy = (None if t is None else _expect(t, like, ctx.had[0][1], "the gradient") for t, like in zip((dh, dy), ctx.of_grads))
+        x, branch, gate, aw, ab, bw, bb = saved[:7]
 
         def like(t, wanted):
             return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted and t is not None else None
@@ -199,7 +219,6 @@ class _Join(torch.autograd.Function):
         dx, df, dgate = like(x, need[1]), like(branch, need[2]), like(gate, need[3])
         daw, dab = like(aw, need[4]), like(ab, need[5])
         dbw, dbb = (like(bw, need[6]), like(bb, need[7])) if dy is not None else (None, None)
-        con = [None if t is None else t.contiguous() for t in (x, branch, gate, aw, ab, bw, dh, dy)]
         with torch.cuda.device(x.device):
             L = _native.lib()
             ws, size = None, 0
@@ -207,13 +226,13 @@ class _Join(torch.autograd.Function):
                 size = L.lutb_join_backward_workspace(ctypes.byref(cfg))
                 ws = torch.empty(size, dtype=torch.uint8, device=x.device)
             _native.check(L.lutb_join_backward(
-                ctypes.byref(cfg), *(_ptr(t) for t in con[:6]), _ptr(state), _ptr(stats), _ptr(con[6]), _ptr(con[7]), _ptr(dx), _ptr(df),
+                ctypes.byref(cfg), *(_ptr(t) for t in con[:6]), _ptr(con[7]), _ptr(con[8]), _ptr(dh), _ptr(dy), _ptr(dx), _ptr(df),
                 _ptr(dgate), _ptr(daw), _ptr(dab), _ptr(dbw), _ptr(dbb), _ptr(ws), size, _stream(x.device)))
         return None, dx, df, dgate, daw, dab, dbw, dbb, None, None
 
 
 def _join_forward(cfg, x, branch, gate, aw, ab, bw, bb, state, stats):
-    con = [None if t is None else t.detach().contiguous() for t in (x, branch, gate, aw, ab, bw, bb)]
+    con = [_whole(t) for t in (x, branch, gate, aw, ab, bw, bb)]
     branch_type = [k for k, v in _TYPES.items() if v == cfg.branch_type][0]
     h = None if branch is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
     y = torch.empty(x.shape, dtype=branch_type, device=x.device) if cfg.before != _native.NORM_NONE else None

@@ -6,6 +6,7 @@ import weakref
 import pytest
 import torch
 
+import residual_oracle as ro
 import test_residual_gpu as plain
 
 pytestmark = pytest.mark.gpu
@@ -137,6 +138,41 @@ def test_contexts(routes):
 
     a, b = routes(contexts)
     assert a.shape == b.shape
+
+
+def test_what_hooks_hand_back_is_checked(routes):
+    """A saved tensor that comes back on another device, of another type or size is an error, not an address for a kernel."""
+    from spiky_b200 import residual
+
+    def hooked():
+        x, f = torch.randn(3, 16, device=DEV, requires_grad=True), torch.randn(3, 16, device=DEV)
+        state = residual.dropout_state(1, DEV)
+        for unpack in (lambda t: t, lambda t: t.to(DEV).double(), lambda t: t.to(DEV).reshape(-1)[:1]):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), unpack):
+                h = residual.residual_join(x, f, branch_norm="rms")
+                y = residual.counter_dropout(x, 0.5, state)
+            for out in (h, y):
+                with pytest.raises(RuntimeError, match="forward pass"):
+                    torch.autograd.grad(out.sum(), x)
+
+    routes(hooked)
+
+
+def test_lazily_negated_tensors(routes):
+    from spiky_b200 import residual
+
+    def negated():
+        x = torch.randn(3, 16, device=DEV)
+        n = torch._neg_view(x)
+        state = residual.dropout_state(1, DEV)
+        assert torch.equal(residual.residual_join(n, n), -2 * x)
+        assert torch.equal(residual.counter_dropout(n, 0.5, state), -residual.counter_dropout(x, 0.5, state))
+        w = torch.ones(16, device=DEV, requires_grad=True)
+        y = residual.row_norm(n, w)
+        g, = torch.autograd.grad(y, w, torch._neg_view(torch.ones_like(y)))
+        ro.assert_near(g, residual.row_norm(x).sum(0).cpu().double(), torch.full((16,), 10.0, dtype=torch.float64), "dw")
+
+    routes(negated)
 
 
 def test_graphs_are_freed(routes):

@@ -393,6 +393,21 @@ def test_join_beyond_32_bits():
     assert torch.equal(dx[some], dx2)
 
 
+def test_more_rows_than_32_bit_numbers_of_the_row_kernels():
+    r, rows = lib(), 2 ** 30 + 3
+    x = torch.empty(rows, 1, dtype=torch.float16, device=DEV).normal_()
+    h = r.residual_join(x, x, branch_scale=0.5)
+    for part in (slice(0, 1000), slice(rows - 1000, rows)):
+        ro.assert_near(h[part], 1.5 * x[part].cpu().double(), 1.5 * x[part].cpu().double().abs(), "h")
+
+
+def test_no_wait_of_a_cluster_ran_out():
+    from spiky_b200 import _native
+
+    run_join(torch.float32, torch.float32, (300,), 16384, "layer", "layer", gate="width", p=0.1, seed=1)
+    assert _native.device_wait_errors() == 0
+
+
 def test_side_stream_and_graph():
     """A training pass on a stream of its own, captured and replayed: each replay moves the dropout on and uses new inputs."""
     r = lib()

@@ -75,6 +75,23 @@ def test_joins_of_a_model(opts):
         assert m.first_norm.weight.grad.isfinite().all()
 
 
+def test_norms_with_stored_masks():
+    """Norms beside torch's own dropout: the modules are called, and evaluation draws nothing."""
+    m = model(norm="rms", dropout=0.3).train()
+    assert not torch.equal(m(tokens()), m(tokens()))
+    m(tokens()).sum().backward()
+    assert all(p.grad.isfinite().all() for n, p in m.named_parameters() if "_join" in n or "first_norm" in n)
+    m.eval()
+    assert torch.equal(m(tokens()), m(tokens()))
+
+
+def test_models_pickled_before_the_options():
+    m = model().eval()
+    for name in ("norm", "norm_after", "gated", "counter_dropout", "_joined", "_n_dropouts"):
+        del m.__dict__[name]
+    assert torch.equal(m(tokens()), m(tokens()))
+
+
 def test_plain_model_is_what_it_was():
     """Without options the sum is torch's, no buffer and no parameter is added; counter dropout in evaluation mode changes nothing."""
     plain, counted = model(dropout=0.5), model(dropout=0.5, counter_dropout=True)
