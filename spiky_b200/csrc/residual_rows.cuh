@@ -343,6 +343,13 @@ __device__ __forceinline__ void collect(RowPlace &p, Slots &slots) {
         }
     }
 }
+// Sums over each N neighbouring lanes, in all of them.
+template <int N>
+__device__ __forceinline__ float lane_sums(float v) {
+#pragma unroll
+    for (int o = N / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
 // The sum of a set of slots, always in the same order.
 template <int N>
 __device__ __forceinline__ float slot_sum(const float *from) {
@@ -380,10 +387,11 @@ __device__ __forceinline__ float2 row_sums(RowPlace &p, Slots &slots, float a, f
     between();
     collect<TEAM>(p, slots);
     const float *const sa = slots.a[p.turn & 1], *const sb = slots.b[p.turn & 1];
+    constexpr int kWarps = Slots::kWarps;
+    const int lane = threadIdx.x & 31;
     p.turn++;
     if (over_cluster<TEAM>(p) && second) {   // the slots' values over the lanes, then as before
-        constexpr int kWarps = Slots::kWarps;
-        const int lane = threadIdx.x & 31, n = p.cluster * kWarps;   // 16, 32 or 64 slots, one or two a lane
+        const int n = p.cluster * kWarps;    // 16, 32 or 64 slots, one or two a lane
         a = lane < n ? sa[lane] : 0.0f;
         b = lane < n ? sb[lane] : 0.0f;
         if (n > 32) {
@@ -392,6 +400,10 @@ __device__ __forceinline__ float2 row_sums(RowPlace &p, Slots &slots, float a, f
         }
         warp_sums(a, b);
         return make_float2(a, b);
+    }
+    if (!over_cluster<TEAM>(p) && second) {   // a slot a lane: the first values, then the second ones
+        const float v = lane_sums<kWarps>((lane & kWarps ? sb : sa)[lane & (kWarps - 1)]);
+        return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, kWarps));
     }
     return make_float2(all_slots<TEAM, Slots>(p, sa), second ? all_slots<TEAM, Slots>(p, sb) : 0.0f);
 }
@@ -454,22 +466,13 @@ __device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const flo
             s = fmaf(n * (m - mean), m - mean, s);
         }
         s = warp_sum(s);
+    } else if (layer) {   // a slot a lane (all threads going through them took three times the instructions)
+        const int w = lane & (kWarps - 1);
+        const float m = slots.b[set][w], n = slots.count[w];
+        mean = lane_sums<kWarps>(m * n) / p.width;
+        s = lane_sums<kWarps>(fmaf(n * (m - mean), m - mean, slots.a[set][w]));
     } else {
         s = slot_sum<kWarps>(slots.a[set]);
-        if (layer) {
-            float m[kWarps], n[kWarps];
-#pragma unroll
-            for (int k = 0; k < kWarps; k++) {
-                m[k] = slots.b[set][k];
-                n[k] = slots.count[k];
-                mean = fmaf(m[k], n[k], mean);
-            }
-            mean /= p.width;
-            float between = 0.0f;
-#pragma unroll
-            for (int k = 0; k < kWarps; k++) between = fmaf(n[k] * (m[k] - mean), m[k] - mean, between);
-            s += between;
-        }
     }
     p.turn++;
     return make_float2(mean, rsqrtf(s * p.inverse + eps));
