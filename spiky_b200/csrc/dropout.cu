@@ -20,8 +20,9 @@ DropRule drop_rule(double p) {
 
 // A thread takes the eight elements of a generator block; VEC, whole blocks in aligned arrays: two such blocks of 4-byte elements side by side, four of
 // 2-byte ones, whose rounds are independent and share the keys; the others element by element.  Bound: 4-byte types by the memory (67 M
-// values 83 us, 6.4 TB/s, with a block for each 4096 of them; 92 us with the same threads on a grid of eight blocks an SM), 2-byte types by
-// the integer unit beside it, some 75 of its operations for eight elements (four side by side 57 us, two 61, one 67).
+// values 83 us, 6.4 TB/s, with a block of threads for each 4096 of them; 92 us when a grid of eight blocks an SM went through them), 2-byte types
+// by the integer unit beside it, some 75 of its operations for eight elements (51 us, 5.3 TB/s; on another, slower-clocked GPU four side
+// by side 57, two 61, one 67).  Tried and slower: the next 32 bytes a thread loaded ahead (67 us), the rounds' keys in registers (54).
 constexpr int64_t kDropMost = 2048ll * INT32_MAX;   // (a grid has 2^31 - 1 blocks, of 2048 elements at least)
 
 template <class T>

@@ -6,6 +6,10 @@
 
 namespace lutb {
 
+// The kernels of this file take rows of any width and any number of rows, the entry points give them those that the row kernels (residual_rows.cuh)
+// do not: a block a row, which goes through the row once for each sum and reads it from L1 and L2 after the first time, and forms the mask
+// again each time.  2048 x 16392 fp32 with both norms, gate and dropout: forward 0.50 ms, backward 1.6 (the row kernels at 16384: 0.12 and
+// 0.25; plain torch operations 7.2 for both).
 constexpr int kRowThreads = 256;
 
 // The sum over the block's threads, in every thread, the same order for all.

@@ -1,15 +1,19 @@
 // Row kernels of the residual joins: a row's elements stay in registers from the first sum to the last store.
 //
-// A thread has groups of eight elements of a row.  A team of threads has a row: a warp or a part of one, a block, or beyond 4096 elements
-// (backward 2048) a cluster of up to eight blocks; sums over a row go through shuffles, shared memory and the cluster's shared memory
-// accordingly, one exchange for each norm and direction (a norm's mean and squares are combined from the warps' own by the pairwise
-// formula of Chan, Golub and LeVeque, 1979, so that no square is taken about a mean that is far off).  What a team does depends on the width
-// alone, so that a row's result does not depend on the rows beside it.
+// A thread has groups of eight elements of a row.  A team of threads has a row: a warp or a part of one up to 1024 elements (backward 256), a block up
+// to 8192 (4096), beyond a cluster of two (or four) blocks; sums over a row go through shuffles, shared memory and the cluster's shared
+// memory accordingly, one exchange for each norm and direction (a norm's mean and squares are combined from the warps' own by the pairwise
+// formula of Chan, Golub and LeVeque, 1979, so that no square is taken about a mean that is far off).  What a team does depends on the
+// width and the arrays' alignment alone, so that a row's result does not depend on the rows beside it.
 //
 // The next rows are fetched into shared memory with 16-byte asynchronous copies.  Rows of a multiple of eight elements in aligned arrays (VEC): a
 // group is eight neighbours, a warp fetches what its threads will read (no barrier of the block), and one generator block decides a group's
 // mask.  Other rows: the team fetches the aligned 16-byte pieces that its row touches, a thread's elements are a team apart, so that a
 // warp reads and stores neighbours, and the mask's bytes go through shared memory too.
+//
+// Bound: the memory at 4-byte types (32768 x 1024 fp32 with both norms, gate and dropout: forward 95 us, 5.6 TB/s, backward 153 us, 5.3 TB/s),
+// instruction issue at 2-byte ones (bf16: 73 us, 3.7 TB/s, and 123 us, 3.3 TB/s: some 290 instructions for a warp's 256 elements forward and 560
+// backward, 110 of them the generator and its mask; 16 warps an SM, as registers allow, issue 2.1 to 2.3 a cycle).
 #pragma once
 
 #include <atomic>
@@ -24,7 +28,6 @@ constexpr int kBlockThreads = 256, kWideThreads = 512;   // of a team; a warp's 
 constexpr int kForwardCluster = 2, kBackwardCluster = 4;
 constexpr int64_t kRowMaxWidth = 16384;   // such clusters of 512 threads, of two groups forward and one backward, or 512 threads of four
 constexpr int64_t kRowMaxRows = 1 << 30;  // (row numbers of 32 bits)
-
 
 enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_ANY = 4 };   // a block of up to 256 or 512 threads; ANY: told at run time (wide rows that are not VEC, backward)
 
@@ -54,7 +57,8 @@ inline void shape_team(RowShape &s, int64_t width, int block) {
 }
 // Forward.  VEC: up to 256 elements one group a thread, up to 1024 four, always within a warp, with the parameters read for each row (20 KB at most, which
 // stay in L1); beyond, two groups with the parameters in registers and slots of shared memory: read again for each row they came from L2, 20 bytes an element
-// against the rows' own 8 at 16 bits (12288 x 8192 bf16 with all of them: 313 us so, 200 us held).  Rows that are not VEC have one group up to
+// against the rows' own 8 at 16 bits (12288 x 8192 bf16 with all of them: 313 us so, 267 held; over a cluster of two blocks of 256 threads
+// instead of one block of 512: 412).  Rows that are not VEC have one group up to
 // 2048, where a warp's loads cover more neighbours.
 inline RowShape forward_shape(int64_t width, bool vec) {
     RowShape s{};
@@ -65,7 +69,8 @@ inline RowShape forward_shape(int64_t width, bool vec) {
     shape_team(s, width, 128);
     return s;
 }
-// Backward: one group, whose five sums over the rows take forty registers.  Stages of a block's or cluster's rows 16 bytes apart measured faster
+// Backward: one group, whose five sums over the rows take forty registers, a block of up to 512 threads (16384 x 4096 bf16 268 us, two blocks of 256 as a
+// cluster 325).  Stages of a block's or cluster's rows 16 bytes apart measured faster
 // than end to end (32768 x 1024 fp32 145 against 165 us, 12288 x 8192 bf16 558 against 575), those of a warp's rows did not (65536 x 256: 78 against
 // 75), nor did the forward pass's.
 inline RowShape backward_shape(int64_t width) {
