@@ -11,7 +11,7 @@
 // mask.  Other rows: the team fetches the aligned 16-byte pieces that its row touches, a thread's elements are a team apart, so that a
 // warp reads and stores neighbours, and the mask's bytes go through shared memory too.
 //
-// Bound: the memory at 4-byte types (32768 x 1024 fp32 with both norms, gate and dropout: forward 95 us, 5.6 TB/s, backward 153 us, 5.3 TB/s),
+// Bound: the memory at 4-byte types (32768 x 1024 fp32 with both norms, gate and dropout: forward 93 us, 5.8 TB/s, backward 153 us, 5.3 TB/s),
 // instruction issue at 2-byte ones (bf16: 73 us, 3.7 TB/s, and 123 us, 3.3 TB/s: some 290 instructions for a warp's 256 elements forward and 560
 // backward, 110 of them the generator and its mask; 16 warps an SM, as registers allow, issue 2.1 to 2.3 a cycle).
 #pragma once
