@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(kRowThreads) join_backward_kernel(const JoinAr
     for (int64_t chunk = blockIdx.x; chunk < a.chunks; chunk += gridDim.x) {
         const int64_t group = chunk / a.per_group, begin = group * a.group_rows + (chunk - group * a.per_group) * a.chunk_rows;
         const int64_t end = min(begin + a.chunk_rows, min((group + 1) * a.group_rows, a.rows));
-        float *const gate_sums = gate_summed ? a.gate_sums + chunk * a.width : nullptr;
+        float *const gate_sums = gate_summed ? a.gate_sums + (a.gate_direct ? (int64_t)blockIdx.x : chunk) * a.width : nullptr;
         if (gate_summed)
             for (int64_t c = threadIdx.x; c < a.width; c += kRowThreads) gate_sums[c] = 0.0f;
         __syncthreads();
@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(kRowThreads) join_backward_kernel(const JoinAr
                     else
                         static_cast<F *>(a.dgate)[group * a.width + c] = from_f32<F>(gate_sums[c]);
                 }
+            __syncthreads();   // (the next chunk clears them by other threads)
         }
     }
 }
@@ -384,6 +385,10 @@ static JoinSplit split_backward(const lutb_join_cfg *cfg, bool gate_gradient, bo
     const int64_t blocks = resident(cfg, true, vec, alone, s);
     return join_split(cfg->rows, group_rows, blocks, s.teams);
 }
+// Rows of workspace for the gate's sums: one a chunk, or where a chunk is a whole gate row none (the kernel for wide rows: one a block).
+static int64_t gate_sum_rows(const lutb_join_cfg *cfg, const JoinSplit &s) {
+    return cfg->gate_rows <= 1 ? 0 : s.per_group > 1 ? s.chunks : row_kernels(cfg) ? 0 : s.blocks;
+}
 static void take_split(JoinArgs &a, const JoinSplit &s) {
     a.group_rows = s.group_rows;
     a.per_group = s.per_group;
@@ -524,7 +529,7 @@ extern "C" size_t lutb_join_backward_workspace(const lutb_join_cfg *cfg) {
             RowShape shape{};
             const bool gated = kind == 1;
             const JoinSplit split = split_backward(cfg, gated, vec != 0, kind == 2, shape);
-            const size_t need = (size_t)(4 * split.blocks + (gated && cfg->gate_rows > 1 ? split.chunks : 0)) * cfg->width;
+            const size_t need = (size_t)(4 * split.blocks + (gated ? gate_sum_rows(cfg, split) : 0)) * cfg->width;
             floats = need > floats ? need : floats;
         }
     return floats * sizeof(float);
@@ -571,7 +576,6 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     const JoinSplit split = split_backward(cfg, dgate != nullptr, vec, f == nullptr, shape);
     take_split(a, split);
     a.gate_direct = gate_summed && split.per_group == 1;
-    const bool gate_parts = gate_summed && !(a.gate_direct && row_kernels(cfg));   // (the kernel for wide rows sums there in any case)
     SumList l{};
     float *at = static_cast<float *>(workspace);
     size_t need = 0;
@@ -582,10 +586,10 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
         l.count++;
         need += (size_t)split.blocks * cfg->width;
     }
-    if (gate_parts) {
+    if (gate_summed) {
         a.gate_sums = at + need;
         l.from[l.count] = a.gate_sums; l.to[l.count] = dgate; l.parts[l.count] = split.per_group; l.f32[l.count] = a.gate_f32;
-        need += (size_t)split.chunks * cfg->width;
+        need += (size_t)gate_sum_rows(cfg, split) * cfg->width;
     }
     LUTB_REQUIRE(need == 0 || (workspace != nullptr && workspace_bytes >= need * sizeof(float)), LUTB_ERR_WORKSPACE,
                  "workspace of %zu bytes needed", need * sizeof(float));

@@ -239,6 +239,10 @@ def test_join_many_rows(C, lead):
 def test_join_very_wide(C):
     run_join(torch.float32, torch.bfloat16, (3,), C, "layer", "rms", gate="width", p=0.1, seed=C)
     run_join(torch.float32, torch.float32, (5,), C, None, "layer", alone=True, seed=C)
+    if C == 20000:   # more gate rows than blocks, fewer, and one in pieces
+        run_join(torch.float32, torch.float32, (700, 2), C, "rms", None, gate="sequence", seed=1)
+        run_join(torch.bfloat16, torch.bfloat16, (3, 40), C, None, "rms", gate="sequence", params=torch.bfloat16, seed=2)
+        run_join(torch.float32, torch.float32, (900,), C, None, None, gate="width", seed=3)
 
 
 @pytest.mark.parametrize("ups", ["h", "y", "hy"])
@@ -466,3 +470,108 @@ def test_modules():
     plain = r.ResidualJoin(24, device=DEV)
     h, y = plain(x, x)
     assert h is y and torch.equal(h, x + x)
+
+
+@pytest.mark.parametrize("C,shift", [(64, 0), (64, 1), (67, 0), (67, 3), (1024, 2), (1031, 0), (5000, 0), (5001, 1), (16400, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+def test_nothing_beside_the_outputs_is_written(C, shift, dtype):
+    """The C entry points on arrays that begin anywhere, each between guards: the results are those of aligned arrays, the guards stay."""
+    import ctypes
+
+    from spiky_b200 import _native as nat
+
+    L, gen, rows, GUARD = nat.lib(), torch.Generator().manual_seed(C), 7, 64
+    code = nat.F32 if dtype == torch.float32 else nat.BF16
+    values = {k: normal(gen, s).to(dtype).to(DEV) for k, s in dict(x=(rows, C), f=(rows, C), gate=(rows, C), aw=(C,), ab=(C,), bw=(C,), bb=(C,),
+                                                                   dh=(rows, C), dy=(rows, C)).items()}
+    state = lib().dropout_state(3, DEV)
+    cfg = nat.JoinCfg(rows=rows, width=C, gate_rows=1, site=1, dropout=0.25, stream_type=code, branch_type=code, param_type=code, gate_type=code,
+                      after=nat.NORM_LAYER, before=nat.NORM_RMS, eps=1e-5, skip_scale=0.5, branch_scale=2.0)
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def run(shift):
+        held, outs = [], {}
+
+        def placed(t, guard):
+            flat = torch.full((t.numel() + shift + GUARD,), guard, dtype=t.dtype, device=DEV)
+            flat[shift:shift + t.numel()] = t.reshape(-1)
+            held.append(flat)
+            return flat[shift:shift + t.numel()]
+
+        v = {k: placed(t, float("nan")) for k, t in values.items()}   # (what is beside an input may be read, never used)
+
+        def out(name, *shape):
+            flat = torch.full((torch.Size(shape).numel() + 2 * GUARD + shift,), 7.0, dtype=dtype, device=DEV)
+            outs[name] = flat
+            return flat.data_ptr() + (GUARD + shift) * flat.element_size()
+
+        stats = torch.zeros(rows, 4, device=DEV)
+        p = {k: t.data_ptr() for k, t in v.items()}
+        nat.check(L.lutb_join_forward(ctypes.byref(cfg), p["x"], p["f"], p["gate"], p["aw"], p["ab"], p["bw"], p["bb"], state.data_ptr(),
+                                      out("h", rows, C), out("y", rows, C), stats.data_ptr(), stream))
+        need = L.lutb_join_backward_workspace(ctypes.byref(cfg))
+        ws = torch.full((need + 64,), 9, dtype=torch.uint8, device=DEV)
+        nat.check(L.lutb_join_backward(ctypes.byref(cfg), p["x"], p["f"], p["gate"], p["aw"], p["ab"], p["bw"], state.data_ptr(), stats.data_ptr(), p["dh"],
+                                       p["dy"], out("dx", rows, C), out("df", rows, C), out("dgate", rows, C), out("daw", C), out("dab", C),
+                                       out("dbw", C), out("dbb", C), ws.data_ptr(), need, stream))
+        nat.check(L.lutb_dropout(code, rows * C, 0.25, state.data_ptr(), 0, p["x"], out("z", rows, C), stream))
+        torch.cuda.synchronize()
+        assert torch.all(ws[need:] == 9)
+        got = {}
+        for name, flat in outs.items():
+            inner = flat[GUARD + shift:-GUARD]
+            assert torch.all(flat[:GUARD + shift] == 7) and torch.all(flat[-GUARD:] == 7), name
+            got[name] = inner.clone()
+        return got
+
+    here, plain = run(shift), run(0)
+    for name in here:
+        a, b = here[name].cpu().double(), plain[name].cpu().double()
+        assert a.isfinite().all(), name
+        # (both were rounded from values that float32 sums in another order made: two halves of a step of the larger, not one)
+        bound = 2 * ro.HALF_STEP[dtype] * torch.maximum(a.abs(), b.abs()) + ro.ROUNDINGS * 2.0 ** -24 * (b.abs() + b.abs().mean() + 1)
+        assert ((a - b).abs() <= bound).all(), name
+
+
+def test_two_streams_at_once():
+    """The same join on two streams and two threads: nothing is shared between calls."""
+    import threading
+
+    r = lib()
+    x, f, w = torch.randn(3000, 1024, device=DEV), torch.randn(3000, 1024, device=DEV), torch.rand(1024, device=DEV)
+    g = torch.randn(3000, 1024, device=DEV)
+    state = r.dropout_state(5, DEV)
+
+    def step():
+        leaves = [t.detach().requires_grad_() for t in (x, f, w)]
+        h, y = r.residual_join(leaves[0], leaves[1], branch_norm="rms", branch_weight=leaves[2], dropout=0.2, state=state, next_norm="layer")
+        return [h, y] + list(torch.autograd.grad([h, y], leaves, [g, g]))
+
+    want = [t.detach().clone() for t in step()]
+    torch.cuda.synchronize()
+    got, streams = {}, [torch.cuda.Stream() for _ in range(2)]
+
+    def work(k):
+        with torch.cuda.stream(streams[k]):
+            for _ in range(10):
+                got[k] = [t.detach().clone() for t in step()]
+
+    threads = [threading.Thread(target=work, args=(k,)) for k in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    for k in range(2):
+        for a, b in zip(got[k], want):
+            assert torch.equal(a, b)
+
+
+def test_gradients_of_expanded_inputs():
+    r = lib()
+    x = torch.randn(1, 5, 48, device=DEV, requires_grad=True)
+    f, gate = torch.randn(4, 5, 48, device=DEV), torch.randn(1, device=DEV, requires_grad=True)
+    h = r.residual_join(x.expand(4, 5, 48), f, gate=gate)
+    dx, dg = torch.autograd.grad(h, [x, gate], torch.ones_like(h))
+    assert torch.equal(dx, torch.full_like(dx, 4.0))
+    ro.assert_near(dg, f.cpu().double().sum().reshape(1), f.cpu().double().abs().sum().reshape(1), "dgate")
