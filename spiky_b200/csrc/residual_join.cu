@@ -339,13 +339,15 @@ int resident_clusters(const void *kernel, const RowShape &s, size_t smem) {
     return n;
 }
 
-// Gives the shape its stages (the most of three with which as many threads as registers allow are resident, 512 an SM or, forward, 384; two or one
-// otherwise) and returns how many teams of blocks the device holds: a cluster beyond those would run in a second round.
+// Gives the shape its stages (the most of three with which as many threads as registers allow are resident, or, forward, 384 an SM; two or one
+// otherwise) and returns how many teams of blocks the device holds: a cluster beyond those would run in a second round.  Threads by registers:
+// 512 an SM, 384 of the forward kernel with four groups (kForwardBlocks), 640 of a norm's backward pass in blocks, which takes 90
+// (32768 x 1024 bf16 52 us with 512, 48 with 640).
 static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, bool alone, RowShape &s) {
     const DeviceInfo info = device_info();
     const int sm = info.sm_count > 0 ? info.sm_count : 148;   // (no device: a size can be asked for all the same)
     const size_t own = backward ? (s.kind == TEAM_WARP ? kBackwardStatic : kBackwardTeamStatic) : vec ? kForwardVecStatic : kForwardStatic;
-    const int most = 512 / s.threads, wanted = backward ? most : 384 / s.threads > 1 ? 384 / s.threads : 1;
+    const int most = !backward && !alone && s.kind == TEAM_WARP && s.groups == 4 ? 3 : (backward && alone && s.kind == TEAM_BLOCK ? 640 : 512) / s.threads, wanted = backward ? most : 384 / s.threads > 1 ? 384 / s.threads : 1;
     int blocks = 1;
     size_t dynamic = 0;
     for (s.stages = 3; s.stages >= 1; s.stages--) {

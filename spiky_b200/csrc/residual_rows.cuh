@@ -12,7 +12,7 @@
 // warp reads and stores neighbours, and the mask's bytes go through shared memory too.
 //
 // Bound: the memory at 4-byte types (32768 x 1024 fp32 with both norms, gate and dropout: forward 93 us, 5.8 TB/s, backward 153 us, 5.3 TB/s),
-// instruction issue at 2-byte ones (bf16: 73 us, 3.7 TB/s, and 123 us, 3.3 TB/s: some 290 instructions for a warp's 256 elements forward and 560
+// instruction issue at 2-byte ones (bf16: 69 us, 3.9 TB/s, and 125 us, 3.2 TB/s: some 290 instructions for a warp's 256 elements forward and 560
 // backward, 110 of them the generator and its mask; 16 warps an SM, as registers allow, issue 2.1 to 2.3 a cycle).
 #pragma once
 
@@ -719,8 +719,13 @@ __host__ __device__ inline int held_bytes(bool vec, const RowShape &s) {
 template <int G, int TEAM>
 constexpr int kThreadsOf = TEAM == TEAM_WARP ? 128 : TEAM == TEAM_BLOCK ? kBlockThreads : kWideThreads;
 
+// Blocks an SM: 512 threads of 128 registers, but three warps a scheduler of 168 where a thread has four groups and a branch (32768 x 1024 bf16 73
+// against 69 us; fp32 the same).
+template <int BRANCH, int G, int TEAM>
+constexpr int kForwardBlocks = BRANCH && G == 4 && TEAM == TEAM_WARP ? 3 : 512 / kThreadsOf<G, TEAM>;
+
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int G, int TEAM>
-__global__ void __launch_bounds__(kThreadsOf<G, TEAM>, 512 / kThreadsOf<G, TEAM>) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
+__global__ void __launch_bounds__(kThreadsOf<G, TEAM>, kForwardBlocks<BRANCH, G, TEAM>) join_rows_forward_kernel(const JoinArgs a, const RowShape shape) {
     constexpr int kThreads = kThreadsOf<G, TEAM>;
     constexpr bool kHeld = VEC ? TEAM != TEAM_WARP : G == 1;   // the parameters are kept
     extern __shared__ __align__(16) unsigned char dynamic[];

@@ -205,6 +205,15 @@ def test_join_widths(types, C):
              p=0.2, params=rng.choice([torch.float32, types[1]]), seed=C)
 
 
+@pytest.mark.parametrize("types", [TYPES[0], TYPES[3]], ids=["f32", "f32-bf16"])
+@pytest.mark.parametrize("C", [2049, 2600, 3001, 4104, 8184, 8193, 12000, 12001, 16383, 16384])
+def test_join_wide_rows(types, C):
+    """Blocks of 512 threads and clusters, of whole groups and of odd rows; each sum, and more rows than are taken at once."""
+    run_join(*types, (2, 3), C, "layer", "layer", gate="sequence", p=0.1, seed=C)
+    run_join(*types, (170, 1), C, "rms", "rms", gate="width", p=0.3, seed=C + 1, params=types[1])
+    run_join(*types, (2, 2), C, None, "layer", alone=True, seed=C)
+
+
 @pytest.mark.parametrize("after", [None, "rms", "layer"])
 @pytest.mark.parametrize("before", [None, "rms", "layer"])
 @pytest.mark.parametrize("gate", ["none", "one", "width", "sequence", "element"])
