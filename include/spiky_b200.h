@@ -571,7 +571,9 @@ int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const void *f, co
 
 /*
  * Gradients of the above from dh and dy (one of them may be NULL: zeros); each output may be NULL.  random, site and dropout are
- * the forward call's, and so are stats.  Sums over rows (of the parameters, and of a gate row that several rows share) are taken
+ * the forward call's, and so are stats.  What is not needed may be NULL: stats without norms, x without dy, f where cfg->before is
+ * LUTB_NORM_NONE, there is no norm after the block and dgate is NULL (with a norm before the next block, f == NULL says that there was
+ * no branch).  Sums over rows (of the parameters, and of a gate row that several rows share) are taken
  * in float32 in an order that does not change from call to call.  The workspace is 16-byte aligned, not kept between calls.
  */
 size_t lutb_join_backward_workspace(const lutb_join_cfg *cfg);

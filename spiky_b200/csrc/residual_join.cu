@@ -59,7 +59,7 @@ struct JoinRow {
     __device__ float gate(int64_t c) const { return a.branch * join_param<F>(a.gate, a.gate_f32, gate_at + c, 1.0f); }
     __device__ float stream(int64_t c, uint32_t stays) const {
         const float x = to_f32(static_cast<const X *>(a.x)[at + c]);
-        return a.f == nullptr ? x : a.skip * x + gate(c) * normed(c, stays);
+        return a.alone ? x : a.skip * x + gate(c) * normed(c, stays);
     }
 };
 
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kRowThreads) join_backward_kernel(const JoinAr
         __syncthreads();
         for (int64_t row = begin; row < end; row++) {
             JoinRow<X, F> j(a, row);
-            const float4 st = a.stats[row];
+            const float4 st = a.stats ? a.stats[row] : make_float4(0.0f, 1.0f, 0.0f, 1.0f);
             j.mean = st.x;
             j.r = st.y;
             float c1 = 0.0f, c2 = 0.0f;
@@ -173,8 +173,8 @@ __global__ void __launch_bounds__(kRowThreads) join_backward_kernel(const JoinAr
                     if (sums[2]) sums[2][c] += g * zh;
                     if (sums[3]) sums[3][c] += g;
                 }
-                if (a.dx) static_cast<X *>(a.dx)[j.at + c] = from_f32<X>(a.f ? a.skip * d : d);
-                if (a.f == nullptr) return;
+                if (a.dx) static_cast<X *>(a.dx)[j.at + c] = from_f32<X>(a.alone ? d : a.skip * d);
+                if (a.alone) return;
                 if (a.dgate) {
                     const float dg = a.branch * d * j.normed(c, k);
                     if (gate_summed)
@@ -184,7 +184,7 @@ __global__ void __launch_bounds__(kRowThreads) join_backward_kernel(const JoinAr
                     else
                         static_cast<F *>(a.dgate)[j.gate_at + c] = from_f32<F>(dg);
                 }
-                const float dn = j.gate(c) * d, xh = j.scaled(c, k);
+                const float dn = j.gate(c) * d, xh = a.after == LUTB_NORM_NONE ? 0.0f : j.scaled(c, k);
                 if (sums[0]) sums[0][c] += dn * xh;
                 if (sums[1]) sums[1][c] += dn;
                 if (a.df) {
@@ -511,6 +511,7 @@ extern "C" int lutb_join_forward(const lutb_join_cfg *cfg, const void *x, const 
     const bool vec = cfg->width % kRowElems == 0 && all_aligned(16, {x, f, gate, after_weight, after_bias, before_weight, before_bias}) && all_aligned(32, {h, y});
     RowShape shape{};
     const JoinSplit split = split_forward(cfg, vec, f == nullptr, shape);
+    a.alone = f == nullptr;
     take_split(a, split);
     const cudaStream_t s = static_cast<cudaStream_t>(stream);
     return by_types(cfg, [&](auto xt, auto ft) -> int {
@@ -556,9 +557,13 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
             if (p) LUTB_CUDA(cudaMemsetAsync(p, 0, bytes, s));
         return LUTB_OK;
     }
-    LUTB_REQUIRE(x != nullptr && stats != nullptr && (dh != nullptr || dy != nullptr), LUTB_ERR_NULL, "x, stats and a gradient are required");
-    LUTB_REQUIRE(f != nullptr || (gate == nullptr && cfg->after == LUTB_NORM_NONE && cfg->dropout == 0.0 && df == nullptr && dy != nullptr && dh == nullptr), LUTB_ERR_NULL,
-                 "a join without branch has no gate, no norm after it, no dropout and no gradients of these");
+    LUTB_REQUIRE(dh != nullptr || dy != nullptr, LUTB_ERR_NULL, "a gradient is required");
+    LUTB_REQUIRE(stats != nullptr || (cfg->after == LUTB_NORM_NONE && dy == nullptr), LUTB_ERR_NULL, "stats are required for norms");
+    LUTB_REQUIRE(x != nullptr || dy == nullptr, LUTB_ERR_NULL, "x is required for the norm before the next block");
+    const bool alone = f == nullptr && cfg->before != LUTB_NORM_NONE;
+    LUTB_REQUIRE(!alone || (gate == nullptr && cfg->after == LUTB_NORM_NONE && cfg->dropout == 0.0 && df == nullptr && dy != nullptr && dh == nullptr), LUTB_ERR_NULL,
+                 "a norm alone has no gate, no norm after it, no dropout and no gradients of these");
+    LUTB_REQUIRE(f != nullptr || alone || (cfg->after == LUTB_NORM_NONE && dgate == nullptr), LUTB_ERR_NULL, "f is required for its norm and for the gate's gradient");
     LUTB_REQUIRE(cfg->dropout == 0.0 || random != nullptr, LUTB_ERR_NULL, "random is required for dropout");
     LUTB_REQUIRE(aligned(x, cfg->stream_type) && aligned(dh, cfg->stream_type) && aligned(dx, cfg->stream_type) && aligned(f, cfg->branch_type) &&
                      aligned(dy, cfg->branch_type) && aligned(df, cfg->branch_type) && aligned(gate, cfg->gate_type) && aligned(dgate, cfg->gate_type) &&
@@ -575,7 +580,8 @@ extern "C" int lutb_join_backward(const lutb_join_cfg *cfg, const void *x, const
     const bool vec = cfg->width % kRowElems == 0 &&
                      all_aligned(16, {x, f, gate, after_weight, after_bias, before_weight, dh, dy}) && all_aligned(32, {dx, df, dgate});
     RowShape shape{};
-    const JoinSplit split = split_backward(cfg, dgate != nullptr, vec, f == nullptr, shape);
+    const JoinSplit split = split_backward(cfg, dgate != nullptr, vec, alone, shape);
+    a.alone = alone;
     take_split(a, split);
     a.gate_direct = gate_summed && split.per_group == 1;
     SumList l{};

@@ -1,6 +1,6 @@
 // Joins of a block with the residual stream, as their kernels see them:
 //   t = drop(f), n = after-norm of t (affine), h = skip x + branch gate n, y = before-norm of h (affine);
-// without f, h is x (the norm before a block alone).
+// alone, h is x (the norm before a block).
 #pragma once
 
 #include "residual.cuh"
@@ -17,6 +17,7 @@ struct JoinArgs {
     int64_t rows, width, gate_rows;   // gate_rows: rows that share a gate row, 0 without gate
     int32_t after, before;            // LUTB_NORM_*
     int32_t params_f32, gate_f32;     // else of the branch's type
+    int32_t alone;                    // no branch: the norm before a block
     float eps, skip, branch;
     // backward
     const void *dh, *dy;

@@ -984,6 +984,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
     }
     if (NEXT) keep_param(2, a.bw, a.params_f32, 0, 1.0f, 1.0f);
     const bool gate_each = BRANCH && a.gate_rows == 1, gate_summed = BRANCH && a.dgate && a.gate_rows > 1, gate_f32 = sizeof(F) == 4 || a.gate_f32;
+    const bool with_f = BRANCH == 2 || (BRANCH && (NEXT || a.dgate));   // whether anything asks for the branch's values
     int gate_end = 0;   // first row of another gate row
     if (BRANCH && a.gate_rows == 0) keep_param(3, nullptr, true, 0, 1.0f, a.branch);
 
@@ -1003,7 +1004,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
         if (load.more(a)) {
             const bool some = sure || load.base + p.which < load.end;
             const int64_t row = some ? load.base + p.which : load.end - 1;
-            if (BRANCH) ring.template fetch<F, kF>(p, shape, part_f, f_in, row, some, a);
+            if (with_f) ring.template fetch<F, kF>(p, shape, part_f, f_in, row, some, a);
             if (NEXT) {
                 ring.template fetch<X, 0>(p, shape, 0, x_in, row, some, a);
                 ring.template fetch<F, kDy>(p, shape, part_dy, dy_in, row, some, a);
@@ -1048,7 +1049,8 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
         const int row = here.base + p.which, chunk = here.chunk;
         const int64_t at = row * a.width;
         const bool on = sure || row < here.end;
-        const float4 st = a.stats[on ? row : here.end - 1];
+        float4 st = make_float4(0.0f, 1.0f, 0.0f, 1.0f);
+        if (BRANCH == 2 || NEXT) st = a.stats[on ? row : here.end - 1];
         if (BRANCH && a.gate_rows > 1 && on && row >= gate_end) {
             const int gate_row = row / (int)a.gate_rows;
             gate_end = (gate_row + 1) * (int)a.gate_rows;
@@ -1082,7 +1084,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
         set ^= 1;
         if (shape.stages > 1) fetch();
         float2 t[4];   // the branch, from its norm on normalised
-        if (BRANCH) {
+        if (with_f) {
             ring.template get<F, kF>(p, shape, 0, part_f, f_in, at, on, t);
             if (a.drop.on) drop8(t, kept, a.drop.scale);
             if (BRANCH == 2)
@@ -1268,7 +1270,7 @@ const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
 template <class X, class F>
 int launch_join_rows(bool backward, bool vec, const JoinArgs &a, const RowShape &s, int clusters, cudaStream_t stream) {
     static std::atomic<uint32_t> opted[2][2][6][8];
-    const int kind = (a.f == nullptr ? 0 : a.after == LUTB_NORM_NONE ? 1 : 2) * 2 + (backward ? a.dy != nullptr : a.y != nullptr);
+    const int kind = (a.alone ? 0 : a.after == LUTB_NORM_NONE ? 1 : 2) * 2 + (backward ? a.dy != nullptr : a.y != nullptr);
     const void *kernel = kind == 1   ? join_rows_kernel<X, F, 0, true>(backward, vec, s)
                          : kind == 2 ? join_rows_kernel<X, F, 1, false>(backward, vec, s)
                          : kind == 3 ? join_rows_kernel<X, F, 1, true>(backward, vec, s)
@@ -1276,7 +1278,7 @@ int launch_join_rows(bool backward, bool vec, const JoinArgs &a, const RowShape 
                          : kind == 5 ? join_rows_kernel<X, F, 2, true>(backward, vec, s)
                                      : nullptr;
     LUTB_REQUIRE(kernel != nullptr, LUTB_ERR_MODE, "nothing to compute");
-    const size_t smem = join_rows_smem<X, F>(backward, vec, s, a.f == nullptr, a.gate_rows == 1);
+    const size_t smem = join_rows_smem<X, F>(backward, vec, s, a.alone != 0, a.gate_rows == 1);
     return launch_rows(kernel, opted[backward][vec][kind][backward ? s.kind : 2 * s.kind + (s.groups > 1)], a, s, clusters, smem, stream);
 }
 

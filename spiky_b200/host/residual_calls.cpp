@@ -196,8 +196,9 @@ enum { X, F, GATE, AW, AB, BW, BB, TENSORS };
 
 struct JoinNode : public ResidualNode {
     lutb_join_cfg cfg;
-    bool has_h = false, had[TENSORS] = {};
+    bool has_h = false, had[TENSORS] = {}, kept[TENSORS] = {};   // what the call had, what of it the backward pass reads
     c10::DeviceIndex device = 0;
+    std::vector<int64_t> shape, gate_shape;
     std::string name() const override { return "_ResidualJoinBackward"; }
     variable_list apply(variable_list &&grads) override {
         std::vector<Tensor> s = unpack();   // the seven tensors, state, stats
@@ -209,27 +210,31 @@ struct JoinNode : public ResidualNode {
         const int types[TENSORS] = {cfg.stream_type, cfg.branch_type, cfg.gate_type, cfg.param_type, cfg.param_type, cfg.param_type, cfg.param_type};
         static const char *const what[TENSORS] = {"x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "next_bias"};
         for (int k = 0; k < TENSORS; k++)
-            if (had[k]) expect(s[k], scalar_type_of(types[k]), k <= F ? all : k == GATE ? all / cfg.gate_rows : cfg.width, device, what[k]);
+            if (kept[k]) expect(s[k], scalar_type_of(types[k]), k <= F ? all : k == GATE ? all / cfg.gate_rows : cfg.width, device, what[k]);
         if (cfg.dropout > 0.0) {
             expect(s[TENSORS], at::kLong, 2, device, "state");
             s[TENSORS] = s[TENSORS].contiguous();
         }
-        expect(s[TENSORS + 1], at::kFloat, 4 * cfg.rows, device, "stats");
-        s[TENSORS + 1] = s[TENSORS + 1].contiguous();
+        if (cfg.after != LUTB_NORM_NONE || cfg.before != LUTB_NORM_NONE) {
+            expect(s[TENSORS + 1], at::kFloat, 4 * cfg.rows, device, "stats");
+            s[TENSORS + 1] = s[TENSORS + 1].contiguous();
+        }
         if (dh.defined()) expect(dh, scalar_type_of(cfg.stream_type), all, device, "the gradient");
         if (dy.defined()) expect(dy, scalar_type_of(cfg.branch_type), all, device, "the gradient");
         {
             at::AutoDispatchBelowADInplaceOrView below;
             c10::cuda::CUDAGuard guard(device);
             for (int k = 0; k < TENSORS; k++)
-                if (s[k].defined() && task_should_compute_output(k) && (k < BW || dy.defined())) out[k] = new_like(s[k], s[k].scalar_type());
+                if (had[k] && task_should_compute_output(k) && (k < BW || dy.defined()))
+                    out[k] = at::empty(k <= F ? at::IntArrayRef(shape) : k == GATE ? at::IntArrayRef(gate_shape) : at::IntArrayRef(cfg.width),
+                                       at::TensorOptions().dtype(scalar_type_of(types[k])).device(at::kCUDA, device));
             for (int k = 0; k < BB; k++) s[k] = whole(s[k]);
             const Tensor dhc = whole(dh), dyc = whole(dy);
             Tensor ws;
             size_t need = 0;
             if (out[AW].defined() || out[AB].defined() || out[BW].defined() || out[BB].defined() || (out[GATE].defined() && cfg.gate_rows > 1)) {
                 need = lib.join_backward_workspace(&cfg);
-                ws = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(s[X].device()));
+                ws = at::empty({(int64_t)need}, at::TensorOptions().dtype(at::kByte).device(at::kCUDA, device));
             }
             check(lib.join_backward(&cfg, pointer(s[X]), pointer(s[F]), pointer(s[GATE]), pointer(s[AW]), pointer(s[AB]), pointer(s[BW]),
                                     random_of(s[TENSORS]), static_cast<const float *>(pointer(s[TENSORS + 1])), pointer(dhc), pointer(dyc), pointer(out[X]),
@@ -333,7 +338,8 @@ PyObject *join_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
         if (t[F].defined()) h = new_like(x, x.scalar_type());
         if (cfg.before != LUTB_NORM_NONE)
             y = new_like(x, scalar_type_of(cfg.branch_type));
-        if (graph) stats = at::empty({cfg.rows, 4}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
+        if (graph && (cfg.after != LUTB_NORM_NONE || cfg.before != LUTB_NORM_NONE))
+            stats = at::empty({cfg.rows, 4}, at::TensorOptions().dtype(at::kFloat).device(x.device()));
         check(lib.join_forward(&cfg, pointer(c[X]), pointer(c[F]), pointer(c[GATE]), pointer(c[AW]), pointer(c[AB]), pointer(c[BW]), pointer(c[BB]),
                                random_of(state), pointer(h), pointer(y), static_cast<float *>(pointer(stats)), stream_on(x.device().index())));
     }
@@ -342,9 +348,15 @@ PyObject *join_entry(PyObject *, PyObject *const *args, Py_ssize_t n) {
         node->cfg = cfg;
         node->has_h = h.defined();
         node->device = t[X].device().index();
-        for (int k = 0; k < TENSORS; k++) node->had[k] = t[k].defined();
+        node->shape = t[X].sizes().vec();
+        if (t[GATE].defined()) node->gate_shape = t[GATE].sizes().vec();
+        const bool norms = cfg.after != LUTB_NORM_NONE || cfg.before != LUTB_NORM_NONE;
+        for (int k = 0; k < TENSORS; k++) {
+            node->had[k] = t[k].defined();
+            node->kept[k] = t[k].defined() && (k == X ? cfg.before != LUTB_NORM_NONE : k == F ? norms || (t[GATE].defined() && t[GATE].requires_grad()) : k != BB);
+        }
         node->set_next_edges(torch::autograd::collect_next_edges(t[X], t[F], t[GATE], t[AW], t[AB], t[BW], t[BB]));
-        for (const Tensor &v : t) node->saved.emplace_back(v, false);
+        for (int k = 0; k < TENSORS; k++) node->saved.emplace_back(node->kept[k] ? t[k] : Tensor(), false);
         node->saved.emplace_back(state, false);
         node->saved.emplace_back(stats, false);
         variable_list outputs;

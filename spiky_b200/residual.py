@@ -7,7 +7,8 @@ No counterpart in the reference, whose transformer composes torch's dropout, ``B
   the backward pass; nothing of the size of ``x`` is kept.
 * ``row_norm(x, weight, bias, kind)``: RMS or layer norm over the last dimension, the norm before a block.
 * ``residual_join(x, branch, ...)``: ``h = skip_scale * x + branch_scale * gate * N(drop(branch))``, with the norm ``N`` after the
-  block, and in the same pass ``y = N'(h)``, the norm before the next block.
+  block, and in the same pass ``y = N'(h)``, the norm before the next block.  Only what the gradients need is kept: nothing of the
+  size of ``x`` where there is no norm and no learned gate.
 
 float32, bfloat16 and float16; a float32 stream may carry a 16-bit branch.  Sums, norms and their statistics are float32, every
 output is rounded once.  ``CounterDropout``, ``RowNorm`` and ``ResidualJoin`` are the modules; ``LUTTransformer`` uses them.  Ordinary calls run through
@@ -195,10 +196,16 @@ class _Join(torch.autograd.Function):
     def forward(ctx, cfg, x, branch, gate, aw, ab, bw, bb, state, stats):
         h, y = _join_forward(cfg, x, branch, gate, aw, ab, bw, bb, state, stats)
         ctx.cfg = cfg
-        ctx.had = [None if t is None else ((t.dtype, t.device), t.numel()) for t in (x, branch, gate, aw, ab, bw, bb, state, stats)]
+        given = (x, branch, gate, aw, ab, bw, bb)
+        ctx.had = [None if t is None else (t.shape, t.dtype, t.device) for t in given]
         ctx.of_grads = [None if t is None else (t.dtype, t.device) for t in (h, y)]
+        # what the backward pass reads: the stream for the next norm, the branch for norms and the gate's gradient
+        norms = cfg.after != _native.NORM_NONE or cfg.before != _native.NORM_NONE
+        kept = [x if cfg.before != _native.NORM_NONE else None, branch if norms or ctx.needs_input_grad[3] else None, gate, aw, ab, bw,
+                state, stats]
+        ctx.kept = [None if t is None else ((t.dtype, t.device), t.numel()) for t in kept]
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, branch, gate, aw, ab, bw, bb, state, stats)
+        ctx.save_for_backward(*kept)
         return h, y
 
     @staticmethod
@@ -207,27 +214,26 @@ class _Join(torch.autograd.Function):
         if dh is None and dy is None:
             return (None,) * 10
         cfg, need = ctx.cfg, ctx.needs_input_grad
-        saved = ctx.saved_tensors
-        names = ("x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "next_bias", "state", "stats")
-        con = [None if had is None else _expect(t, *had, name) for t, had, name in zip(saved, ctx.had, names)]
-        dh, dy = (None if t is None else _expect(t, like, ctx.had[0][1], "the gradient") for t, like in zip((dh, dy), ctx.of_grads))
-        x, branch, gate, aw, ab, bw, bb = saved[:7]
+        names = ("x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "state", "stats")
+        con = [None if kept is None else _expect(t, *kept, name) for t, kept, name in zip(ctx.saved_tensors, ctx.kept, names)]
+        shape, _, device = ctx.had[0]
+        dh, dy = (None if t is None else _expect(t, like, shape.numel(), "the gradient") for t, like in zip((dh, dy), ctx.of_grads))
 
-        def like(t, wanted):
-            return torch.empty(t.shape, dtype=t.dtype, device=t.device) if wanted and t is not None else None
+        def like(k, wanted=True):
+            had = ctx.had[k]
+            return torch.empty(had[0], dtype=had[1], device=had[2]) if had is not None and need[k + 1] and wanted else None
 
-        dx, df, dgate = like(x, need[1]), like(branch, need[2]), like(gate, need[3])
-        daw, dab = like(aw, need[4]), like(ab, need[5])
-        dbw, dbb = (like(bw, need[6]), like(bb, need[7])) if dy is not None else (None, None)
-        with torch.cuda.device(x.device):
+        dx, df, dgate, daw, dab = (like(k) for k in range(5))
+        dbw, dbb = like(5, dy is not None), like(6, dy is not None)
+        with torch.cuda.device(device):
             L = _native.lib()
             ws, size = None, 0
             if any(t is not None for t in (daw, dab, dbw, dbb)) or (dgate is not None and cfg.gate_rows > 1):
                 size = L.lutb_join_backward_workspace(ctypes.byref(cfg))
-                ws = torch.empty(size, dtype=torch.uint8, device=x.device)
+                ws = torch.empty(size, dtype=torch.uint8, device=device)
             _native.check(L.lutb_join_backward(
-                ctypes.byref(cfg), *(_ptr(t) for t in con[:6]), _ptr(con[7]), _ptr(con[8]), _ptr(dh), _ptr(dy), _ptr(dx), _ptr(df),
-                _ptr(dgate), _ptr(daw), _ptr(dab), _ptr(dbw), _ptr(dbb), _ptr(ws), size, _stream(x.device)))
+                ctypes.byref(cfg), *(_ptr(t) for t in con), _ptr(dh), _ptr(dy), _ptr(dx), _ptr(df),
+                _ptr(dgate), _ptr(daw), _ptr(dab), _ptr(dbw), _ptr(dbb), _ptr(ws), size, _stream(device)))
         return None, dx, df, dgate, daw, dab, dbw, dbb, None, None
 
 
@@ -289,7 +295,7 @@ def _join(x, branch, branch_type, after, aw, ab, gate, skip_scale, branch_scale,
         branch, gate = branch * gate.to(branch.dtype), None
         tensors = (x, branch, gate, aw, ab, bw, bb)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        stats = torch.empty((rows, 4), dtype=torch.float32, device=device)
+        stats = torch.empty((rows, 4), dtype=torch.float32, device=device) if after is not None or before is not None else None
         return _Join.apply(cfg, *tensors, state, stats)
     return _join_forward(cfg, *tensors, state, None)
 

@@ -140,6 +140,39 @@ def test_contexts(routes):
     assert a.shape == b.shape
 
 
+@pytest.mark.parametrize("kw,kept", [(dict(), 0), (dict(dropout=0.3), 0), (dict(gate="fixed"), 0), (dict(gate="learned"), 1), (dict(branch_norm="rms"), 1),
+                                     (dict(next_norm="layer"), 2), (dict(branch_norm="rms", next_norm="rms", dropout=0.3, gate="learned"), 2)])
+def test_what_is_kept_for_the_backward_pass(routes, kw, kept):
+    """Tensors of the stream's size that a join keeps: none without norms and a learned gate; its gradients are right all the same."""
+    from spiky_b200 import residual
+
+    def run():
+        for C in (64, 65, 16400):
+            x, f = (torch.randn(4, 5, C, device=DEV, requires_grad=True) for _ in range(2))
+            more = dict(kw)
+            if "gate" in more:
+                more["gate"] = torch.full((C,), 0.5, device=DEV, requires_grad=more["gate"] == "learned")
+            if "dropout" in more:
+                more["state"] = residual.dropout_state(2, DEV)
+            seen = []
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: seen.append(t.numel()) or t, lambda t: t):
+                out = residual.residual_join(x, f, skip_scale=0.5, **more)
+            assert seen.count(x.numel()) == kept
+            if not kept:
+                dh = torch.randn_like(x)
+                dx, df = torch.autograd.grad(out, [x, f], dh)
+                assert torch.equal(dx, 0.5 * dh)
+                want = dh * 0.5 if "gate" in kw else dh
+                if "dropout" in kw:
+                    want = residual.counter_dropout(want, 0.3, more["state"])
+                assert torch.equal(df, want)
+            else:
+                first = out if torch.is_tensor(out) else out[1]
+                assert all(g.isfinite().all() for g in torch.autograd.grad(first.sum(), [x, f]))
+
+    routes(run)
+
+
 def test_what_hooks_hand_back_is_checked(routes):
     """A saved tensor that comes back on another device, of another type or size is an error, not an address for a kernel."""
     from spiky_b200 import residual
