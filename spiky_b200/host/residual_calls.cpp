@@ -112,6 +112,12 @@ struct ResidualNode : public torch::autograd::Node {
 void expect(const Tensor &t, at::ScalarType type, int64_t numel, c10::DeviceIndex device, const char *name) {
     TORCH_CHECK(plain_cuda(t, type, device) && t.numel() == numel, name, " is not what the forward pass saved: ", numel, " elements of ", type, " on cuda:", (int)device);
 }
+// A gradient as the kernels read it: no lazy negation, no stand-in for zeros.
+Tensor settled(const Tensor &t) {
+    if (!t.defined()) return t;
+    if (t._is_zerotensor()) return at::zeros(t.sizes(), at::TensorOptions().dtype(t.scalar_type()).device(t.device()));
+    return t.is_neg() ? t.resolve_neg() : t;
+}
 at::ScalarType scalar_type_of(int type) { return type == LUTB_F32 ? at::kFloat : type == LUTB_BF16 ? at::kBFloat16 : at::kHalf; }
 
 // ------------------------------------------------------------------------------------------------ dropout
@@ -124,10 +130,11 @@ struct DropoutNode : public ResidualNode {
     variable_list apply(variable_list &&grads) override {
         const std::vector<Tensor> s = unpack();
         if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
-        expect(grads[0], grads[0].scalar_type(), grads[0].numel(), grads[0].device().index(), "the gradient");
-        expect(s[0], at::kLong, 2, grads[0].device().index(), "state");
-        TORCH_CHECK(type_of(grads[0].scalar_type()) >= 0 && s[0].is_contiguous(), "the gradient or state is not what the forward pass had");
-        return {dropout(grads[0], p, s[0], site)};   // (with a graph of its own where one is asked for)
+        const Tensor dy = settled(grads[0]);
+        expect(dy, dy.scalar_type(), dy.numel(), dy.device().index(), "the gradient");
+        expect(s[0], at::kLong, 2, dy.device().index(), "state");
+        TORCH_CHECK(type_of(dy.scalar_type()) >= 0 && s[0].is_contiguous(), "the gradient or state is not what the forward pass had");
+        return {dropout(dy, p, s[0], site)};   // (with a graph of its own where one is asked for)
     }
 };
 
@@ -202,7 +209,7 @@ struct JoinNode : public ResidualNode {
     std::string name() const override { return "_ResidualJoinBackward"; }
     variable_list apply(variable_list &&grads) override {
         std::vector<Tensor> s = unpack();   // the seven tensors, state, stats
-        const Tensor dh = has_h ? grads[0] : Tensor(), dy = cfg.before != LUTB_NORM_NONE ? grads[has_h ? 1 : 0] : Tensor();
+        const Tensor dh = has_h ? settled(grads[0]) : Tensor(), dy = cfg.before != LUTB_NORM_NONE ? settled(grads[has_h ? 1 : 0]) : Tensor();
         variable_list out(TENSORS);
         if (!dh.defined() && !dy.defined()) return out;
         const bool again = needs_graph({&dh, &dy});

@@ -204,6 +204,12 @@ def test_lazily_negated_tensors(routes):
         y = residual.row_norm(n, w)
         g, = torch.autograd.grad(y, w, torch._neg_view(torch.ones_like(y)))
         ro.assert_near(g, residual.row_norm(x).sum(0).cpu().double(), torch.full((16,), 10.0, dtype=torch.float64), "dw")
+        z = x.detach().requires_grad_()
+        up = torch.randn_like(x)
+        for out in (residual.residual_join(z, x, skip_scale=0.5), residual.counter_dropout(z, 0.5, state)):
+            plain, = torch.autograd.grad(out, z, up, retain_graph=True)
+            lazy, = torch.autograd.grad(out, z, torch._neg_view(up))
+            assert torch.equal(lazy, -plain)
 
     routes(negated)
 
