@@ -1089,7 +1089,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             if (a.drop.on) drop8(t, kept, a.drop.scale);
             if (BRANCH == 2)
 #pragma unroll
-                for (int k = 0; k < 4; k++) t[k] = fma2(t[k], both(st.y), both(-st.x * st.y));
+                for (int k = 0; k < 4; k++) t[k] = mul2(add2(t[k], both(-st.x)), both(st.y));   // (mean times r, rounded, would cost rows far from zero a bit)
         }
         auto branch_out = [&](float2 *n) {   // the branch after its norm
             if (BRANCH == 2) {
@@ -1119,7 +1119,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             param(2, u);
 #pragma unroll
             for (int k = 0; k < 4; k++) {
-                z[k] = fma2(z[k], both(st.w), both(-st.z * st.w));
+                z[k] = mul2(add2(z[k], both(-st.z)), both(st.w));
                 u[k] = mul2(g[k], u[k]);
                 s1 = fma2(u[k], z[k], s1);
             }
