@@ -11,7 +11,7 @@
 // mask.  Other rows: the team fetches the aligned 16-byte pieces that its row touches, a thread's elements are a team apart, so that a
 // warp reads and stores neighbours, and the mask's bytes go through shared memory too.
 //
-// Bound: the memory at 4-byte types (32768 x 1024 fp32 with both norms, gate and dropout: forward 93 us, 5.8 TB/s, backward 153 us, 5.3 TB/s),
+// Bound: the memory at 4-byte types (32768 x 1024 fp32 with both norms, gate and dropout: forward 93 us, 5.8 TB/s, backward 145 us, 5.6 TB/s),
 // instruction issue at 2-byte ones (bf16: 69 us, 3.9 TB/s, and 125 us, 3.2 TB/s: some 290 instructions for a warp's 256 elements forward and 560
 // backward, 110 of them the generator and its mask; 16 warps an SM, as registers allow, issue 2.1 to 2.3 a cycle).
 #pragma once
@@ -1089,7 +1089,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
             if (a.drop.on) drop8(t, kept, a.drop.scale);
             if (BRANCH == 2)
 #pragma unroll
-                for (int k = 0; k < 4; k++) t[k] = mul2(add2(t[k], both(-st.x)), both(st.y));   // (mean times r, rounded, would cost rows far from zero a bit)
+                for (int k = 0; k < 4; k++) t[k] = mul2(add2(t[k], both(-st.x)), both(st.y));   // (r t - r mean would cost rows far from zero a bit)
         }
         auto branch_out = [&](float2 *n) {   // the branch after its norm
             if (BRANCH == 2) {
