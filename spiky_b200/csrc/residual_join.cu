@@ -347,7 +347,8 @@ static int64_t resident(const lutb_join_cfg *cfg, bool backward, bool vec, bool 
     const DeviceInfo info = device_info();
     const int sm = info.sm_count > 0 ? info.sm_count : 148;   // (no device: a size can be asked for all the same)
     const size_t own = backward ? (s.kind == TEAM_WARP ? kBackwardStatic : kBackwardTeamStatic) : vec ? kForwardVecStatic : kForwardStatic;
-    const int most = !backward && !alone && s.kind == TEAM_WARP && s.groups == 4 ? 3 : (backward && alone && s.kind == TEAM_BLOCK ? 640 : 512) / s.threads, wanted = backward ? most : 384 / s.threads > 1 ? 384 / s.threads : 1;
+    const int threads = backward ? (alone && s.kind == TEAM_BLOCK ? 640 : 512) : !alone && s.kind == TEAM_WARP && s.groups == 4 ? 384 : 512;
+    const int most = threads / s.threads, wanted = backward ? most : 384 / s.threads > 1 ? 384 / s.threads : 1;
     int blocks = 1;
     size_t dynamic = 0;
     for (s.stages = 3; s.stages >= 1; s.stages--) {

@@ -29,7 +29,8 @@ constexpr int kForwardCluster = 2, kBackwardCluster = 4;
 constexpr int64_t kRowMaxWidth = 16384;   // such clusters of 512 threads, of two groups forward and one backward, or 512 threads of four
 constexpr int64_t kRowMaxRows = 1 << 30;  // (row numbers of 32 bits)
 
-enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_ANY = 4 };   // a block of up to 256 or 512 threads; ANY: told at run time (wide rows that are not VEC, backward)
+// BLOCK and WIDE: a block of up to 256 or 512 threads.  ANY: told at run time (backward, wide rows that are not VEC).
+enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_ANY = 4 };
 
 struct RowShape {
     int groups;                 // of a thread
