@@ -112,6 +112,11 @@ struct ResidualNode : public torch::autograd::Node {
 void expect(const Tensor &t, at::ScalarType type, int64_t numel, c10::DeviceIndex device, const char *name) {
     TORCH_CHECK(plain_cuda(t, type, device) && t.numel() == numel, name, " is not what the forward pass saved: ", numel, " elements of ", type, " on cuda:", (int)device);
 }
+// As residual.py's _refuse_recording.
+void refuse_recording() {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() && !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value(),
+                "residual operators cannot be traced: their kernels would be missing from what is recorded");
+}
 // A gradient as the kernels read it: no lazy negation, no stand-in for zeros.
 Tensor settled(const Tensor &t) {
     if (!t.defined()) return t;
@@ -130,6 +135,7 @@ struct DropoutNode : public ResidualNode {
     variable_list apply(variable_list &&grads) override {
         const std::vector<Tensor> s = unpack();
         if (!grads[0].defined() || !task_should_compute_output(0)) return variable_list(1);
+        refuse_recording();
         const Tensor dy = settled(grads[0]);
         expect(dy, dy.scalar_type(), dy.numel(), dy.device().index(), "the gradient");
         expect(s[0], at::kLong, 2, dy.device().index(), "state");
@@ -212,6 +218,7 @@ struct JoinNode : public ResidualNode {
         const Tensor dh = has_h ? settled(grads[0]) : Tensor(), dy = cfg.before != LUTB_NORM_NONE ? settled(grads[has_h ? 1 : 0]) : Tensor();
         variable_list out(TENSORS);
         if (!dh.defined() && !dy.defined()) return out;
+        refuse_recording();
         const bool again = needs_graph({&dh, &dy});
         const int64_t all = cfg.rows * cfg.width;
         const int types[TENSORS] = {cfg.stream_type, cfg.branch_type, cfg.gate_type, cfg.param_type, cfg.param_type, cfg.param_type, cfg.param_type};

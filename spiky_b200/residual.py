@@ -19,6 +19,7 @@ contiguous are copied.  Work goes to torch's current stream of the tensors' devi
 """
 import ctypes
 import math
+import sys
 import warnings
 
 import torch
@@ -62,6 +63,14 @@ def _stream(device):
     return torch.cuda.current_stream(device).cuda_stream
 
 
+def _refuse_recording():
+    """The kernels are called past torch: a trace or a graph of torch's operators would keep the outputs' allocation alone, and the sizes of
+    this call whatever it is given later."""
+    fx = sys.modules.get("torch.fx.experimental.proxy_tensor")
+    if torch.jit.is_tracing() or (fx is not None and fx.get_proxy_mode() is not None):
+        raise RuntimeError("residual operators cannot be traced: their kernels would be missing from what is recorded")
+
+
 def _check_data(t, name, device=None):
     if not isinstance(t, torch.Tensor):
         raise RuntimeError(f"{name} must be a tensor")
@@ -100,6 +109,7 @@ def take_dropout_state(state, count):
     used = (_calls or _native_calls()).take(state, count)
     if used is not None:
         return used
+    _refuse_recording()
     _check_dropout(1.0, state, 0, state.device if isinstance(state, torch.Tensor) else None)
     if not state.is_cuda:
         raise RuntimeError("state must be on CUDA: spiky_b200 has no CPU path")
@@ -163,6 +173,7 @@ def counter_dropout(x, p, state, site=0):
     _check_dropout(p, state, site, x.device)
     if p == 0.0:
         return x.clone()
+    _refuse_recording()
     if x.requires_grad and torch.is_grad_enabled():
         return _CounterDropout.apply(x, p, state, site)
     return _dropout(x, p, state, site)
@@ -213,6 +224,7 @@ class _Join(torch.autograd.Function):
     def backward(ctx, dh, dy):
         if dh is None and dy is None:
             return (None,) * 10
+        _refuse_recording()
         cfg, need = ctx.cfg, ctx.needs_input_grad
         names = ("x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "state", "stats")
         con = [None if kept is None else _expect(t, *kept, name) for t, kept, name in zip(ctx.saved_tensors, ctx.kept, names)]
@@ -249,6 +261,7 @@ def _join_forward(cfg, x, branch, gate, aw, ab, bw, bb, state, stats):
 
 
 def _join(x, branch, branch_type, after, aw, ab, gate, skip_scale, branch_scale, p, state, site, before, bw, bb, eps):
+    _refuse_recording()
     _check_data(x, "x")
     if x.dim() == 0 or x.shape[-1] == 0:
         raise ValueError("x must have rows of at least one element")
