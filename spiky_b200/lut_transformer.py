@@ -190,8 +190,20 @@ class LUTTransformer(nn.Module):
         return block[part + "_join"](z, out, state, site)
 
     # ------------------------------------------------------------------ forward
-    def forward(self, tokens):
-        """tokens: int64 [B, context_size] -> logits fp32 [B, context_size, vocab_size]."""
+    def _drops(self):
+        """Whether a pass draws masks from the counter."""
+        return self.counter_dropout and self.training and self.dropout > 0.0
+
+    def take_dropout_state(self):
+        """The state of one training pass's counter dropouts, for ``forward``; None where nothing is dropped."""
+        return take_dropout_state(self.dropout_state, self._n_dropouts) if self._drops() else None
+
+    def forward(self, tokens, dropout_state=None):
+        """tokens: int64 [B, context_size] -> logits fp32 [B, context_size, vocab_size].
+
+        ``dropout_state``: what ``take_dropout_state`` returned, for a model that ``torch.utils.checkpoint`` runs again in the backward pass
+        (``checkpoint(model, tokens, model.take_dropout_state())``); by default the call takes its own.
+        """
         B, S, E = tokens.shape[0], self.context_size, self._n_embeddings
         record = self._debug_last_forward is not None
         if record:
@@ -200,9 +212,11 @@ class LUTTransformer(nn.Module):
         if record:
             self._debug_last_forward.append(z.detach().clone())
         flat = isinstance(self.embedding_dim, int)
+        if dropout_state is not None and not self.counter_dropout:
+            raise ValueError("dropout_state goes with counter_dropout")
         state = None   # of this pass's dropouts, each with a site of its own
-        if self.counter_dropout and self.training and self.dropout > 0.0:
-            state = take_dropout_state(self.dropout_state, self._n_dropouts)
+        if self._drops():
+            state = self.take_dropout_state() if dropout_state is None else dropout_state
         site = 0
         y = z if self.norm is None else self.first_norm(z)
         for block in self.layers:

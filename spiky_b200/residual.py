@@ -105,7 +105,14 @@ def dropout_state(seed, device, offset=0):
 
 
 def take_dropout_state(state, count):
-    """A copy of ``state`` for ``count`` dropouts (their sites 0 .. count - 1); the offset in ``state`` moves on by ``count``."""
+    """A copy of ``state`` for ``count`` dropouts (their sites 0 .. count - 1); the offset in ``state`` moves on by ``count``.
+
+    A part that ``torch.utils.checkpoint`` runs again in the backward pass has to be handed its copy from outside: one taken inside would be
+    another one the second time, with another mask.  Taking one during a backward pass is therefore an error.
+    """
+    if torch._C._current_graph_task_id() != -1:
+        raise RuntimeError("a dropout state is taken during a backward pass: take it outside the part that is run again (torch.utils.checkpoint) "
+                           "and hand it in, or the mask would be another one than the outputs were made with")
     used = (_calls or _native_calls()).take(state, count)
     if used is not None:
         return used
@@ -351,7 +358,11 @@ def residual_join(x, branch, *, branch_norm=None, branch_weight=None, branch_bia
 # ------------------------------------------------------------------------------------------------ modules
 class CounterDropout(nn.Module):
     """``nn.Dropout`` with a mask that is never stored.  ``state`` is a buffer: checkpoints carry it on, replayed graphs move it on.  Give
-    the replicas of a data-parallel model different seeds."""
+    the replicas of a data-parallel model different seeds.
+
+    A part that ``torch.utils.checkpoint`` runs again gets its state from outside: ``checkpoint(part, x, drop.take_state())`` with
+    ``drop(x, state)`` in it; without one the run in the backward pass raises.
+    """
 
     def __init__(self, p=0.5, seed=0, device=None):
         super().__init__()
@@ -360,10 +371,14 @@ class CounterDropout(nn.Module):
         self.p = float(p)
         self.register_buffer("state", dropout_state(seed, device))
 
-    def forward(self, x):
+    def take_state(self):
+        """The state of one call, which moves on; for ``forward``."""
+        return take_dropout_state(self.state, 1)
+
+    def forward(self, x, state=None):
         if not self.training or self.p == 0.0:
             return x
-        return counter_dropout(x, self.p, take_dropout_state(self.state, 1))
+        return counter_dropout(x, self.p, self.take_state() if state is None else state)
 
     def extra_repr(self):
         return f"p={self.p}"

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from test_residual_calls_gpu import routes  # noqa: F401
+from test_transformer_joins_gpu import model, tokens
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda:0"
@@ -43,3 +44,64 @@ def test_traces_are_refused(routes):  # noqa: F811
         assert torch.equal(none(2 * x.detach()), 2 * x)
 
     routes(traced)
+
+
+# ------------------------------------------------------------------------------------------------ recomputation
+@pytest.mark.parametrize("reentrant", [False, True])
+def test_checkpointed_dropout(routes, reentrant):  # noqa: F811
+    """A state from outside gives both runs one mask; a state taken inside would be another one the second time, which is refused."""
+    from spiky_b200 import residual
+    from torch.utils.checkpoint import checkpoint
+
+    def checkpointed():
+        drop = residual.CounterDropout(0.5, seed=3, device=DEV)
+        x = torch.randn(64, device=DEV, requires_grad=True)
+        for part in (drop, lambda v: residual.counter_dropout(v, 0.5, residual.take_dropout_state(drop.state, 1))):
+            y = checkpoint(part, x, use_reentrant=reentrant)
+            with pytest.raises(RuntimeError, match="outside the part that is run again"):
+                y.sum().backward()
+        drop.load_state_dict({"state": residual.dropout_state(3, "cpu")})
+        want = drop(x)
+        dwant, = torch.autograd.grad((want * want).sum(), x)
+        drop.load_state_dict({"state": residual.dropout_state(3, "cpu")})
+        x.grad = None
+        y = checkpoint(lambda v, s: drop(v, s) ** 2, x, drop.take_state(), use_reentrant=reentrant)
+        y.sum().backward()
+        assert torch.equal(y, want * want) and torch.equal(x.grad, dwant)
+        assert drop.state.tolist() == [3, 1]
+        assert torch.equal(drop.eval()(x, drop.take_state()), x)
+
+    routes(checkpointed)
+
+
+@pytest.mark.parametrize("opts", [dict(), dict(use_batch_norm=True), dict(norm="rms", gated=True)])
+def test_checkpointed_model(opts):
+    """A whole model run again in the backward pass (table gradients are summed by atomics)."""
+    from torch.utils.checkpoint import checkpoint
+
+    start = model(dropout=0.4, counter_dropout=True, **opts).state_dict()   # (a seed is that of anchors and embeddings, not of the tables)
+
+    def gradients(call):
+        m = model(dropout=0.4, counter_dropout=True, **opts).train()
+        m.load_state_dict(start)
+        params = [p for p in m.parameters() if p.requires_grad]
+        out = call(m)
+        dl = torch.randn(out.shape, generator=torch.Generator().manual_seed(3)).to(DEV)
+        out.backward(dl)
+        assert m.dropout_state.tolist() == [7, m._n_dropouts]
+        return out, [p.grad for p in params]
+
+    want, dwant = gradients(lambda m: m(tokens()))
+    got, dgot = gradients(lambda m: checkpoint(m, tokens(), m.take_dropout_state(), use_reentrant=False))
+    assert torch.equal(got, want)
+    for a, b in zip(dgot, dwant):
+        assert (a - b).abs().max() <= 1e-5 * b.abs().max() + 1e-12
+    m = model(dropout=0.4, counter_dropout=True, **opts).train()
+    out = checkpoint(m, tokens(), use_reentrant=False)
+    with pytest.raises(RuntimeError, match="outside the part that is run again"):
+        out.sum().backward()
+    m.eval()
+    state = m.train().take_dropout_state()
+    assert m.eval().take_dropout_state() is None and torch.equal(m(tokens(), state), m(tokens()))
+    with pytest.raises(ValueError, match="counter_dropout"):
+        model(dropout=0.4)(tokens(), state)
