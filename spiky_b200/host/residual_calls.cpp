@@ -111,6 +111,7 @@ struct ResidualNode : public torch::autograd::Node {
 // What a backward pass is handed can come from hooks: the kernels get nothing that is not what the forward pass had.
 void expect(const Tensor &t, at::ScalarType type, int64_t numel, c10::DeviceIndex device, const char *name) {
     TORCH_CHECK(plain_cuda(t, type, device) && t.numel() == numel, name, " is not what the forward pass saved: ", numel, " elements of ", type, " on cuda:", (int)device);
+    TORCH_CHECK(!t._fw_grad(0).defined(), name, " has a tangent: residual operators have no forward-mode derivatives");
 }
 // As residual.py's _refuse_recording.
 void refuse_recording() {

@@ -23,6 +23,7 @@ import sys
 import warnings
 
 import torch
+import torch.autograd.forward_ad as forward_ad
 import torch.nn as nn
 
 from . import _native
@@ -84,6 +85,11 @@ def _check_data(t, name, device=None):
         raise RuntimeError(f"{name} must be on {device}")
 
 
+def _check_tangent(t, name):
+    if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+        raise RuntimeError(f"{name} has a tangent: residual operators have no forward-mode derivatives")
+
+
 def _check_dropout(p, state, site, device):
     if not 0.0 <= p <= 1.0:
         raise ValueError(f"dropout probability has to be between 0 and 1, but got {p}")
@@ -139,6 +145,7 @@ def _expect(t, like, numel, name):
     dtype, device = like
     if not isinstance(t, torch.Tensor) or t.dtype != dtype or t.device != device or t.numel() != numel or t.layout != torch.strided:
         raise RuntimeError(f"{name} is not what the forward pass saved: {numel} elements of {dtype} on {device}")
+    _check_tangent(t, name)
     return _whole(t)
 
 
@@ -181,6 +188,7 @@ def counter_dropout(x, p, state, site=0):
     if p == 0.0:
         return x.clone()
     _refuse_recording()
+    _check_tangent(x, "x")
     if x.requires_grad and torch.is_grad_enabled():
         return _CounterDropout.apply(x, p, state, site)
     return _dropout(x, p, state, site)
@@ -311,6 +319,8 @@ def _join(x, branch, branch_type, after, aw, ab, gate, skip_scale, branch_scale,
                   skip_scale=skip_scale, branch_scale=branch_scale, reserved0=0)
     state = state if p > 0.0 else None
     tensors = (x, branch, gate, aw, ab, bw, bb)
+    for t, name in zip(tensors, ("x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "next_bias")):
+        _check_tangent(t, name)
     if rows == 0 and gate is not None:   # no gate row is read; its gradient is nothing, or zeros
         branch, gate = branch * gate.to(branch.dtype), None
         tensors = (x, branch, gate, aw, ab, bw, bb)

@@ -1,6 +1,7 @@
 """Residual-stream operators under what torch does around a call - traces, recomputation, forward mode, second derivatives - on both routes."""
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from test_residual_calls_gpu import routes  # noqa: F401
 from test_transformer_joins_gpu import model, tokens
@@ -105,3 +106,30 @@ def test_checkpointed_model(opts):
     assert m.eval().take_dropout_state() is None and torch.equal(m(tokens(), state), m(tokens()))
     with pytest.raises(ValueError, match="counter_dropout"):
         model(dropout=0.4)(tokens(), state)
+
+
+# ------------------------------------------------------------------------------------------------ forward mode
+def test_forward_mode_is_refused(routes):  # noqa: F811
+    """A tangent is not dropped in silence: dual inputs that want no gradient, dual parameters, dual gradients."""
+    from spiky_b200 import residual
+
+    def dual_calls():
+        x, w = torch.randn(3, 16, device=DEV), torch.ones(16, device=DEV)
+        with forward_ad.dual_level():
+            d, dw = forward_ad.make_dual(x, torch.ones_like(x)), forward_ad.make_dual(w, torch.ones_like(w))
+            calls = [lambda fn=fn: fn(d) for fn in operators(residual).values()]
+            calls += [lambda: residual.row_norm(x, dw), lambda: residual.row_norm(x, w, dw), lambda: residual.residual_join(x, d),
+                      lambda: residual.residual_join(x, x, gate=dw), lambda: residual.residual_join(x, x, gate=dw[:1]), lambda: residual.row_norm(d[:0]),
+                      lambda: residual.residual_join(x, x, branch_norm="rms", branch_weight=dw)]
+            for call in calls:
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    call()
+            assert torch.equal(forward_ad.unpack_dual(residual.counter_dropout(d, 0.0, None)).tangent, torch.ones_like(x))
+            assert residual.row_norm(x, w).shape == x.shape   # (a level without tangents is an ordinary one)
+            for fn in operators(residual).values():
+                z = x.clone().requires_grad_()
+                y = fn(z)
+                with pytest.raises(RuntimeError, match="forward-mode"):
+                    torch.autograd.grad(y, z, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
+
+    routes(dual_calls)
