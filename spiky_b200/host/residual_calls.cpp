@@ -214,13 +214,25 @@ struct JoinNode : public ResidualNode {
     c10::DeviceIndex device = 0;
     std::vector<int64_t> shape, gate_shape;
     std::string name() const override { return "_ResidualJoinBackward"; }
+    // Which tensors gradient k depends on, as residual.py's _sources; a bit each.
+    uint32_t sources(int k, bool next) const {
+        if (next) return k == BB ? 0 : (1u << BB) - 1;
+        const bool normed = cfg.after != LUTB_NORM_NONE;
+        switch (k) {
+            case F: return 1u << GATE | (normed ? 1u << F | 1u << AW : 0);
+            case GATE: return 1u << F | (normed ? 1u << AW | 1u << AB : 0);
+            case AW: return 1u << F | 1u << GATE;
+            case AB: return 1u << GATE;
+            default: return 0;
+        }
+    }
     variable_list apply(variable_list &&grads) override {
         std::vector<Tensor> s = unpack();   // the seven tensors, state, stats
         const Tensor dh = has_h ? settled(grads[0]) : Tensor(), dy = cfg.before != LUTB_NORM_NONE ? settled(grads[has_h ? 1 : 0]) : Tensor();
         variable_list out(TENSORS);
         if (!dh.defined() && !dy.defined()) return out;
         refuse_recording();
-        const bool again = needs_graph({&dh, &dy});
+        const std::vector<Tensor> given = at::GradMode::is_enabled() ? s : std::vector<Tensor>();   // (with the graph behind them)
         const int64_t all = cfg.rows * cfg.width;
         const int types[TENSORS] = {cfg.stream_type, cfg.branch_type, cfg.gate_type, cfg.param_type, cfg.param_type, cfg.param_type, cfg.param_type};
         static const char *const what[TENSORS] = {"x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "next_bias"};
@@ -256,11 +268,17 @@ struct JoinNode : public ResidualNode {
                                     pointer(out[F]), pointer(out[GATE]), pointer(out[AW]), pointer(out[AB]), pointer(out[BW]), pointer(out[BB]),
                                     pointer(ws), need, stream_on(device)));
         }
-        if (again) {   // a graph is asked for: one that says so when it is used
-            for (Tensor &o : out)
-                if (o.defined()) o.set_requires_grad(true);   // (the error hangs on what wants a gradient)
-            auto error = std::make_shared<torch::autograd::DelayedError>("a residual join is differentiable once", (int64_t)TENSORS);
-            return (*error)(std::move(out));
+        for (int k = 0; k < TENSORS && !given.empty(); k++) {   // a graph is asked for: one that says so when it is used
+            if (!out[k].defined()) continue;
+            std::vector<Tensor> of;
+            for (const Tensor *t : {&dh, &dy})
+                if (t->defined() && t->requires_grad()) of.push_back(*t);
+            for (int i = 0; i < BB; i++)
+                if ((sources(k, dy.defined()) >> i & 1) && given[i].defined() && given[i].requires_grad()) of.push_back(given[i]);
+            if (of.empty()) continue;
+            auto error = std::shared_ptr<torch::autograd::Error>(
+                new torch::autograd::Error("a residual join is differentiable once", torch::autograd::collect_next_edges(at::ArrayRef<Tensor>(of))), torch::autograd::deleteNode);
+            torch::autograd::set_history(out[k], error);
         }
         return out;
     }

@@ -217,6 +217,29 @@ def _gate_rows(gate, x):
     return math.prod(lead[k:])
 
 
+# Which saved tensors (of _Join.backward's names) the gradients of (x, branch, gate, branch_weight, branch_bias, next_weight, next_bias)
+# depend on, where the next norm has no gradient to hand on and where it has one; of the first, those in brackets with a norm of the branch alone.
+_SOURCES = (((), ()), ((2,), (1, 3)), ((1,), (3, 4)), ((1, 2), ()), ((2,), ()), ((), ()), ((), ()))
+
+
+def _sources(cfg, k, dy):
+    if dy is not None:
+        return range(6 if k < 6 else 0)
+    return _SOURCES[k][0] + (_SOURCES[k][1] if cfg.after != _native.NORM_NONE else ())
+
+
+class _Once(torch.autograd.Function):
+    """A gradient tied to what it was formed from, so that a second derivative raises instead of being left out."""
+
+    @staticmethod
+    def forward(ctx, grad, *sources):
+        return grad.detach()
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("a residual join is differentiable once")
+
+
 class _Join(torch.autograd.Function):
     @staticmethod
     def forward(ctx, cfg, x, branch, gate, aw, ab, bw, bb, state, stats):
@@ -235,14 +258,25 @@ class _Join(torch.autograd.Function):
         return h, y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dh, dy):
         if dh is None and dy is None:
             return (None,) * 10
         _refuse_recording()
+        saved = ctx.saved_tensors   # (once: hooks may run a part again for it)
+        with torch.no_grad():
+            grads = _Join.gradients(ctx, saved, dh, dy)
+        if torch.is_grad_enabled():   # a graph is asked for: one that says so when it is used
+            for k, grad in enumerate(grads):
+                of = [t for t in (dh, dy) + tuple(saved[i] for i in _sources(ctx.cfg, k, dy)) if t is not None and t.requires_grad]
+                if grad is not None and of:
+                    grads[k] = _Once.apply(grad, *of)
+        return (None, *grads, None, None)
+
+    @staticmethod
+    def gradients(ctx, saved, dh, dy):
         cfg, need = ctx.cfg, ctx.needs_input_grad
         names = ("x", "branch", "gate", "branch_weight", "branch_bias", "next_weight", "state", "stats")
-        con = [None if kept is None else _expect(t, *kept, name) for t, kept, name in zip(ctx.saved_tensors, ctx.kept, names)]
+        con = [None if kept is None else _expect(t, *kept, name) for t, kept, name in zip(saved, ctx.kept, names)]
         shape, _, device = ctx.had[0]
         dh, dy = (None if t is None else _expect(t, like, shape.numel(), "the gradient") for t, like in zip((dh, dy), ctx.of_grads))
 
@@ -261,7 +295,7 @@ class _Join(torch.autograd.Function):
             _native.check(L.lutb_join_backward(
                 ctypes.byref(cfg), *(_ptr(t) for t in con), _ptr(dh), _ptr(dy), _ptr(dx), _ptr(df),
                 _ptr(dgate), _ptr(daw), _ptr(dab), _ptr(dbw), _ptr(dbb), _ptr(ws), size, _stream(device)))
-        return None, dx, df, dgate, daw, dab, dbw, dbb, None, None
+        return [dx, df, dgate, daw, dab, dbw, dbb]
 
 
 def _join_forward(cfg, x, branch, gate, aw, ab, bw, bb, state, stats):

@@ -133,3 +133,56 @@ def test_forward_mode_is_refused(routes):  # noqa: F811
                     torch.autograd.grad(y, z, forward_ad.make_dual(torch.ones_like(y), torch.ones_like(y)))
 
     routes(dual_calls)
+
+
+# ------------------------------------------------------------------------------------------------ second derivatives
+def test_second_derivatives_are_not_left_out(routes):  # noqa: F811
+    """A penalty on a gradient raises, whether the incoming gradient wants one (y * y) or is a constant (a plain sum), whichever way it is asked."""
+    from spiky_b200 import residual
+    from torch.utils.checkpoint import checkpoint
+
+    def penalties():
+        def leaf(*shape):
+            return torch.randn(*shape, device=DEV, requires_grad=True)
+
+        def raises(loss, of):
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                torch.autograd.grad(loss, of, retain_graph=True)
+            with pytest.raises(RuntimeError, match="differentiable once"):
+                loss.backward()
+
+        x, f, gate, w, b = leaf(3, 16), leaf(3, 16), leaf(16), leaf(16), leaf(16)
+        for fn in (lambda: residual.row_norm(x, w, b), lambda: residual.residual_join(x, f, gate=gate, next_norm="layer", next_weight=w, next_bias=b)[1]):
+            for loss in (lambda y: y.sum(), lambda y: (y * y).sum()):
+                g, = torch.autograd.grad(loss(fn()), x, create_graph=True)
+                raises(x.sum() + (g * g).sum(), x)
+                g, = torch.autograd.grad(loss(fn()), w, create_graph=True)
+                raises(w.sum() + g.sum(), [w, x])
+        # a join without the next norm: what does not depend on an input stays an ordinary constant
+        h = residual.residual_join(x, f, branch_norm="rms", branch_weight=w, branch_bias=b, gate=gate, skip_scale=0.5)
+        for name, t, of in (("branch", f, f), ("branch by weight", f, w), ("branch by gate", f, gate), ("gate", gate, b), ("weight", w, gate), ("bias", b, gate)):
+            g, = torch.autograd.grad(h.sum(), t, create_graph=True)
+            raises(of.sum() + g.sum(), of)
+        g, = torch.autograd.grad(h.sum(), x, create_graph=True)
+        assert not g.requires_grad and torch.equal(g, torch.full_like(g, 0.5))
+        y = residual.row_norm(x, w, b)
+        g, = torch.autograd.grad(y.sum(), b, create_graph=True)
+        assert not g.requires_grad and torch.equal(g, torch.full_like(g, 3.0))
+        # the gradients themselves are those without a graph, and so is a sum of ordinary terms
+        up = torch.randn(3, 16, device=DEV)
+        plain = torch.autograd.grad(h, [x, f, gate, w, b], up, retain_graph=True)
+        graphed = torch.autograd.grad(h, [x, f, gate, w, b], up, create_graph=True)
+        assert all(torch.equal(p, g) for p, g in zip(plain, graphed))
+        x.grad = None
+        (x.sum() + residual.row_norm(x).sum()).backward(create_graph=True)
+        assert x.grad.requires_grad
+        x.grad = None
+        # a join that is run again, with a graph of its gradient
+        fn = lambda v: residual.residual_join(v, v * 2, branch_norm="rms", gate=gate[:1], next_norm="layer")[1]  # noqa: E731
+        g, = torch.autograd.grad(checkpoint(fn, x, use_reentrant=False), x, up, create_graph=True)
+        want, = torch.autograd.grad(fn(x), x, up)
+        assert torch.equal(g, want)
+        with pytest.raises(RuntimeError, match="differentiable once"):
+            torch.autograd.grad(g.sum(), x)
+
+    routes(penalties)
