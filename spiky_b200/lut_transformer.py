@@ -17,7 +17,7 @@ import torch.nn as nn
 
 from .lut_layer import (Conv2DLUTLayer, GradientPolicy, GradientType, LUTLayer, LUTSharedContext,  # noqa: F401
                         SynapseMeta, _normalise_device)
-from .residual import ResidualJoin, RowNorm, counter_dropout as _counter_dropout, dropout_state, take_dropout_state
+from .residual import ResidualJoin, RowNorm, counter_dropout as _counter_dropout, dropout_state, drawn_seed, take_dropout_state
 
 
 class LUTTransformer(nn.Module):
@@ -111,7 +111,7 @@ class LUTTransformer(nn.Module):
         self._n_dropouts = num_layers * (1 if no_ffn else 2)
         if counter_dropout:
             if dropout_seed is None:
-                dropout_seed = int(torch.randint(2 ** 62, (1,))) if seed is None else seed
+                dropout_seed = drawn_seed() if seed is None else seed
             self.register_buffer("dropout_state", dropout_state(dropout_seed, self.device))
         if norm is not None:
             self.first_norm = RowNorm(n_emb, norm, device=self.device)

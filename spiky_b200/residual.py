@@ -110,6 +110,11 @@ def dropout_state(seed, device, offset=0):
     return torch.tensor(wrap, dtype=torch.int64, device=device)
 
 
+def drawn_seed():
+    """A seed from torch's generator of the host."""
+    return int(torch.randint(2 ** 62, (1,), device="cpu"))
+
+
 def take_dropout_state(state, count):
     """A copy of ``state`` for ``count`` dropouts (their sites 0 .. count - 1); the offset in ``state`` moves on by ``count``.
 
@@ -401,19 +406,20 @@ def residual_join(x, branch, *, branch_norm=None, branch_weight=None, branch_bia
 
 # ------------------------------------------------------------------------------------------------ modules
 class CounterDropout(nn.Module):
-    """``nn.Dropout`` with a mask that is never stored.  ``state`` is a buffer: checkpoints carry it on, replayed graphs move it on.  Give
+    """``nn.Dropout`` with a mask that is never stored.  ``state`` is a buffer: checkpoints carry it on, replayed graphs move it on.  ``seed``: by
+    default drawn from torch's generator, so that two modules have different masks.  Give
     the replicas of a data-parallel model different seeds.
 
     A part that ``torch.utils.checkpoint`` runs again gets its state from outside: ``checkpoint(part, x, drop.take_state())`` with
     ``drop(x, state)`` in it; without one the run in the backward pass raises.
     """
 
-    def __init__(self, p=0.5, seed=0, device=None):
+    def __init__(self, p=0.5, seed=None, device=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability has to be between 0 and 1, but got {p}")
         self.p = float(p)
-        self.register_buffer("state", dropout_state(seed, device))
+        self.register_buffer("state", dropout_state(drawn_seed() if seed is None else seed, device))
 
     def take_state(self):
         """The state of one call, which moves on; for ``forward``."""
