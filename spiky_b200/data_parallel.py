@@ -61,7 +61,8 @@ def allreduce_gradients(params, group=None, average=False, bucket_bytes=256 << 2
 
 
 def broadcast_structure(module, src=0, group=None):
-    """Make every rank's replica identical to rank ``src``'s: parameters and buffers (anchors included)."""
+    """Make every rank's replica identical to rank ``src``'s: parameters and buffers (anchors included; the states of dropout
+    masks too, whose replicas are told apart by ``residual.replica_site``)."""
     if not dist.is_available() or not dist.is_initialized() or dist.get_world_size(group) == 1:
         return
     for t in list(module.parameters()) + list(module.buffers()):

@@ -9,20 +9,20 @@ vocabulary.  ``forward(tokens[B, S]) -> logits[B, S, V]``.
 Beyond the reference: ``norm`` ('rms' or 'layer') puts a norm of each token before every block and before the unembedder,
 ``norm_after`` one after every block, ``gated`` a learned gate row on every block's output, ``skip_scale`` and ``branch_scale`` scale the two
 parts of every residual sum, and ``counter_dropout`` draws the dropout masks from (``dropout_seed``, a buffer that counts training
-passes) instead of storing them.  Each block is then joined to the stream, with the next block's norm, in one kernel
-(:mod:`spiky_b200.residual`).
+passes) instead of storing them (``dropout_replica``: whose masks, by default those of the process's rank).  Each block is then joined to
+the stream, with the next block's norm, in one kernel (:mod:`spiky_b200.residual`).
 """
 import torch
 import torch.nn as nn
 
 from .lut_layer import (Conv2DLUTLayer, GradientPolicy, GradientType, LUTLayer, LUTSharedContext,  # noqa: F401
                         SynapseMeta, _normalise_device)
-from .residual import ResidualJoin, RowNorm, counter_dropout as _counter_dropout, dropout_state, drawn_seed, take_dropout_state
+from .residual import ResidualJoin, RowNorm, counter_dropout as _counter_dropout, dropout_state, drawn_seed, replica_site, take_dropout_state
 
 
 class LUTTransformer(nn.Module):
     # (of models that were pickled before these options)
-    norm, counter_dropout, _joined = None, False, False
+    norm, counter_dropout, _joined, dropout_replica = None, False, False, None
 
     def __init__(self, vocab_size, embedding_dim, context_size, positional_dim, num_layers, num_heads, n_detectors,
                  n_anchors_per_detector, n_anchors_per_detector_attention=None, no_ffn=False,
@@ -30,7 +30,7 @@ class LUTTransformer(nn.Module):
                  weights_gradient_policy=None, device=None, synapse_meta=SynapseMeta(), lut_shared_context=None,
                  seed=None, summation_dtype=torch.float32, _int_rescaler=0.001, _forward_group_size=32,
                  _backward_group_size=32, dropout=0.0, use_batch_norm=False, norm=None, norm_after=False, gated=False, skip_scale=1.0,
-                 branch_scale=1.0, counter_dropout=False, dropout_seed=None):
+                 branch_scale=1.0, counter_dropout=False, dropout_seed=None, dropout_replica=None):
         super().__init__()
         if norm not in (None, "rms", "layer"):
             raise ValueError("norm is None, 'rms' or 'layer'")
@@ -41,6 +41,10 @@ class LUTTransformer(nn.Module):
             raise ValueError("use_batch_norm goes without norm, gated, skip_scale and branch_scale")
         if dropout_seed is not None and not counter_dropout:
             raise ValueError("dropout_seed is the seed of counter_dropout")
+        if dropout_replica is not None:
+            if not counter_dropout:
+                raise ValueError("dropout_replica goes with counter_dropout")
+            replica_site(dropout_replica)   # (refuses)
         self.vocab_size = vocab_size
         self.embedding_dim = embedding_dim
         self.context_size = context_size
@@ -58,6 +62,7 @@ class LUTTransformer(nn.Module):
         self.dropout = dropout
         self.use_batch_norm = use_batch_norm
         self.norm, self.norm_after, self.gated, self.counter_dropout = norm, norm_after, gated, counter_dropout
+        self.dropout_replica = dropout_replica   # (None: the rank)
         self._joined = shaped or (counter_dropout and not use_batch_norm)
         self.unified_pe = unified_pe
         self.no_ffn = no_ffn
@@ -217,7 +222,7 @@ class LUTTransformer(nn.Module):
         state = None   # of this pass's dropouts, each with a site of its own
         if self._drops():
             state = self.take_dropout_state() if dropout_state is None else dropout_state
-        site = 0
+        site = replica_site(self.dropout_replica) if state is not None else 0
         y = z if self.norm is None else self.first_norm(z)
         for block in self.layers:
             att_in = y if flat else y.reshape((B, S) + tuple(self.embedding_dim))

@@ -115,6 +115,21 @@ def drawn_seed():
     return int(torch.randint(2 ** 62, (1,), device="cpu"))
 
 
+def replica_site(replica=None):
+    """The first site of a replica's dropouts: ``site = replica_site() + k`` gives data-parallel replicas masks of their own from one state.
+    ``replica``: a number below 2**15, by default the process's rank in torch.distributed's default group, 0 without one.
+
+    The state is a buffer, and buffers are made alike on all ranks (``broadcast_structure``, ``DistributedDataParallel``, a checkpoint that
+    all load): what tells replicas apart must not lie in it.  Replicas are 2**48 sites apart, more than any run's dropouts.
+    """
+    if replica is None:
+        dist = torch.distributed
+        replica = dist.get_rank() if dist.is_available() and dist.is_initialized() else 0
+    if not 0 <= replica < 2 ** 15:
+        raise ValueError("replica must be a number from 0 to 2**15 - 1")
+    return int(replica) << 48
+
+
 def take_dropout_state(state, count):
     """A copy of ``state`` for ``count`` dropouts (their sites 0 .. count - 1); the offset in ``state`` moves on by ``count``.
 
@@ -407,18 +422,22 @@ def residual_join(x, branch, *, branch_norm=None, branch_weight=None, branch_bia
 # ------------------------------------------------------------------------------------------------ modules
 class CounterDropout(nn.Module):
     """``nn.Dropout`` with a mask that is never stored.  ``state`` is a buffer: checkpoints carry it on, replayed graphs move it on.  ``seed``: by
-    default drawn from torch's generator, so that two modules have different masks.  Give
-    the replicas of a data-parallel model different seeds.
+    default drawn from torch's generator, so that two modules have different masks.  ``replica``: see ``replica_site``; by default each rank of a
+    data-parallel model has masks of its own, with one seed and one state.
 
     A part that ``torch.utils.checkpoint`` runs again gets its state from outside: ``checkpoint(part, x, drop.take_state())`` with
     ``drop(x, state)`` in it; without one the run in the backward pass raises.
     """
 
-    def __init__(self, p=0.5, seed=None, device=None):
+    replica = None   # (of modules that were pickled before it)
+
+    def __init__(self, p=0.5, seed=None, device=None, replica=None):
         super().__init__()
         if not 0.0 <= p <= 1.0:
             raise ValueError(f"dropout probability has to be between 0 and 1, but got {p}")
-        self.p = float(p)
+        if replica is not None:
+            replica_site(replica)   # (refuses)
+        self.p, self.replica = float(p), replica
         self.register_buffer("state", dropout_state(drawn_seed() if seed is None else seed, device))
 
     def take_state(self):
@@ -428,7 +447,7 @@ class CounterDropout(nn.Module):
     def forward(self, x, state=None):
         if not self.training or self.p == 0.0:
             return x
-        return counter_dropout(x, self.p, self.take_state() if state is None else state)
+        return counter_dropout(x, self.p, self.take_state() if state is None else state, replica_site(self.replica))
 
     def extra_repr(self):
         return f"p={self.p}"
@@ -466,7 +485,7 @@ class ResidualJoin(nn.Module):
     """``residual_join`` with its parameters: the norms' weights (and, by default for 'layer', biases) and a gate row.
 
     ``forward(x, branch, state, site)`` returns ``(h, y)``, ``y`` is ``h`` without ``next_norm``.  Dropout needs a ``state``
-    (``take_dropout_state``); it is off in evaluation mode.
+    (``take_dropout_state``) and, in a data-parallel model, sites from ``replica_site`` on; it is off in evaluation mode.
     """
 
     def __init__(self, width, branch_norm=None, next_norm=None, gated=False, gate_init=1.0, skip_scale=1.0, branch_scale=1.0, dropout=0.0,
