@@ -363,8 +363,8 @@ def _join(x, branch, branch_type, after, aw, ab, gate, skip_scale, branch_scale,
         _check_data(gate, "gate", device)
         if gate.dtype not in (torch.float32, branch_type):
             raise RuntimeError("gate must be float32 or of the branch's type")
-        if gate.numel() == 1 and width > 1:   # (a learned scalar: autograd sums its gradient)
-            gate = gate.reshape(1).expand(width)
+        if gate.numel() == 1:   # (a learned scalar: autograd sums the row of its gradient, in float32 up to the one rounding behind the cast)
+            gate = gate.float().reshape(1).expand(width)
         gate_rows = _gate_rows(gate, x)
     rows = x.numel() // width
     cfg = JoinCfg(rows=rows, width=width, gate_rows=gate_rows if rows else 0, site=site, dropout=p, stream_type=_TYPES[x.dtype],
