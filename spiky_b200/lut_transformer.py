@@ -186,8 +186,8 @@ class LUTTransformer(nn.Module):
         if not self._joined:
             dropout = block[part + "_dropout"]
             if self.counter_dropout:
-                def dropout(o):
-                    return o if state is None else _counter_dropout(o, self.dropout, state, site)
+                def dropout(o, training=dropout.training):
+                    return _counter_dropout(o, self.dropout, state, site) if training and self.dropout > 0.0 else o
             z = self._residual_branch(z, out, dropout, block[part + "_bn"])
             return z, z
         if not self.counter_dropout:
@@ -196,8 +196,12 @@ class LUTTransformer(nn.Module):
 
     # ------------------------------------------------------------------ forward
     def _drops(self):
-        """Whether a pass draws masks from the counter."""
-        return self.counter_dropout and self.training and self.dropout > 0.0
+        """Whether a pass draws masks from the counter: where what has a block's dropout - the join, or torch's module without one - is in training
+        mode, whatever the model's own mode is, as with torch's dropout."""
+        if not self.counter_dropout or self.dropout == 0.0:
+            return False
+        which = "_join" if self._joined else "_dropout"
+        return any(block[part + which].training for block in self.layers for part in (("attention",) if self.no_ffn else ("attention", "ffn")))
 
     def take_dropout_state(self):
         """The state of one training pass's counter dropouts, for ``forward``; None where nothing is dropped."""
