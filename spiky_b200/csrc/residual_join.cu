@@ -313,9 +313,6 @@ static auto by_types(const lutb_join_cfg *c, Fn fn) {
     return fn(float(), float());
 }
 
-// The kernels' own arrays at most, and what a block takes beside them.
-constexpr size_t kForwardStatic = 10 * 1024, kForwardVecStatic = 2 * 1024, kBackwardStatic = 13 * 1024, kBackwardTeamStatic = 4 * 1024;
-
 int resident_clusters(const void *kernel, const RowShape &s, size_t smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSmemPerBlock - kBackwardStatic) != cudaSuccess) {
         cudaGetLastError();

@@ -29,8 +29,8 @@ constexpr int kForwardCluster = 2, kBackwardCluster = 4;
 constexpr int64_t kRowMaxWidth = 16384;   // such clusters of 512 threads, of two groups forward and one backward, or 512 threads of four
 constexpr int64_t kRowMaxRows = 1 << 30;  // (row numbers of 32 bits)
 
-// BLOCK and WIDE: a block of up to 256 or 512 threads.  ANY: told at run time (backward, wide rows that are not VEC).
-enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_ANY = 4 };
+// BLOCK and WIDE: a block of up to 256 or 512 threads.  BLOCKS: WIDE or CLUSTER, told at run time (backward, rows that are not VEC).
+enum RowTeam { TEAM_WARP = 0, TEAM_BLOCK = 1, TEAM_WIDE = 2, TEAM_CLUSTER = 3, TEAM_BLOCKS = 4 };
 
 struct RowShape {
     int groups;                 // of a thread
@@ -212,10 +212,10 @@ __device__ __forceinline__ RowPlace row_place(const JoinArgs &a, const RowShape 
     RowPlace p;
     const int tid = threadIdx.x;
     p.team = s.team;
-    p.teams = TEAM == TEAM_WARP || TEAM == TEAM_ANY ? s.teams : 1;
-    p.which = p.teams == 1 ? 0 : tid / s.team;
+    p.teams = TEAM == TEAM_WARP ? s.teams : 1;
+    p.which = TEAM == TEAM_WARP ? tid / s.team : 0;
     p.t = tid - p.which * s.team;
-    p.cluster = TEAM == TEAM_CLUSTER || TEAM == TEAM_ANY ? s.cluster : 1;
+    p.cluster = TEAM == TEAM_CLUSTER || TEAM == TEAM_BLOCKS ? s.cluster : 1;
     p.rank = p.cluster > 1 ? (int)(blockIdx.x % p.cluster) : 0;
     p.first = p.rank * s.slice;
     p.limit = (int)min((int64_t)p.first + s.slice, a.width);
@@ -234,7 +234,7 @@ __device__ __forceinline__ RowPlace row_place(const JoinArgs &a, const RowShape 
                 if (row_column<VEC>(p, g, k) < p.limit) p.valid |= 1u << (g * 8 + k);
         }
     }
-    if (TEAM != TEAM_WARP && s.team > 32) {
+    if (TEAM != TEAM_WARP) {
         constexpr int kAll = sizeof(slots.a[0]) / sizeof(float), kWarps = Slots::kWarps;
         for (int k = tid; k < kAll; k += blockDim.x) slots.a[0][k] = slots.a[1][k] = slots.b[0][k] = slots.b[1][k] = 0.0f;
         constexpr int kCounts = sizeof(slots.count) / sizeof(float);
@@ -290,9 +290,7 @@ __device__ __forceinline__ void warp_sums(float &a, float &b) {
     b = upper ? v : other;
 }
 template <int TEAM>
-__device__ __forceinline__ bool within_warp(const RowPlace &p) { return TEAM == TEAM_WARP || (TEAM == TEAM_ANY && p.team <= 32); }
-template <int TEAM>
-__device__ __forceinline__ bool over_cluster(const RowPlace &p) { return TEAM == TEAM_CLUSTER || (TEAM == TEAM_ANY && p.cluster > 1); }
+__device__ __forceinline__ bool over_cluster(const RowPlace &p) { return TEAM == TEAM_CLUSTER || (TEAM == TEAM_BLOCKS && p.cluster > 1); }
 
 static __device__ int g_join_wait_errors;   // bounded waits that ran out (lutb_device_wait_errors)
 
@@ -379,7 +377,7 @@ __device__ __forceinline__ float all_slots(const RowPlace &p, const float *from)
 // Sums of two values over the row; `between` runs while the others arrive.
 template <int TEAM, class Slots, class Fn>
 __device__ __forceinline__ float2 row_sums(RowPlace &p, Slots &slots, float a, float b, bool second, Fn between) {
-    if (within_warp<TEAM>(p)) {
+    if (TEAM == TEAM_WARP) {
         a = team_sum(a, p.team);
         if (second) b = team_sum(b, p.team);
         between();
@@ -448,7 +446,7 @@ __device__ __forceinline__ float2 row_stats(RowPlace &p, Slots &slots, const flo
         }
         return s.x + s.y;
     };
-    if (within_warp<TEAM>(p)) {
+    if (TEAM == TEAM_WARP) {
         const float mean = layer ? team_sum(sum(), p.team) / p.width : 0.0f;
         return make_float2(mean, rsqrtf(team_sum(squares(mean), p.team) * p.inverse + eps));
     }
@@ -558,8 +556,8 @@ struct RowCursor {
 };
 
 template <int TEAM>
-__device__ __forceinline__ void team_barrier(const RowPlace &p) {
-    if (within_warp<TEAM>(p))
+__device__ __forceinline__ void team_barrier() {
+    if (TEAM == TEAM_WARP)
         __syncwarp();
     else
         __syncthreads();
@@ -636,7 +634,7 @@ struct RowRing {
         fill = fill + stage_bytes == stages * stage_bytes ? 0 : fill + stage_bytes;
     }
     // The current row's elements are there, for the team; what was read of the row before may be overwritten.
-    __device__ __forceinline__ void ready(const RowPlace &p) const {
+    __device__ __forceinline__ void ready() const {
         if (stages == 3)
             asm volatile("cp.async.wait_group 1;" ::: "memory");
         else
@@ -644,7 +642,7 @@ struct RowRing {
         if (VEC)
             __syncwarp();
         else
-            team_barrier<TEAM>(p);
+            team_barrier<TEAM>();
     }
     __device__ __forceinline__ void taken() { take = take + stage_bytes == stages * stage_bytes ? 0 : take + stage_bytes; }
     // Eight elements; where there are none: 0, in VEC rows those of another group or row.
@@ -711,6 +709,9 @@ __device__ __forceinline__ uint32_t read_masks(const RowPlace &p, const JoinArgs
 template <int G, int THREADS>
 constexpr size_t kMaskBytes = 2 * (G * THREADS + THREADS);   // two sets, a byte a group and one more a team
 
+// The kernels' own arrays at most (5456, 656, 9216 and 3344 bytes), and what a block takes beside them: what launches count with.
+constexpr size_t kForwardStatic = 10 * 1024, kForwardVecStatic = 2 * 1024, kBackwardStatic = 13 * 1024, kBackwardTeamStatic = 4 * 1024;
+
 // ------------------------------------------------------------------------------------------------ forward
 // BRANCH: 0 no branch (the norm alone), 1 a branch, 2 a branch with a norm of its own.  NEXT: the norm before the next block.
 // The parameters that a forward kernel keeps in shared memory.
@@ -732,6 +733,7 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, kForwardBlocks<BRANCH, G,
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) RowSlots<TEAM == TEAM_WARP ? 4 : kThreads / 32, TEAM == TEAM_CLUSTER ? kForwardCluster : 1> slots;
     __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<G, kThreads>];
+    static_assert(sizeof(slots) + sizeof(masks) <= (VEC ? kForwardVecStatic : kForwardStatic));
     RowPlace p = row_place<VEC, G, TEAM>(a, shape, slots);
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
     const bool gate_each = BRANCH && a.gate_rows == 1, gate_f32 = sizeof(F) == 4 || a.gate_f32;
@@ -828,10 +830,10 @@ __global__ void __launch_bounds__(kThreadsOf<G, TEAM>, kForwardBlocks<BRANCH, G,
         const bool drop = BRANCH && a.drop.on;
         if (!VEC && drop) form_masks<G>(p, a, key, row, masks, set);
         if (shape.stages == 1) {
-            team_barrier<TEAM>(p);
+            team_barrier<TEAM>();
             fetch();
         }
-        ring.ready(p);
+        ring.ready();
         uint32_t kept = 0;
         if (!VEC && drop) kept = read_masks<G>(p, a, row, masks, set);
         set ^= 1;
@@ -946,11 +948,12 @@ constexpr int kBackwardThreads = TEAM == TEAM_WARP || TEAM == TEAM_BLOCK ? kBloc
 template <class X, class F, int BRANCH, bool NEXT, bool VEC, int TEAM>
 __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads<TEAM>) join_rows_backward_kernel(const JoinArgs a, const RowShape shape) {
     constexpr int kThreads = kBackwardThreads<TEAM>;
-    constexpr bool kTeams = TEAM == TEAM_WARP || TEAM == TEAM_ANY, kClusters = TEAM == TEAM_CLUSTER || TEAM == TEAM_ANY;
+    constexpr bool kTeams = TEAM == TEAM_WARP, kClusters = TEAM == TEAM_CLUSTER || TEAM == TEAM_BLOCKS;
     extern __shared__ __align__(16) unsigned char dynamic[];
     __shared__ __align__(16) RowSlots<kThreads / 32, kClusters ? kBackwardCluster : 1> slots;
     __shared__ uint8_t masks[VEC ? 1 : kMaskBytes<1, kThreads>];
     __shared__ float2 joined[kTeams ? 4 * kBlockThreads : 1];   // the teams' sums of a block
+    static_assert(sizeof(slots) + sizeof(masks) + sizeof(joined) <= (TEAM == TEAM_WARP ? kBackwardStatic : kBackwardTeamStatic));
     RowPlace p = row_place<VEC, 1, TEAM>(a, shape, slots);
     const int threads = blockDim.x, tid = threadIdx.x;
     const DropKey key = BRANCH && a.drop.on ? drop_key(a.random, a.site) : DropKey{};
@@ -1027,7 +1030,7 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
     for (int s = 0; s < kSums; s++) zero8(sums[s]);
     // this thread's sum of eight columns, joined over the block's teams, handed on column by column
     auto hand_out = [&](const float2 *v, auto put) {
-        if (!kTeams || p.teams == 1) {
+        if (!kTeams) {
 #pragma unroll
             for (int k = 0; k < 8; k++)
                 if (row_valid<VEC>(p, 0, k)) put(row_column<VEC>(p, 0, k), k & 1 ? v[k >> 1].y : v[k >> 1].x);
@@ -1077,10 +1080,10 @@ __global__ void __launch_bounds__(kBackwardThreads<TEAM>, 512 / kBackwardThreads
                 form_masks<1>(p, a, key, row, masks, set);
         }
         if (shape.stages == 1) {
-            team_barrier<TEAM>(p);
+            team_barrier<TEAM>();
             fetch();
         }
-        ring.ready(p);
+        ring.ready();
         if (!VEC && BRANCH && a.drop.on) kept = read_masks<1>(p, a, row, masks, set);
         set ^= 1;
         if (shape.stages > 1) fetch();
@@ -1256,7 +1259,7 @@ const void *join_rows_kernel(bool backward, bool vec, const RowShape &s) {
 #define LUTB_FORWARD(VEC, G, TEAM) reinterpret_cast<const void *>(&join_rows_forward_kernel<X, F, BRANCH, NEXT, VEC, G, TEAM>)
 #define LUTB_BACKWARD(VEC, TEAM) reinterpret_cast<const void *>(&join_rows_backward_kernel<X, F, BRANCH, NEXT, VEC, TEAM>)
     if (backward) {
-        if (!vec) return s.kind == TEAM_WARP ? LUTB_BACKWARD(false, TEAM_WARP) : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(false, TEAM_BLOCK) : LUTB_BACKWARD(false, TEAM_ANY);
+        if (!vec) return s.kind == TEAM_WARP ? LUTB_BACKWARD(false, TEAM_WARP) : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(false, TEAM_BLOCK) : LUTB_BACKWARD(false, TEAM_BLOCKS);
         return s.kind == TEAM_WARP    ? LUTB_BACKWARD(true, TEAM_WARP)
                : s.kind == TEAM_BLOCK ? LUTB_BACKWARD(true, TEAM_BLOCK)
                : s.kind == TEAM_WIDE  ? LUTB_BACKWARD(true, TEAM_WIDE)
