@@ -12,8 +12,9 @@
 // warp reads and stores neighbours, and the mask's bytes go through shared memory too.
 //
 // Bound: the memory at 4-byte types (32768 x 1024 fp32 with both norms, gate and dropout: forward 93 us, 5.8 TB/s, backward 145 us, 5.6 TB/s),
-// instruction issue at 2-byte ones (bf16: 69 us, 3.9 TB/s, and 125 us, 3.2 TB/s: some 290 instructions for a warp's 256 elements forward and 560
-// backward, 110 of them the generator and its mask; 16 warps an SM, as registers allow, issue 2.1 to 2.3 a cycle).
+// latency at 2-byte ones, whose instructions are nearly as many for half the bytes (bf16: 68 us, 3.9 TB/s, and 126 us, 3.2 TB/s: some 290
+// for a warp's 256 elements forward and 560 backward, 110 of them the generator and its mask; the 16 warps an SM that registers allow issue
+// 2.1 to 2.3 a cycle of the four that an SM can, waiting for loads, shared memory and results of fixed latency).
 #pragma once
 
 #include <atomic>

@@ -14,8 +14,8 @@ float32, bfloat16 and float16; a float32 stream may carry a 16-bit branch.  Sums
 output is rounded once.  ``CounterDropout``, ``RowNorm`` and ``ResidualJoin`` are the modules; ``LUTTransformer`` uses them.  Ordinary calls run through
 the native host side (host/residual_calls.cpp); the functions here define them all and take the rest.
 
-Argument mistakes raise ``ValueError``, mistakes of type or device ``RuntimeError``; there is no CPU path.  Tensors that are not
-contiguous are copied.  Work goes to torch's current stream of the tensors' device.
+Argument mistakes raise ``ValueError``, mistakes of type or device ``RuntimeError``; there is no CPU path.  Traces, forward-mode
+derivatives and second derivatives of joins raise too: none is left out in silence.  Tensors that are not contiguous are copied.  Work goes to torch's current stream of the tensors' device.
 """
 import ctypes
 import math
