@@ -61,7 +61,7 @@ def _ptr(t):
 
 
 def _stream(device):
-    return torch.cuda.current_stream(device).cuda_stream
+    return torch._C._cuda_getCurrentRawStream(device.index)   # (a stream's object has no such number under torch.compile)
 
 
 def _refuse_recording():

@@ -186,3 +186,32 @@ def test_second_derivatives_are_not_left_out(routes):  # noqa: F811
             torch.autograd.grad(g.sum(), x)
 
     routes(penalties)
+
+
+# ------------------------------------------------------------------------------------------------ compiled functions
+@pytest.mark.parametrize("backend", ["eager", "aot_eager"])
+def test_calls_in_compiled_functions(routes, backend):  # noqa: F811
+    """torch.compile runs the calls between its graphs, on either route, on the stream that is current when they run."""
+    from spiky_b200 import residual
+
+    def compiled():
+        gate, state = torch.full((1,), 0.5, device=DEV), residual.dropout_state(1, DEV)
+        calls = [lambda v: residual.residual_join(v, v * 2, gate=gate) * 2, lambda v: residual.residual_join(v, v, next_norm="rms")[1] + v,
+                 lambda v: residual.counter_dropout(v, 0.5, state) + v, lambda v: residual.row_norm(v) * v]
+        for fn in calls:
+            torch._dynamo.reset()
+            x = torch.randn(5, 16, device=DEV)
+            quick = torch.compile(fn, backend=backend)
+            assert torch.equal(quick(x), fn(x))
+            z = x.clone().requires_grad_()
+            got, want = (torch.autograd.grad(f(z).sum(), z)[0] for f in (quick, fn))
+            assert torch.equal(got, want)
+            graph = torch.cuda.CUDAGraph()
+            with torch.no_grad(), torch.cuda.graph(graph):
+                out = quick(x)
+            x.normal_()
+            graph.replay()
+            assert torch.equal(out, fn(x))
+
+    routes(compiled)
+    torch._dynamo.reset()
