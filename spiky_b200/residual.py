@@ -15,7 +15,8 @@ output is rounded once.  ``CounterDropout``, ``RowNorm`` and ``ResidualJoin`` ar
 the native host side (host/residual_calls.cpp); the functions here define them all and take the rest.
 
 Argument mistakes raise ``ValueError``, mistakes of type or device ``RuntimeError``; there is no CPU path.  Traces, forward-mode
-derivatives and second derivatives of joins raise too: none is left out in silence.  Tensors that are not contiguous are copied.  Work goes to torch's current stream of the tensors' device.
+derivatives and second derivatives of joins raise too: none is left out in silence.  Tensors that are not contiguous are copied.
+Work goes to torch's current stream of the tensors' device.
 """
 import ctypes
 import math
